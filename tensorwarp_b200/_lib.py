@@ -13,7 +13,7 @@ PKG = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("TWMARLIN_LIB", os.path.join(PKG, "libtwmarlin.so"))
 
 TWM_OK, TWM_EINVAL, TWM_EALIGN, TWM_EWORKSPACE, TWM_ELAUNCH, TWM_EARCH, TWM_ETIMEOUT = 0, -1, -2, -3, -4, -5, -6
-TWM_F32, TWM_F16 = 0, 1
+TWM_F32, TWM_F16, TWM_BF16 = 0, 1, 2
 TWM_KERNEL_AUTO, TWM_KERNEL_SIMT, TWM_KERNEL_TC, TWM_KERNEL_MMA, TWM_KERNEL_TCW, TWM_KERNEL_TCR = 0, 1, 2, 3, 4, 5
 TWM_FLAG_PDL, TWM_FLAG_ACCUMULATE, TWM_FLAG_INDEPENDENT = 1, 2, 4
 TWM_A_PLAIN, TWM_A_SILU_MUL, TWM_A_GEGLU = 0, 1, 2
@@ -59,6 +59,21 @@ class MoeArgs(C.Structure):
                 ("topk_ids", C.c_void_p), ("topk_weights", C.c_void_p),
                 ("c", C.c_void_p), ("c_dtype", C.c_int), ("c_slot_stride", C.c_long),
                 ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t), ("flags", C.c_int)]
+
+
+class Cache8(C.Structure):
+    """``twm_cache8``."""
+    _fields_ = [("seqs", C.c_int), ("kv_heads", C.c_int), ("head_dim", C.c_int), ("capacity", C.c_int),
+                ("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
+                ("k_tail", C.c_void_p), ("v_tail", C.c_void_p)]
+
+
+class SampleArgs(C.Structure):
+    """``twm_sample_args``."""
+    _fields_ = [("rows", C.c_int), ("vocab", C.c_int), ("dtype", C.c_int), ("logits", C.c_void_p), ("ld", C.c_long),
+                ("random", C.c_void_p), ("temperature", C.c_void_p), ("top_k", C.c_void_p), ("top_p", C.c_void_p), ("min_p", C.c_void_p),
+                ("tokens", C.c_void_p), ("prob", C.c_void_p), ("step", C.c_void_p), ("random_count", C.c_int), ("history", C.c_void_p),
+                ("history_capacity", C.c_int), ("pos", C.c_void_p), ("len", C.c_void_p)]
 
 
 class ChainOp(C.Structure):
@@ -133,6 +148,13 @@ SIGNATURES = {
     "twm_argmax_scratch_bytes": (C.c_size_t, []),
     "twm_argmax_advance": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int,
                                      C.c_void_p, C.c_size_t, C.c_int, C.c_void_p]),
+    # include/twm_serve.h (a twm_cache8 by address)
+    "twm_cache8_append": (C.c_int, [C.c_void_p, C.c_void_p, C.c_long, C.c_void_p, C.c_long, C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_void_p,
+                                    C.c_int, C.c_void_p, C.c_int, C.c_void_p]),
+    "twm_cache8_attention_bytes": (C.c_size_t, [C.c_void_p, C.c_int, C.c_int]),
+    "twm_cache8_attention": (C.c_int, [C.c_void_p, C.c_void_p, C.c_long, C.c_void_p, C.c_long, C.c_int, C.c_int, C.c_void_p, C.c_int, C.c_void_p,
+                                       C.c_float, C.c_int, C.c_void_p, C.c_size_t, C.c_int, C.c_void_p]),
+    "twm_sample": (C.c_int, [C.POINTER(SampleArgs), C.c_int, C.c_void_p]),
     "twm_status_string": (C.c_char_p, [C.c_int]),
     "twm_last_error": (C.c_char_p, []),
     "twm_version": (C.c_char_p, []),

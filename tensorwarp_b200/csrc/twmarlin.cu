@@ -1729,3 +1729,5 @@ const char* twm_last_error(void) { return t_last_error; }
 const char* twm_version(void) { return "twmarlin 0.1 sm_100a"; }
 
 }  // extern "C"
+
+#include "twm_serve.cuh"         // its checks and launches use what is above

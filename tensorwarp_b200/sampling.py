@@ -1,0 +1,63 @@
+"""Sampling from logits: temperature, top-k, top-p and min-p, from given random numbers (``twm_sample``, ``include/twm_serve.h``)."""
+from __future__ import annotations
+
+import math
+from dataclasses import dataclass
+from typing import Optional
+
+import torch
+
+from . import _lib
+from ._lib import TwmError, check
+from .cache8 import _on
+from .quantize import _require_cuda, _stream_ptr
+
+_DTYPES = {torch.float32: _lib.TWM_F32, torch.float16: _lib.TWM_F16, torch.bfloat16: _lib.TWM_BF16}
+
+
+@dataclass
+class SamplingParams:
+    """How a request's tokens are chosen.  temperature 0: greedily; top_k 0, top_p 1 and min_p 0 leave that cut out."""
+    temperature: float = 1.0
+    top_k: int = 0
+    top_p: float = 1.0
+    min_p: float = 0.0
+    seed: int = 0
+
+    def __post_init__(self):
+        if not (math.isfinite(self.temperature) and self.temperature >= 0):
+            raise ValueError("temperature must be finite and not negative")
+        if self.top_k < 0 or not 0 < self.top_p <= 1 or not 0 <= self.min_p <= 1:
+            raise ValueError("top_k must not be negative, top_p in (0, 1] and min_p in [0, 1]")
+
+
+def _column(name: str, t: Optional[torch.Tensor], dtype: torch.dtype, rows: int, device: torch.device) -> Optional[int]:
+    if t is None:
+        return None
+    if t.dtype is not dtype or t.numel() != rows or not t.is_contiguous() or t.device != device:
+        if not t.is_cuda:
+            _require_cuda(t)
+        raise TwmError(_lib.TWM_EINVAL, f"sample: {name} must be {dtype} [{rows}] on {device}")
+    return t.data_ptr()
+
+
+def sample(logits: torch.Tensor, random: torch.Tensor, tokens: torch.Tensor, *, temperature: Optional[torch.Tensor] = None,
+           top_k: Optional[torch.Tensor] = None, top_p: Optional[torch.Tensor] = None, min_p: Optional[torch.Tensor] = None,
+           prob: Optional[torch.Tensor] = None, stream: Optional[torch.cuda.Stream] = None, flags: int = 0) -> None:
+    """tokens int32 [rows]: one of each row of logits (f32, f16 or bf16 [rows, vocab]), chosen by random f32 [rows] in [0, 1).
+    temperature, top_p, min_p f32 [rows] and top_k int32 [rows], None to leave one out (1 for the temperature); prob f32 [rows]
+    gets what the kept tokens' distribution gave the token.  ``include/twm_serve.h`` has the definition."""
+    if not logits.is_cuda:
+        _require_cuda(logits)
+    dtype = _DTYPES.get(logits.dtype)
+    if dtype is None or logits.dim() != 2 or logits.stride(1) != 1:
+        raise TwmError(_lib.TWM_EINVAL, "sample: logits must be a float32, float16 or bfloat16 matrix with contiguous rows")
+    (rows, vocab), device, f32, i32 = logits.shape, logits.device, torch.float32, torch.int32
+    if rows == 0:
+        return
+    args = _lib.SampleArgs(rows, vocab, dtype, logits.data_ptr(), logits.stride(0) if rows > 1 else vocab, _column("random", random, f32, rows, device),
+                           _column("temperature", temperature, f32, rows, device), _column("top_k", top_k, i32, rows, device),
+                           _column("top_p", top_p, f32, rows, device), _column("min_p", min_p, f32, rows, device),
+                           _column("tokens", tokens, i32, rows, device), _column("prob", prob, f32, rows, device))
+    with _on(device):
+        check(_lib.lib().twm_sample(args, flags, _stream_ptr(stream)), "twm_sample")

@@ -1,0 +1,93 @@
+"""CPU tests of what the cache held in 8 bits and sampling refuse; nothing here makes a CUDA call."""
+import ctypes as C
+
+import pytest
+import torch
+
+from tensorwarp_b200 import _lib, cache8, sampling
+
+
+def cache(**kw):
+    fields = dict(seqs=2, kv_heads=4, head_dim=128, capacity=256, k=0x10000, v=0x20000, k_scale=0x30000, v_scale=0x40000, k_tail=0x50000, v_tail=0x60000)
+    fields.update(kw)
+    return _lib.Cache8(**fields)
+
+
+def append(lib, c, q=0x1000, ldq=1024, qkv=0x2000, ldqkv=2048, bias=None, rope=None, heads=8, rows=2, row_start=None, max_rows=1, start=0x3000):
+    return lib.twm_cache8_append(C.addressof(c) if c is not None else None, q, ldq, qkv, ldqkv, bias, rope, heads, rows, row_start, max_rows, start, 0, None)
+
+
+def attention(lib, c, out=0x1000, ldo=1024, q=0x2000, ldq=1024, heads=8, rows=2, row_start=None, max_rows=1, start=0x3000, scale=0.1, window=0, ws=0x4000,
+              nbytes=1 << 40):
+    return lib.twm_cache8_attention(C.addressof(c) if c is not None else None, out, ldo, q, ldq, heads, rows, row_start, max_rows, start, scale, window, ws,
+                                    nbytes, 0, None)
+
+
+BAD_CACHES = [dict(seqs=0), dict(seqs=65536), dict(kv_heads=0), dict(head_dim=96), dict(head_dim=0), dict(capacity=100), dict(capacity=0), dict(k=None), dict(v=None),
+              dict(k_scale=None), dict(v_scale=None), dict(k_tail=None), dict(v_tail=None), dict(seqs=60000, capacity=1 << 20)]
+
+
+@pytest.mark.parametrize("call", [append, attention])
+def test_caches_that_are_refused(twm_lib, call):
+    assert call(twm_lib, None) == _lib.TWM_EINVAL
+    for bad in BAD_CACHES:
+        assert call(twm_lib, cache(**bad)) == _lib.TWM_EINVAL, bad
+    for bad in (dict(k=0x10008), dict(v=0x20004), dict(k_tail=0x50002), dict(v_tail=0x60008)):
+        assert call(twm_lib, cache(**bad)) == _lib.TWM_EALIGN, bad
+
+
+@pytest.mark.parametrize("call", [append, attention])
+def test_rows_that_are_refused(twm_lib, call):
+    for bad in (dict(heads=0), dict(heads=6), dict(rows=0), dict(rows=3), dict(max_rows=0), dict(max_rows=2), dict(start=None), dict(q=None), dict(ldq=1016),
+                dict(row_start=0x5000, rows=4, max_rows=5)):
+        assert call(twm_lib, cache(), **bad) == _lib.TWM_EINVAL, bad
+    for bad in (dict(ldq=1025), dict(q=0x1008)):
+        assert call(twm_lib, cache(), **bad) == _lib.TWM_EALIGN, bad
+
+
+def test_other_refusals(twm_lib):
+    for bad in (dict(qkv=None), dict(ldqkv=2040)):
+        assert append(twm_lib, cache(), **bad) == _lib.TWM_EINVAL, bad
+    for bad in (dict(qkv=0x2002), dict(ldqkv=2052), dict(bias=0x7004), dict(rope=0x7008)):
+        assert append(twm_lib, cache(), **bad) == _lib.TWM_EALIGN, bad
+    for bad in (dict(out=None), dict(ldo=1000), dict(scale=0.0), dict(scale=-1.0), dict(scale=float("nan")), dict(window=-1), dict(ws=None)):
+        assert attention(twm_lib, cache(), **bad) == _lib.TWM_EINVAL, bad
+    for bad in (dict(out=0x1001), dict(ldo=1028), dict(ws=0x4008)):
+        assert attention(twm_lib, cache(), **bad) == _lib.TWM_EALIGN, bad
+    assert attention(twm_lib, cache(), nbytes=8) == _lib.TWM_EWORKSPACE
+
+
+def test_workspace_sizes(twm_lib):
+    size = lambda c, heads, rows: twm_lib.twm_cache8_attention_bytes(C.addressof(c), heads, rows)  # noqa: E731
+    assert twm_lib.twm_cache8_attention_bytes(None, 8, 1) == 0 and size(cache(), 0, 1) == 0 and size(cache(), 8, 0) == 0 and size(cache(head_dim=80), 8, 1) == 0
+    assert size(cache(), 8, 1) > 0
+
+
+def sample_args(**kw):
+    fields = dict(rows=1, vocab=100, dtype=_lib.TWM_F32, logits=0x1000, ld=100, random=0x2000, tokens=0x3000)
+    fields.update(kw)
+    return _lib.SampleArgs(**fields)
+
+
+def test_sampling_that_is_refused(twm_lib):
+    assert twm_lib.twm_sample(None, 0, None) == _lib.TWM_EINVAL
+    loop = dict(step=0x4000, random_count=3, pos=0x5000, len=0x6000)
+    for bad in (dict(rows=0), dict(vocab=0), dict(dtype=3), dict(logits=None), dict(ld=99), dict(random=None), dict(tokens=None),
+                dict(loop, rows=2), dict(loop, random_count=0), dict(loop, pos=None), dict(loop, len=None), dict(loop, history=0x7000, history_capacity=0)):
+        assert twm_lib.twm_sample(sample_args(**bad), 0, None) == _lib.TWM_EINVAL, bad
+    assert twm_lib.twm_sample(sample_args(logits=0x1002), 0, None) == _lib.TWM_EALIGN
+
+
+def test_host_tensors_are_refused():
+    with pytest.raises(_lib.TwmError):
+        sampling.sample(torch.zeros(1, 8), torch.zeros(1), torch.zeros(1, dtype=torch.int32))
+    with pytest.raises(_lib.TwmError):
+        cache8.Cache8.empty(1, 64, 1, 64, device="cpu")
+
+
+def test_sampling_params():
+    sampling.SamplingParams(temperature=0.0, top_k=3, top_p=0.5, min_p=0.1)
+    for bad in (dict(temperature=-1.0), dict(temperature=float("inf")), dict(temperature=float("nan")), dict(top_k=-1), dict(top_p=0.0), dict(top_p=1.5),
+                dict(min_p=-0.1), dict(min_p=1.1)):
+        with pytest.raises(ValueError):
+            sampling.SamplingParams(**bad)
