@@ -1,10 +1,23 @@
-// twm_cache8_attn.cuh — softmax attention over the cache held in 8 bits.
+// twm_cache8_attn.cuh — softmax attention over the cache held in 8 bits: how the work is dealt out, attention of few rows a sequence, and
+// the merge of what several CTAs have of a tile.
+//
+// Mathematics, common to all kernels.  Keys are c_k 2^ek and values c_v 2^ev with one ek and ev a block of 64 tokens (0 in the tail, whose
+// tokens are FP16).  The codes enter the tensor core as FP16, exactly.  The exponent of key j for a row is
+//     x_j = (q . c_k) (scale 2^ek log2 e) + ev,
+// so that 2^x_j is the factor of the CODES c_v in the output, and 2^(x_j - ev) the weight that belongs into the sum of weights:
+//     o = sum 2^(x_j - m) c_v / sum 2^(x_j - m) 2^-ev.
+// One fused multiply-add an element as without scales, and since the running reference m is that of x_j, scale of the value
+// included, the largest FP16 factor of a row is near 1 however the scales of its blocks differ.  m moves only when a factor would pass 2^8.
+// A factor is rounded to FP16 (2^-11 of itself): the values' codes have four bits, and sums, scores and statistics are FP32.
 #pragma once
 
 #include "twm_cache8.cuh"
+#include "twm_gemm_tc.cuh"
 
 namespace twm {
 namespace cache8 {
+
+constexpr float LOG2E = 1.4426950408889634f;
 
 struct AttnArgs {
     Cache c;
@@ -14,54 +27,579 @@ struct AttnArgs {
     long ldo, ldq;
     int num_heads, window;       // window: INT_MAX = all
     float scale;
+    float* partial;              // [2 CTAs][tile]: what a CTA has of its first and of its last tile, where others have the rest
+    alignas(64) CUtensorMap k_map, v_map;        // bytes [cached rows][D], boxes of a block, swizzled
 };
 
-__device__ __forceinline__ float code_value(uint8_t code) { return __half2float(__half(__nv_cvt_fp8_to_halfraw(code, __NV_E4M3))); }
-
-// A warp a query and head, a key at a time, FP32.
-constexpr int PLAIN_THREADS = 128;
-template <int D>
-__global__ void __launch_bounds__(PLAIN_THREADS)
-attn_plain_kernel(const __grid_constant__ AttnArgs a)
+// ------------------------------------------------------------------------------------------------------ dealing out --
+// The rows of a sequence and key/value head, i * group + (head in the group), are cut into tiles of `tile` rows; the keys that any row
+// of a tile sees into units of 64 tokens, blocks of the cache.  All units of a call stand in one line, by sequence, head, tile
+// and key, and every CTA takes an equal run of it, whatever the lengths: a CTA's first and last tile may be shared with its neighbours, which
+// merge_kernel then joins; the ones between are its own.
+struct Tile { int lo, end; };    // first unit, unit behind the last
+__device__ __forceinline__ Tile tile_units(const Span& sp, int t, int tile, int group, int window)
 {
+    const int rows = sp.n * group, first = sp.pos + t * tile / group, last = sp.pos + (min(rows, (t + 1) * tile) - 1) / group;
+    return {(window > first ? 0 : first - window + 1) / BLOCK, last / BLOCK + 1};
+}
+struct Deal {
+    int group, tile, window;
+    __device__ __forceinline__ int tiles(const Span& sp) const { return (sp.n * group + tile - 1) / tile; }
+    __device__ __forceinline__ int units(const Span& sp, int t) const
+    {
+        const Tile x = tile_units(sp, t, tile, group, window);
+        return x.end - x.lo;
+    }
+    // units of one head of a sequence, by all lanes of a warp
+    __device__ __forceinline__ long long units_by_warp(const Span& sp) const
+    {
+        const int n = sp.n > 0 ? tiles(sp) : 0;
+        long long u = 0;
+        for (int t = threadIdx.x & 31; t < n; t += 32) u += units(sp, t);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) u += __shfl_xor_sync(0xffffffffu, u, o);
+        return u;
+    }
+};
+
+// Where a CTA's run begins, found by the whole CTA.
+struct Start {
+    long long units;             // of the CTA
+    long long share;             // of every CTA but the last ones
+    long long before;            // units of the sequence ahead of the run
+    int seq;
+};
+// A thread takes neighbouring sequences; where a sequence can have several tiles, a warp does, its lanes the tiles.
+template <int THREADS>
+__device__ __forceinline__ Start find_start(const AttnArgs& a, const Deal& deal, int cta, int ctas)
+{
+    __shared__ long long sums[THREADS / 32];
+    __shared__ Start found;
+    const int tid = threadIdx.x, lane = tid & 31;
+    const bool by_warp = (long long)a.r.max_rows * deal.group > deal.tile;
+    const int takers = by_warp ? THREADS / 32 : THREADS, me = by_warp ? tid / 32 : tid;
+    const int per = (a.c.seqs + takers - 1) / takers, s0 = min(a.c.seqs, me * per), s1 = min(a.c.seqs, s0 + per);
+    auto units = [&](int s) {
+        const Span sp = span_of(a.r, s, a.c.capacity);
+        return (by_warp ? deal.units_by_warp(sp) : sp.n > 0 ? (long long)deal.units(sp, 0) : 0LL) * a.c.kv_heads;
+    };
+    long long mine = 0;
+    for (int s = s0; s < s1; ++s) mine += units(s);
+    long long upto = mine;
+    if (!by_warp) {
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long v = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += v;
+        }
+    }
+    if (lane == 31) sums[tid / 32] = upto;
+    if (tid == 0) found = {0, 0, 0, 0};
+    __syncthreads();
+    long long base = 0, total = 0;
+    for (int w = 0; w < THREADS / 32; ++w) {
+        if (w < tid / 32) base += sums[w];
+        total += sums[w];
+    }
+    upto += base;
+    const long long share = max(1LL, (total + ctas - 1) / ctas), begin = min(total, share * cta), end = min(total, begin + share);
+    if (begin < end && upto - mine <= begin && begin < upto) {           // the same in all lanes of a warp where warps take sequences
+        long long at = upto - mine;
+        for (int s = s0; s < s1; ++s) {
+            const long long n = units(s);
+            if (begin < at + n) {
+                if (!by_warp || lane == 0) found = {end - begin, share, begin - at, s};
+                break;
+            }
+            at += n;
+        }
+    }
+    __syncthreads();
+    return found;
+}
+
+// The tiles of a CTA's run, one after another.
+struct Walk {
+    long long left;              // units of the run behind the current tile
+    int seq, head, t;            // the current tile
+    int u0, n;                   // its first unit and number of units in this run
+    bool begins, ends;           // whether the run has the tile's first and last unit
+    Span sp;
+    Tile whole;
+
+    __device__ __forceinline__ void take(const Deal& d, int skip)
+    {
+        whole = tile_units(sp, t, d.tile, d.group, d.window);
+        u0 = whole.lo + skip;
+        n = (int)min((long long)(whole.end - u0), left);
+        begins = skip == 0;
+        ends = u0 + n == whole.end;
+        left -= n;
+    }
+    // by all lanes of a warp
+    __device__ __forceinline__ void begin(const AttnArgs& a, const Deal& d, const Start& s)
+    {
+        left = s.units;
+        seq = s.seq;
+        sp = span_of(a.r, seq, a.c.capacity);
+        const int n = d.tiles(sp), lane = threadIdx.x & 31;
+        const long long per = n == 1 ? d.units(sp, 0) : d.units_by_warp(sp);
+        head = (int)(s.before / per);
+        int rest = (int)(s.before - head * per);
+        t = 0;
+        while (n > 1) {                                                  // 32 tiles at a time
+            const int mine = t + lane < n ? d.units(sp, t + lane) : 0;
+            int upto = mine;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int v = __shfl_up_sync(0xffffffffu, upto, o);
+                if (lane >= o) upto += v;
+            }
+            const unsigned int in = __ballot_sync(0xffffffffu, rest < upto);
+            if (in != 0) {
+                const int x = __ffs(in) - 1;
+                rest -= __shfl_sync(0xffffffffu, upto - mine, x);
+                t += x;
+                break;
+            }
+            rest -= __shfl_sync(0xffffffffu, upto, 31);
+            t += 32;
+        }
+        take(d, rest);
+    }
+    __device__ __forceinline__ bool next(const AttnArgs& a, const Deal& d)
+    {
+        if (left <= 0) return false;
+        if (++t >= d.tiles(sp)) {
+            t = 0;
+            if (++head >= a.c.kv_heads) {
+                head = 0;
+                do sp = span_of(a.r, ++seq, a.c.capacity); while (sp.n <= 0);
+            }
+        }
+        take(d, 0);
+        return true;
+    }
+};
+
+// Rows of sequences that are out of the call are zeros; CTA `cta` of `ctas` takes its share of the sequences.
+__device__ __forceinline__ void zero_rows(const AttnArgs& a, int D, int cta, int ctas, int tid, int threads)
+{
+    for (int s = cta; s < a.c.seqs; s += ctas) {
+        if (a.r.start[s] >= 0) continue;
+        const int r0 = a.r.row_start ? min(max(a.r.row_start[s], 0), a.r.rows) : s;
+        const int r1 = a.r.row_start ? min(min(max(a.r.row_start[s + 1], r0), a.r.rows), r0 + a.r.max_rows) : s + 1;
+        const int pieces = a.num_heads * D / 8;
+        for (long long i = tid; i < (long long)(r1 - r0) * pieces; i += threads)
+            *reinterpret_cast<uint4*>(a.out + (r0 + i / pieces) * a.ldo + i % pieces * 8) = make_uint4(0, 0, 0, 0);
+    }
+}
+
+// A tile in the workspace: [tile rows][D] sums, then the rows' references and sums of weights.
+__host__ __device__ inline size_t partial_floats(int tile, int D) { return (size_t)tile * (D + 2); }
+
+__device__ __forceinline__ float ex2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
+// the exponent of a block's scale, from the scale
+__device__ __forceinline__ int exponent_of(float scale) { return (int)(__float_as_uint(scale) >> 23) - 127; }
+
+// --------------------------------------------------------------------------------------------- few rows a sequence --
+// Up to 8 NT rows a sequence and key/value head (the query heads that share it, times the new tokens): a tile is all of them, and every key is
+// read once.  Bound by HBM.  Four consumer warps take 16 keys each of a unit, a producer warp brings units by TMA into a ring that runs on over
+// the borders of tiles.  S^T = K Q^T and O^T += V^T P^T as mma.m16n8k16 with the keys, and then the head's elements, as the 16 rows, so that eight
+// rows of queries are a whole operand.  Elements and keys may stand in any order in a sum: lane (g, t) takes 32 elements of keys g and g + 8 for the
+// scores (two 16-byte reads a key, 4 codes a k-step of both registers), and 16 elements of four keys for the output, whose codes
+// are paired by a byte permutation; both reads are free of bank conflicts in the layout that the TMA's swizzle leaves.  P^T needs only a
+// transposition of 8 x 8.  Each warp has its own m; they are joined when the tile ends.
+constexpr int FEW_WARPS = 4, FEW_THREADS = 32 * FEW_WARPS + 32;
+template <int D, int NT>
+struct Few {
+    static constexpr int STAGE = 2 * BLOCK * D;                          // bytes: keys, values
+    static constexpr int CTAS = NT == 4 ? 1 : 2;                         // to an SM
+    static constexpr int STAGES = NT == 4 ? 10 * 128 / D : 6 * 128 / D;
+    static constexpr int TILE = 8 * NT;
+    static constexpr size_t SMEM = 1024 + (size_t)STAGES * STAGE + (size_t)TILE * D * 4;
+};
+
+__device__ __forceinline__ uint32_t codes_f16(uint32_t pair)            // two codes in the low half
+{
+    uint32_t r;
+    asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\t}" : "=r"(r) : "r"(pair));
+    return r;
+}
+__device__ __forceinline__ uint32_t codes_f16_hi(uint32_t pair)         // in the high half
+{
+    uint32_t r;
+    asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, hi;\n\t}" : "=r"(r) : "r"(pair));
+    return r;
+}
+__device__ __forceinline__ void mma_16x8x16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1)
+{
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transposed_8x8(uint32_t v)
+{
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
+}
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi)
+{
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+template <int D, int NT>
+__global__ void __launch_bounds__(FEW_THREADS, Few<D, NT>::CTAS)
+few_kernel(const __grid_constant__ AttnArgs a)
+{
+    using F = Few<D, NT>;
+    constexpr int KS = D / 16, WK = D / 64, DPL = D / 8;     // k-steps, 16-byte words a key and lane for the scores, elements of a lane for the output
+    extern __shared__ uint8_t few_raw[];
+    __shared__ uint64_t full[F::STAGES], empty[F::STAGES];
+    __shared__ float s_m[FEW_WARPS][F::TILE], s_l[FEW_WARPS][F::TILE];
+    __shared__ int s_abort;
+    uint8_t* stages = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(few_raw) + 1023) & ~(uintptr_t)1023);
+    float* join = reinterpret_cast<float*>(stages + (size_t)F::STAGES * F::STAGE);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    if (tid == 0) {
+        for (int i = 0; i < F::STAGES; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], FEW_WARPS); }
+        s_abort = 0;
+        mbar_fence_init();
+    }
     pdl_launch_dependents();
     pdl_wait_prior_grids();
-    const int seq = blockIdx.y, lane = threadIdx.x & 31;
-    int w = blockIdx.x * (PLAIN_THREADS / 32) + (threadIdx.x >> 5);
-    const int i = w / a.num_heads, head = w % a.num_heads;
-    const Span sp = span_of(a.r, seq, a.c.capacity);
-    if (a.r.start[seq] < 0) {                                   // out of the call: zeros
-        const int row = a.r.row_start ? a.r.row_start[seq] + i : seq;
-        const int end = a.r.row_start ? a.r.row_start[seq + 1] : seq + 1;
-        if (row < 0 || row >= min(end, a.r.rows) || i >= a.r.max_rows) return;
-        for (int d = lane; d < D; d += 32) a.out[(size_t)row * a.ldo + head * D + d] = __float2half_rn(0.0f);
+    const Deal deal = {a.num_heads / a.c.kv_heads, F::TILE, a.window};
+    const Start start = find_start<FEW_THREADS>(a, deal, blockIdx.x, gridDim.x);
+    zero_rows(a, D, blockIdx.x, gridDim.x, tid, FEW_THREADS);
+    if (start.units == 0) return;
+    volatile int* abort_flag = &s_abort;
+    Walk w;
+    w.begin(a, deal, start);
+
+    if (warp == FEW_WARPS) {
+        if (lane == 0) {
+            int i = 0;
+            bool ok = true;
+            do {
+                const int held = (w.sp.pos + w.sp.n) / BLOCK;           // units that are codes
+                const int row0 = (w.seq * a.c.kv_heads + w.head) * a.c.capacity;
+                for (int u = w.u0; u < min(w.u0 + w.n, held) && ok; ++u, ++i) {
+                    const int slot = i % F::STAGES;
+                    if (i >= F::STAGES) ok = mbar_wait_bounded(&empty[slot], (uint32_t)(i / F::STAGES - 1) & 1u, abort_flag);
+                    if (!ok) break;
+                    mbar_arrive_expect_tx(&full[slot], F::STAGE);
+                    tma_load_2d(stages + slot * F::STAGE, &a.k_map, 0, row0 + u * BLOCK, &full[slot]);
+                    tma_load_2d(stages + slot * F::STAGE + BLOCK * D, &a.v_map, 0, row0 + u * BLOCK, &full[slot]);
+                }
+            } while (ok && w.next(a, deal));
+        }
         return;
     }
-    if (i >= sp.n) return;
-    const int h = head / (a.num_heads / a.c.kv_heads), pos = sp.pos + i, full = (sp.pos + sp.n) / BLOCK;
-    const size_t at = (size_t)seq * a.c.kv_heads + h;
-    float q[D / 32], o[D / 32];
-    for (int d = 0; d < D / 32; ++d) { q[d] = __half2float(a.q[(size_t)(sp.row + i) * a.ldq + head * D + lane + d * 32]); o[d] = 0.0f; }
-    float m = -INFINITY, l = 0.0f;
-    for (int j = a.window > pos ? 0 : pos - a.window + 1; j <= pos; ++j) {
-        const int b = j / BLOCK;
-        float k[D / 32], v[D / 32], s = 0.0f;
-        if (b < full) {
-            const size_t src = (at * a.c.capacity + j) * D + lane, sc = at * (a.c.capacity / BLOCK) + b;
-            for (int d = 0; d < D / 32; ++d) { k[d] = code_value(a.c.k[src + d * 32]) * a.c.k_scale[sc]; v[d] = code_value(a.c.v[src + d * 32]) * a.c.v_scale[sc]; }
-        } else {
-            const size_t src = ((at * 2 + (b & 1)) * BLOCK + j % BLOCK) * D + lane;
-            for (int d = 0; d < D / 32; ++d) { k[d] = __half2float(a.c.k_tail[src + d * 32]); v[d] = __half2float(a.c.v_tail[src + d * 32]); }
-        }
-        for (int d = 0; d < D / 32; ++d) s = fmaf(q[d], k[d], s);
-        for (int x = 16; x > 0; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
-        s *= a.scale;
-        const float top = fmaxf(m, s), before = m == -INFINITY ? 0.0f : expf(m - top), p = expf(s - top);
-        m = top;
-        l = l * before + p;
-        for (int d = 0; d < D / 32; ++d) o[d] = fmaf(p, v[d], o[d] * before);
+
+    const int g = lane >> 2, t = lane & 3;
+    const int key0 = warp * 16 + g, key1 = key0 + 8;                     // this lane's keys of a unit, for the scores
+    // where in a stage this lane's words are
+    const uint32_t base = smem_u32(stages);
+    auto word = [](int row, int chunk) {                                 // byte of a 16-byte chunk in the swizzled block
+        return D == 128 ? row * 128 + ((chunk ^ (row & 7)) << 4) : row * 64 + ((chunk ^ ((row >> 1) & 3)) << 4);
+    };
+    uint32_t k_at[2][WK], v_at[4];
+#pragma unroll
+    for (int j = 0; j < WK; ++j) { k_at[0][j] = word(key0, t * WK + j); k_at[1][j] = word(key1, t * WK + j); }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const int row = warp * 16 + 2 * t + (j & 1) + (j >> 1) * 8;
+        v_at[j] = BLOCK * D + (D == 128 ? word(row, g) : word(row, g >> 1) + (g & 1) * 8);
     }
-    for (int d = 0; d < D / 32; ++d) a.out[(size_t)(sp.row + i) * a.ldo + head * D + lane + d * 32] = __float2half_rn(o[d] / l);
+
+    int i = 0;
+    do {                                                                 // a warp whose wait ran out goes on to the end, so that all meet at the barriers
+        const int row0 = w.t * F::TILE, rows = min(F::TILE, w.sp.n * deal.group - row0), length = w.sp.pos + w.sp.n, held = length / BLOCK;
+        const size_t at = (size_t)w.seq * a.c.kv_heads + w.head;
+        uint32_t q[NT][KS][2];
+        int pos[NT][2];                                                  // of the two rows whose scores this lane has
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            const int r = nt * 8 + g;
+            const bool live = r < rows;
+            const int rq = row0 + min(r, rows - 1);                     // rows that are not there: zeros at the last one's position
+            const __half* src = a.q + (size_t)(w.sp.row + rq / deal.group) * a.ldq + (w.head * deal.group + rq % deal.group) * D + t * (D / 4);
+#pragma unroll
+            for (int j = 0; j < D / 32; ++j) {
+                const uint4 v = live ? reinterpret_cast<const uint4*>(src)[j] : make_uint4(0, 0, 0, 0);
+                q[nt][2 * j][0] = v.x; q[nt][2 * j][1] = v.y;
+                q[nt][2 * j + 1][0] = v.z; q[nt][2 * j + 1][1] = v.w;
+            }
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                pos[nt][c] = w.sp.pos + (row0 + min(nt * 8 + 2 * t + c, rows - 1)) / deal.group;
+            }
+        }
+        const int first = w.sp.pos + row0 / deal.group, last = w.sp.pos + (row0 + rows - 1) / deal.group;
+        float o[KS][NT][4], m[NT][2], l[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            m[nt][0] = m[nt][1] = -INFINITY;
+            l[nt][0] = l[nt][1] = 0.0f;
+#pragma unroll
+            for (int mt = 0; mt < KS; ++mt)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) o[mt][nt][c] = 0.0f;
+        }
+        for (int u = w.u0; u < w.u0 + w.n; ++u) {
+            float s[NT][4];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) s[nt][c] = 0.0f;
+            uint32_t vw[4][DPL / 4];                              // codes of this lane's elements of four keys
+            uint32_t vt[4][DPL / 2];                                     // the tail's, FP16
+            float factor = a.scale * LOG2E, inv = 1.0f;
+            int ev = 0;
+            const bool codes = u < held;
+            if (codes) {
+                const size_t sc = at * (a.c.capacity / BLOCK) + u;
+                const float ks = a.c.k_scale[sc], vs = a.c.v_scale[sc];
+                const int slot = i % F::STAGES;
+                tc::wait_uniform(&full[slot], (uint32_t)(i / F::STAGES) & 1u, abort_flag);
+                const uint32_t src = base + slot * F::STAGE;
+                uint4 kw[2][WK];
+#pragma unroll
+                for (int j = 0; j < WK; ++j)
+#pragma unroll
+                    for (int k = 0; k < 2; ++k)
+                        asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(kw[k][j].x), "=r"(kw[k][j].y), "=r"(kw[k][j].z), "=r"(kw[k][j].w)
+                                     : "r"(src + k_at[k][j]));
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    if constexpr (D == 128)
+                        asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(vw[j][0]), "=r"(vw[j][1]), "=r"(vw[j][2]), "=r"(vw[j][3]) : "r"(src + v_at[j]));
+                    else
+                        asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(vw[j][0]), "=r"(vw[j][1]) : "r"(src + v_at[j]));
+                }
+                factor *= ks;
+                ev = exponent_of(vs);
+                inv = power_of_two(-ev);
+#pragma unroll
+                for (int j = 0; j < WK; ++j) {
+                    const uint32_t x[4] = {kw[0][j].x, kw[0][j].y, kw[0][j].z, kw[0][j].w}, y[4] = {kw[1][j].x, kw[1][j].y, kw[1][j].z, kw[1][j].w};
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const uint32_t a0 = codes_f16(x[k]), a1 = codes_f16(y[k]), a2 = codes_f16_hi(x[k]), a3 = codes_f16_hi(y[k]);
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) mma_16x8x16(s[nt], a0, a1, a2, a3, q[nt][j * 4 + k][0], q[nt][j * 4 + k][1]);
+                    }
+                }
+            } else {
+                // the tail, FP16, from its place in memory; rows behind the sequence's end are taken as zeros
+                const __half *kt = a.c.k_tail + (at * 2 + (u & 1)) * BLOCK * D, *vt_ = a.c.v_tail + (at * 2 + (u & 1)) * BLOCK * D;
+                const int valid = length - u * BLOCK;
+                const uint4 none = make_uint4(0, 0, 0, 0);
+#pragma unroll
+                for (int j = 0; j < D / 32; ++j) {
+                    const uint4 x = key0 < valid ? reinterpret_cast<const uint4*>(kt + key0 * D + t * (D / 4))[j] : none;
+                    const uint4 y = key1 < valid ? reinterpret_cast<const uint4*>(kt + key1 * D + t * (D / 4))[j] : none;
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        mma_16x8x16(s[nt], x.x, y.x, x.y, y.y, q[nt][2 * j][0], q[nt][2 * j][1]);
+                        mma_16x8x16(s[nt], x.z, y.z, x.w, y.w, q[nt][2 * j + 1][0], q[nt][2 * j + 1][1]);
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int row = warp * 16 + 2 * t + (j & 1) + (j >> 1) * 8;
+#pragma unroll
+                    for (int k = 0; k < DPL / 8; ++k) {
+                        const uint4 x = row < valid ? reinterpret_cast<const uint4*>(vt_ + row * D + g * DPL)[k] : none;
+                        vt[j][4 * k] = x.x; vt[j][4 * k + 1] = x.y; vt[j][4 * k + 2] = x.z; vt[j][4 * k + 3] = x.w;
+                    }
+                }
+            }
+            // exponents, masked where not every row sees every key of the unit
+            const bool all_seen = (u + 1) * BLOCK - 1 <= first && last - u * BLOCK < a.window;
+            bool over = false;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    s[nt][c] = fmaf(s[nt][c], factor, (float)ev);
+                    if (!all_seen) {
+                        const int key = u * BLOCK + (c < 2 ? key0 : key1), p = pos[nt][c & 1];
+                        if (!(key <= p && p - key < a.window)) s[nt][c] = -INFINITY;
+                    }
+                    over |= s[nt][c] > m[nt][c & 1] + 8.0f;
+                }
+            if (__any_sync(0xffffffffu, over)) {
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        float top = fmaxf(s[nt][c], s[nt][c + 2]);
+#pragma unroll
+                        for (int x = 4; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+                        if (top > m[nt][c]) {
+                            const float before = ex2(m[nt][c] - top);
+                            m[nt][c] = top;
+                            l[nt][c] *= before;
+#pragma unroll
+                            for (int mt = 0; mt < KS; ++mt) { o[mt][nt][c] *= before; o[mt][nt][c + 2] *= before; }
+                        }
+                    }
+            }
+            uint32_t p[NT][2];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                float e[4];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) e[c] = ex2(s[nt][c] - (m[nt][c & 1] == -INFINITY ? 0.0f : m[nt][c & 1]));
+                l[nt][0] = fmaf(e[0] + e[2], inv, l[nt][0]);
+                l[nt][1] = fmaf(e[1] + e[3], inv, l[nt][1]);
+                p[nt][0] = transposed_8x8(pack_f16(e[0], e[1]));
+                p[nt][1] = transposed_8x8(pack_f16(e[2], e[3]));
+            }
+            if (codes) {
+#pragma unroll
+                for (int k = 0; k < DPL / 4; ++k) {                      // four elements: two m-tiles
+                    const uint32_t lo0 = __byte_perm(vw[0][k], vw[1][k], 0x5140), hi0 = __byte_perm(vw[0][k], vw[1][k], 0x7362);
+                    const uint32_t lo1 = __byte_perm(vw[2][k], vw[3][k], 0x5140), hi1 = __byte_perm(vw[2][k], vw[3][k], 0x7362);
+                    const uint32_t a0 = codes_f16(lo0), a1 = codes_f16_hi(lo0), a2 = codes_f16(lo1), a3 = codes_f16_hi(lo1);
+                    const uint32_t b0 = codes_f16(hi0), b1 = codes_f16_hi(hi0), b2 = codes_f16(hi1), b3 = codes_f16_hi(hi1);
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        mma_16x8x16(o[2 * k][nt], a0, a1, a2, a3, p[nt][0], p[nt][1]);
+                        mma_16x8x16(o[2 * k + 1][nt], b0, b1, b2, b3, p[nt][0], p[nt][1]);
+                    }
+                }
+                // Not ahead of the products: words that were only asked for were overtaken by the next copy in a call of forty.
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&empty[i % F::STAGES]);
+                ++i;
+            } else {
+#pragma unroll
+                for (int mt = 0; mt < KS; ++mt) {
+                    const uint32_t a0 = __byte_perm(vt[0][mt], vt[1][mt], 0x5410), a1 = __byte_perm(vt[0][mt], vt[1][mt], 0x7632);
+                    const uint32_t a2 = __byte_perm(vt[2][mt], vt[3][mt], 0x5410), a3 = __byte_perm(vt[2][mt], vt[3][mt], 0x7632);
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) mma_16x8x16(o[mt][nt], a0, a1, a2, a3, p[nt][0], p[nt][1]);
+                }
+            }
+        }
+        // ---- the four warps' parts of the tile, in warp order ----
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+#pragma unroll
+                for (int x = 4; x < 32; x <<= 1) l[nt][c] += __shfl_xor_sync(0xffffffffu, l[nt][c], x);
+                if (g == 0) { s_m[warp][nt * 8 + 2 * t + c] = m[nt][c]; s_l[warp][nt * 8 + 2 * t + c] = l[nt][c]; }
+            }
+        named_bar_sync(1, 32 * FEW_WARPS);
+        float f[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                const int r = nt * 8 + 2 * t + c;
+                const float top = fmaxf(fmaxf(s_m[0][r], s_m[1][r]), fmaxf(s_m[2][r], s_m[3][r]));
+                f[nt][c] = ex2(m[nt][c] - (top == -INFINITY ? 0.0f : top));      // a NaN sum stays one
+            }
+        for (int turn = 0; turn < FEW_WARPS; ++turn) {
+            if (turn == warp) {
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        float* row = join + (nt * 8 + 2 * t + c) * D + g * DPL;      // elements 2 mt, 2 mt + 1 of this lane's
+#pragma unroll
+                        for (int mt = 0; mt < KS; ++mt) {
+                            float2 v = make_float2(o[mt][nt][c] * f[nt][c], o[mt][nt][c + 2] * f[nt][c]);
+                            if (turn > 0) { const float2 x = *reinterpret_cast<float2*>(row + 2 * mt); v.x += x.x; v.y += x.y; }
+                            *reinterpret_cast<float2*>(row + 2 * mt) = v;
+                        }
+                    }
+            }
+            named_bar_sync(1, 32 * FEW_WARPS);
+        }
+        // ---- out, or to the workspace where other CTAs have keys of the tile ----
+        const bool alone = w.begins && w.ends, ok = *abort_flag == 0;
+        float* part = a.partial + (2 * (size_t)blockIdx.x + (w.begins ? 1 : 0)) * partial_floats(F::TILE, D);
+        for (int j = tid; j < rows * (D / 4); j += 32 * FEW_WARPS) {
+            const int r = j / (D / 4), d = j % (D / 4) * 4;
+            const float4 v = *reinterpret_cast<const float4*>(join + r * D + d);
+            const float top = fmaxf(fmaxf(s_m[0][r], s_m[1][r]), fmaxf(s_m[2][r], s_m[3][r]));
+            const float ref = top == -INFINITY ? 0.0f : top;
+            float sum = 0.0f;
+#pragma unroll
+            for (int x = 0; x < FEW_WARPS; ++x) sum = fmaf(s_l[x][r], ex2(s_m[x][r] - ref), sum);
+            if (!ok) continue;
+            if (alone) {
+                const float n = 1.0f / sum;
+                __half* dst = a.out + (size_t)(w.sp.row + (row0 + r) / deal.group) * a.ldo + (w.head * deal.group + (row0 + r) % deal.group) * D + d;
+                *reinterpret_cast<uint2*>(dst) = make_uint2(pack_f16(v.x * n, v.y * n), pack_f16(v.z * n, v.w * n));
+            } else {
+                *reinterpret_cast<float4*>(part + r * D + d) = v;
+                if (d == 0) { part[F::TILE * D + r] = top; part[F::TILE * (D + 1) + r] = sum; }
+            }
+        }
+        named_bar_sync(1, 32 * FEW_WARPS);                               // `join` and the statistics are the next tile's
+    } while (w.next(a, deal));
+}
+
+// ------------------------------------------------------------------------------------------------------------- merge --
+// Joins the tiles that several CTAs have keys of: CTA x takes the tile that CTA x of the kernel before began and did not end.  Its parts are
+// the last part of that CTA and the first parts of those behind it, added in that order: the same call gives the same bits.
+constexpr int MERGE_THREADS = 256;
+template <int D>
+__global__ void __launch_bounds__(MERGE_THREADS)
+merge_kernel(const __grid_constant__ AttnArgs a, int tile, int rows_each)
+{
+    constexpr int LANES = D / 4, SIDES = MERGE_THREADS / LANES;          // threads of a row; parts taken at once
+    __shared__ float4 red[SIDES][LANES];
+    __shared__ float red_l[SIDES];
+    pdl_launch_dependents();
+    pdl_wait_prior_grids();
+    const Deal deal = {a.num_heads / a.c.kv_heads, tile, a.window};
+    const Start start = find_start<MERGE_THREADS>(a, deal, blockIdx.x, gridDim.x);
+    if (start.units == 0) return;
+    Walk w;
+    w.begin(a, deal, start);
+    while (w.left > 0) w.next(a, deal);                                  // the run's last tile
+    if (!w.begins || w.ends) return;
+    const int parts = 1 + (int)((w.whole.end - w.u0 - w.n + start.share - 1) / start.share);
+    const size_t each = partial_floats(tile, D);
+    const float* base = a.partial + (2 * (size_t)blockIdx.x + 1) * each;         // part j > 0: the first of CTA x + j
+    auto part = [&](int j) { return j == 0 ? base : base + (2 * (size_t)j - 1) * each; };
+    const int rows = min(tile, w.sp.n * deal.group - w.t * tile), side = threadIdx.x / LANES, lane = threadIdx.x % LANES;
+    for (int r = blockIdx.y * rows_each; r < min(rows, (blockIdx.y + 1) * rows_each); ++r) {
+        float top = -INFINITY;
+        for (int j = 0; j < parts; ++j) top = fmaxf(top, part(j)[tile * D + r]);
+        const float ref = top == -INFINITY ? 0.0f : top;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        float l = 0.0f;
+        for (int j = side; j < parts; j += SIDES) {
+            const float* p = part(j);
+            const float f = ex2(p[tile * D + r] - ref);
+            const float4 x = reinterpret_cast<const float4*>(p + r * D)[lane];
+            v.x = fmaf(x.x, f, v.x); v.y = fmaf(x.y, f, v.y); v.z = fmaf(x.z, f, v.z); v.w = fmaf(x.w, f, v.w);
+            l = fmaf(p[tile * (D + 1) + r], f, l);
+        }
+        red[side][lane] = v;
+        if (lane == 0) red_l[side] = l;
+        __syncthreads();
+        if (side == 0) {
+            for (int x = 1; x < SIDES; ++x) {
+                const float4 y = red[x][lane];
+                v.x += y.x; v.y += y.y; v.z += y.z; v.w += y.w;
+                l += red_l[x];
+            }
+            const float n = 1.0f / l;
+            const int row = w.t * tile + r;
+            __half* dst = a.out + (size_t)(w.sp.row + row / deal.group) * a.ldo + (w.head * deal.group + row % deal.group) * D + lane * 4;
+            *reinterpret_cast<uint2*>(dst) = make_uint2(pack_f16(v.x * n, v.y * n), pack_f16(v.z * n, v.w * n));
+        }
+        __syncthreads();
+    }
 }
 
 }  // namespace cache8

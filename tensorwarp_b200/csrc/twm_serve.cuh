@@ -30,6 +30,59 @@ twm::cache8::Cache device_cache(const twm_cache8* c)
     return {c->seqs, c->kv_heads, c->capacity, (uint8_t*)c->k, (uint8_t*)c->v, c->k_scale, c->v_scale, (__half*)c->k_tail, (__half*)c->v_tail};
 }
 
+// How attention is launched: the rows of a tile and the CTAs of the grid, whatever the lengths (which are on the device).
+struct AttnPlan { int tile, ctas; };
+AttnPlan plan_attention(int group, int max_rows)
+{
+    const long rows = (long)max_rows * group;
+    if (rows <= 8) return {8, 2 * kDefaultSms};
+    if (rows <= 16) return {16, 2 * kDefaultSms};
+    return {32, kDefaultSms};
+}
+
+// The codes of keys or values as [cached rows][head_dim], a box a block, swizzled over its whole row.
+bool make_codes_map(CUtensorMap* map, const twm_cache8* c, void* codes)
+{
+    EncodeTiledFn enc = get_encode_tiled();
+    if (!enc) return false;
+    const cuuint64_t gdim[2] = {(cuuint64_t)c->head_dim, (cuuint64_t)c->seqs * c->kv_heads * c->capacity};
+    const cuuint64_t gstride[1] = {(cuuint64_t)c->head_dim};
+    const cuuint32_t box[2] = {(cuuint32_t)c->head_dim, TWM_CACHE8_BLOCK};
+    const cuuint32_t estride[2] = {1, 1};
+    return enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, codes, gdim, gstride, box, estride, CU_TENSOR_MAP_INTERLEAVE_NONE,
+               c->head_dim == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// Lets a kernel take more than 48 KB of shared memory on the current device.  The limit belongs to the function: it is set once a device, to what
+// every launch of it asks for.
+twm_status allow_shared(const char* name, const void* kernel, size_t bytes)
+{
+    static std::mutex mutex;
+    static std::vector<std::pair<const void*, int>> done;
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e == cudaSuccess) {
+        std::lock_guard<std::mutex> lock(mutex);
+        for (const auto& x : done)
+            if (x.first == kernel && x.second == dev) return TWM_OK;
+        if ((e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes)) == cudaSuccess) done.emplace_back(kernel, dev);
+    }
+    if (e == cudaSuccess) return TWM_OK;
+    set_error(name, e);
+    return TWM_ELAUNCH;
+}
+
+template <int D, int NT>
+twm_status launch_few(const twm::cache8::AttnArgs& a, const AttnPlan& p, int flags, void* stream)
+{
+    auto* kernel = twm::cache8::few_kernel<D, NT>;
+    constexpr size_t smem = twm::cache8::Few<D, NT>::SMEM;
+    const twm_status st = allow_shared("twm_cache8_attention", (const void*)kernel, smem);
+    if (st != TWM_OK) return st;
+    return launch_op("twm_cache8_attention", kernel, dim3(p.ctas), dim3(twm::cache8::FEW_THREADS), smem, flags, stream, a);
+}
+
 }  // namespace
 
 extern "C" {
@@ -54,8 +107,9 @@ twm_status twm_cache8_append(const twm_cache8* cache, void* q_out, long ldq, con
 
 size_t twm_cache8_attention_bytes(const twm_cache8* c, int num_heads, int max_rows)
 {
-    if (!c || num_heads < 1 || max_rows < 1 || c->seqs < 1 || c->kv_heads < 1 || (c->head_dim != 64 && c->head_dim != 128)) return 0;
-    return 16;
+    if (!c || num_heads < 1 || max_rows < 1 || c->kv_heads < 1 || num_heads % c->kv_heads || (c->head_dim != 64 && c->head_dim != 128)) return 0;
+    const AttnPlan p = plan_attention(num_heads / c->kv_heads, max_rows);
+    return 2 * (size_t)p.ctas * twm::cache8::partial_floats(p.tile, c->head_dim) * sizeof(float);
 }
 
 twm_status twm_cache8_attention(const twm_cache8* cache, void* out, long ldo, const void* q, long ldq, int num_heads, int rows, const int* row_start,
@@ -64,17 +118,27 @@ twm_status twm_cache8_attention(const twm_cache8* cache, void* out, long ldo, co
 {
     twm_status st = check_cache8(cache, num_heads, rows, row_start, max_rows, start);
     if (st == TWM_EINVAL) return st;
-    if (!out || !q || !workspace || window < 0 || !(scale > 0.0f) || ldo < (long)num_heads * cache->head_dim || ldq < (long)num_heads * cache->head_dim)
-        return TWM_EINVAL;
+    const int D = cache->head_dim;
+    if (!out || !q || !workspace || window < 0 || !(scale > 0.0f) || ldo < (long)num_heads * D || ldq < (long)num_heads * D) return TWM_EINVAL;
     if (st != TWM_OK) return st;
     if (off16(out) || off16(q) || off16(workspace) || (ldo & 7) || (ldq & 7)) return TWM_EALIGN;
     if (workspace_bytes < twm_cache8_attention_bytes(cache, num_heads, max_rows)) return TWM_EWORKSPACE;
     if ((st = ensure_device(nullptr)) != TWM_OK) return st;
-    const twm::cache8::AttnArgs a = {device_cache(cache), {row_start, start, rows, max_rows}, (__half*)out, (const __half*)q, ldo, ldq, num_heads,
-                                     window ? window : INT_MAX, scale};
-    const dim3 grid((unsigned)(((long)max_rows * num_heads + 3) / 4), cache->seqs);
-    return launch_op("twm_cache8_attention", cache->head_dim == 64 ? twm::cache8::attn_plain_kernel<64> : twm::cache8::attn_plain_kernel<128>, grid,
-                     dim3(twm::cache8::PLAIN_THREADS), 0, flags, stream, a);
+    const AttnPlan p = plan_attention(num_heads / cache->kv_heads, max_rows);
+    twm::cache8::AttnArgs a = {device_cache(cache), {row_start, start, rows, max_rows}, (__half*)out, (const __half*)q, ldo, ldq, num_heads,
+                               window ? window : INT_MAX, scale, (float*)workspace, {}, {}};
+    if (!make_codes_map(&a.k_map, cache, cache->k) || !make_codes_map(&a.v_map, cache, cache->v)) {
+        snprintf(t_last_error, sizeof(t_last_error), "cuTensorMapEncodeTiled failed for a cache held in 8 bits");
+        return TWM_ELAUNCH;
+    }
+    if (D == 64)
+        st = p.tile == 8 ? launch_few<64, 1>(a, p, flags, stream) : p.tile == 16 ? launch_few<64, 2>(a, p, flags, stream) : launch_few<64, 4>(a, p, flags, stream);
+    else
+        st = p.tile == 8 ? launch_few<128, 1>(a, p, flags, stream) : p.tile == 16 ? launch_few<128, 2>(a, p, flags, stream) : launch_few<128, 4>(a, p, flags, stream);
+    if (st != TWM_OK) return st;
+    constexpr int each = 1;          // rows of a merging CTA
+    return launch_op("twm_cache8_attention(merge)", D == 64 ? twm::cache8::merge_kernel<64> : twm::cache8::merge_kernel<128>,
+                     dim3(p.ctas, (p.tile + each - 1) / each), dim3(twm::cache8::MERGE_THREADS), 0, flags, stream, a, p.tile, each);
 }
 
 twm_status twm_sample(const twm_sample_args* args, int flags, void* stream)

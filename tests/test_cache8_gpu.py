@@ -320,6 +320,27 @@ def test_far_places():
     assert bool(((out.double() - want).abs() <= off).all())
 
 
+@pytest.mark.parametrize("heads,kv_heads,dim,rows", [(40, 8, 128, 1), (16, 8, 64, 4), (28, 4, 128, 5), (16, 4, 128, 40)])
+def test_long_batches_give_the_same_bits_again(heads, kv_heads, dim, rows):
+    """Stages are used over and over, tiles begin and end anywhere in a CTA's run: a hundred calls, one result."""
+    seqs, cap = 64, 4096
+    cache = cache8.Cache8.empty(seqs, cap, kv_heads, dim)
+    g = gen("long", heads, rows)
+    for t in (cache.k, cache.v):
+        t.view(torch.uint8).copy_(torch.randint(0, 0x70, t.shape, generator=g, device="cuda", dtype=torch.uint8))
+    for t in (cache.k_tail, cache.v_tail):
+        t.copy_(torch.randn(t.shape, generator=g, device="cuda"))
+    cache.k_scale.fill_(2.0 ** -7), cache.v_scale.fill_(2.0 ** -6)
+    q = torch.randn((seqs * rows, heads * dim), generator=g, device="cuda").half()
+    start = torch.randint(0, cap - rows, (seqs,), generator=g, device="cuda", dtype=torch.int32)
+    row_start = ints([rows * s for s in range(seqs + 1)])
+    ws, outs = cache8.Workspace.for_cache(cache, heads, rows), []
+    for _ in range(100):
+        outs.append(torch.zeros_like(q))
+        cache8.attention(cache, q, outs[-1], start, num_heads=heads, row_start=row_start, max_rows=rows, workspace=ws)
+    assert all(torch.equal(outs[0], o) for o in outs[1:])
+
+
 def test_captured_step_serves_every_position():
     b = Batch(2, 256, 8, 2, 128)
     b.append([0, 0], [126, 60])
