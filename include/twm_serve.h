@@ -68,9 +68,9 @@ twm_status twm_cache8_attention(const twm_cache8* cache, void* out_f16, long ldo
  *   min_p   of these the ones with w >= min_p (<= 0: all; values over 1 count as 1).
  * The token is the first index, rising, at which the running sum of the kept w exceeds random * their sum; prob is its w over
  * that sum.  temperature 0 (or not > 0): the first largest logit.  A NaN logit counts as -inf; a row without any other gives
- * token 0.  Sums are those of 64-bit numbers, in an order of their own: the same call gives the same token. */
+ * token 0.  Sums do not depend on an order: the same call gives the same token. */
 typedef struct twm_sample_args {
-    int rows, vocab;
+    int rows, vocab;             /* vocab: at most 2^20 */
     int dtype;                   /* TWM_F32, TWM_F16 or TWM_BF16 */
     const void* logits;          /* [rows], row stride ld */
     long ld;

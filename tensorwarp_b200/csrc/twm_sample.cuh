@@ -1,4 +1,16 @@
 // twm_sample.cuh — one token of every row of logits: temperature, top-k, top-p, min-p (include/twm_serve.h).
+//
+// A row belongs to a cluster of CTAs, each with a slice of it in shared memory: logits are read from memory once, whatever cuts are asked for.
+// Nothing is sorted.  The kept tokens are the head of an order, so all cuts come down to one key and how many of the tokens equal to it are
+// kept; that border is found by histograms, narrowing in on the bin it lies in:
+//   level 0   bins of 1/16 octave of weight below the largest logit's, 1024 of them (what is beyond, 2^-64, is one more bin);
+//   level 1   1024 parts of the bin that the border lies in;
+//   then      keys (logits as ordered integers), 1024 parts of what is left, which only many equal or nearly equal logits need;
+// and once 32 tokens or fewer are left they are ordered by one warp.  A bin holds its number of tokens and its mass.  Within a bin weights are
+// within 2^(1/16) of its largest W: mass = W (count - sum of delta), delta = 1 - w / W in fixed point, so that both are integer sums, the
+// same in any order: the result does not depend on which thread comes first.
+// Then running sums, by index, of the kept weights find the token.
+// Bound by memory for many rows, by the chain of cluster barriers for one.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -12,155 +24,471 @@ namespace sample {
 __device__ __forceinline__ float logit_f32(float v) { return v; }
 __device__ __forceinline__ float logit_f32(__half v) { return __half2float(v); }
 __device__ __forceinline__ float logit_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
-
-// Numbers in the order of unsigned integers: NaN as -inf, both zeros alike.
+// NaN as -inf, both zeros alike
+__device__ __forceinline__ float plain(float v) { return v == v ? v + 0.0f : -INFINITY; }
+// numbers in the order of unsigned integers
 __device__ __forceinline__ uint32_t order_of(float v)
 {
-    v = v == v ? v + 0.0f : -INFINITY;
     const uint32_t b = __float_as_uint(v);
     return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 __device__ __forceinline__ float value_of(uint32_t o) { return __uint_as_float(o & 0x80000000u ? o & 0x7fffffffu : ~o); }
 
-constexpr int THREADS = 1024;
+constexpr int THREADS = 512, WARPS = THREADS / 32, BINS = 1024, MAX_CTAS = 16, FEW = 32;
+constexpr int MAX_SLICE = 40960;         // logits of a CTA in shared memory; what is beyond is read again
+
+__device__ __forceinline__ void st_cluster_u32(uint32_t at, uint32_t v) { asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(at), "r"(v) : "memory"); }
+__device__ __forceinline__ void st_cluster_u64(uint32_t at, unsigned long long v) { asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(at), "l"(v) : "memory"); }
+__device__ __forceinline__ uint32_t ld_cluster_u32(uint32_t at)
+{
+    uint32_t v;
+    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
+    return v;
+}
+
+// Weights below the largest logit's: exponents in octaves, the factor in two parts so that a weight is good to the last bits that ex2 has.
+struct Weights {
+    float top, hi, lo;
+    __device__ __forceinline__ void set(float mx, double temperature)
+    {
+        const double c = fmin(1.4426950408889634 / temperature, 1e30);
+        top = mx;
+        hi = (float)c;
+        lo = (float)(c - (double)hi);
+    }
+    __device__ __forceinline__ float octaves(float v) const { return (v - top) * hi; }         // <= 0, rising with v; NaN for no number of them
+    __device__ __forceinline__ float of(float v) const
+    {
+        if (v == top) return 1.0f;
+        const float d = v - top, x = d * hi;
+        if (!(x > -140.0f)) return 0.0f;
+        const float rest = fmaf(d, lo, fmaf(d, hi, -x));
+        float y;
+        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+        return fmaf(y, rest * 0.69314718f, y);
+    }
+};
+
+struct Shared {
+    uint32_t count[BINS], delta[BINS];                   // this CTA's, as it counts
+    uint32_t all_count[BINS];                            // the cluster's
+    unsigned long long all_delta[BINS];
+    uint32_t part_count[THREADS];
+    unsigned long long part_delta[THREADS];
+    uint32_t warp_u32[WARPS];
+    double warp_f64[WARPS];
+    uint32_t cta_max[MAX_CTAS];
+    uint32_t cta_lo[2][MAX_CTAS], cta_hi[2][MAX_CTAS];   // smallest and largest key of a range, two turns
+    uint32_t cta_ties[MAX_CTAS];
+    unsigned long long cta_above[MAX_CTAS];
+    uint32_t list_n[2], list[2][FEW];                    // the last tokens of top-k's border, of top-p's
+    uint32_t found_bin, found_count, found_over;
+    double found_mass, found_over_mass;
+    uint32_t cut, ties;
+    double cut_mass;
+};
+
+// counts and masses ahead of this thread's two bins, and of all
+struct Scan { uint32_t before, all; double mass_before, mass_all; };
+__device__ __forceinline__ Scan scan(Shared& sh, uint32_t c, double m)
+{
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    uint32_t uc = c;
+    double um = m;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t xc = __shfl_up_sync(0xffffffffu, uc, o);
+        const double xm = __shfl_up_sync(0xffffffffu, um, o);
+        if (lane >= o) { uc += xc; um += xm; }
+    }
+    __syncthreads();
+    if (lane == 31) { sh.warp_u32[warp] = uc; sh.warp_f64[warp] = um; }
+    __syncthreads();
+    Scan s = {0, 0, 0.0, 0.0};
+    uint32_t bc = 0;
+    double bm = 0.0;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) {
+        if (w == warp) { bc = s.all; bm = s.mass_all; }
+        s.all += sh.warp_u32[w];
+        s.mass_all += sh.warp_f64[w];
+    }
+    const uint32_t xc = __shfl_up_sync(0xffffffffu, uc, 1);
+    const double xm = __shfl_up_sync(0xffffffffu, um, 1);
+    s.before = bc + (lane ? xc : 0u);
+    s.mass_before = bm + (lane ? xm : 0.0);
+    return s;
+}
 
 template <typename T>
-__global__ void __launch_bounds__(THREADS)
-sample_kernel(const __grid_constant__ twm_sample_args a)
+__global__ void __launch_bounds__(THREADS, 2)
+sample_kernel(const __grid_constant__ twm_sample_args a, int slice)
 {
-    __shared__ double red[32];
-    __shared__ double prefix[THREADS + 1];
-    __shared__ int s_token;
+    extern __shared__ __align__(16) float vals[];
+    __shared__ Shared sh;
+    cluster_started();
     pdl_launch_dependents();
+    const int row = blockIdx.x, rank = blockIdx.y, ctas = gridDim.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int n = a.vocab, n0 = min(n, rank * slice), ns = min(n - n0, slice);
+    for (int i = tid; i < BINS; i += THREADS) sh.count[i] = sh.delta[i] = 0;
+    if (tid < 2) sh.list_n[tid] = 0;
     pdl_wait_prior_grids();
-    const int row = blockIdx.x, tid = threadIdx.x, n = a.vocab;
-    const T* logits = reinterpret_cast<const T*>(a.logits) + (size_t)row * a.ld;
-    auto total = [&](double v) {
-        for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-        __syncthreads();
-        if ((tid & 31) == 0) red[tid >> 5] = v;
-        __syncthreads();
-        double t = 0;
-        for (int w = 0; w < THREADS / 32; ++w) t += red[w];
-        return t;
-    };
-    auto key = [&](int i) { return order_of(logit_f32(logits[i])); };
-    // largest, first index of it
-    __shared__ unsigned long long s_best;
-    if (tid == 0) s_best = 0;
-    __syncthreads();
-    unsigned long long best = 0;
-    for (int i = tid; i < n; i += THREADS) best = max(best, ((unsigned long long)key(i) << 32) | (0xffffffffu - (uint32_t)i));
-    atomicMax(&s_best, best);
-    __syncthreads();
-    const uint32_t top = (uint32_t)(s_best >> 32);
-    const int first = (int)(0xffffffffu - (uint32_t)s_best);
-    const float mx = value_of(top);
+    const T* logits = reinterpret_cast<const T*>(a.logits) + (size_t)row * a.ld + n0;
     const float t = a.temperature ? a.temperature[row] : 1.0f;
-    float prob = 1.0f;
-    int token = mx == -INFINITY ? 0 : first;
-    if (t > 0.0f && mx != -INFINITY) {
-        const double inv_t = 1.0 / (double)t;
-        auto weight = [&](uint32_t k) {
-            const float v = value_of(k);
-            return v == mx ? 1.0 : mx == INFINITY || v == -INFINITY ? 0.0 : exp(((double)v - (double)mx) * inv_t);
-        };
-        // kept: keys over `cut`, and the first `ties` of those equal to it
-        uint32_t cut = 0;
-        double ties = n;
-        const int k = a.top_k ? a.top_k[row] : 0;
-        const float p = a.top_p ? a.top_p[row] : 1.0f, mp = fminf(a.min_p ? a.min_p[row] : 0.0f, 1.0f);
-        // the largest key with measure(keys >= it) >= want, and what of the measure is over it
-        auto search = [&](auto measure, double want, double& over) {
-            uint32_t lo = 0;                                     // measure(>= 0) >= want
-            for (int bit = 31; bit >= 0; --bit) {
-                const uint32_t mid = lo | (1u << bit);
-                double v = 0;
-                for (int i = tid; i < n; i += THREADS) { const uint32_t x = key(i); if (x >= mid) v += measure(x); }
-                if (total(v) >= want) lo = mid;
-            }
-            double v = 0;
-            for (int i = tid; i < n; i += THREADS) { const uint32_t x = key(i); if (x > lo) v += measure(x); }
-            over = total(v);
-            return lo;
-        };
-        double mass = 0, over;
-        if (k > 0 && k < n) {
-            cut = search([](uint32_t) { return 1.0; }, k, over);
-            ties = k - over;
+    const int k = a.top_k ? a.top_k[row] : 0;
+    const float p = a.top_p ? a.top_p[row] : 1.0f, mp = a.min_p ? a.min_p[row] : 0.0f;
+    const float random = a.random[a.step ? min(max(a.step[0], 0), a.random_count - 1) : row];
+
+    // ---- the slice into shared memory, and its largest logit ----
+    const int held = min(ns, MAX_SLICE);
+    float mx = -INFINITY;
+    constexpr int V = 16 / sizeof(T);
+    const int vecs = (reinterpret_cast<uintptr_t>(logits) & 15) == 0 ? held / V : 0;
+    for (int i = tid; i < vecs; i += THREADS) {
+        const uint4 u = __ldcs(reinterpret_cast<const uint4*>(logits) + i);
+        T x[V];
+        *reinterpret_cast<uint4*>(x) = u;
+#pragma unroll
+        for (int j = 0; j < V; j += 4) {
+            const float4 f = make_float4(plain(logit_f32(x[j])), plain(logit_f32(x[j + 1])), plain(logit_f32(x[j + 2])), plain(logit_f32(x[j + 3])));
+            mx = fmaxf(mx, fmaxf(fmaxf(f.x, f.y), fmaxf(f.z, f.w)));
+            *reinterpret_cast<float4*>(vals + i * V + j) = f;
         }
-        if (p < 1.0f) {
-            double v = 0;
-            for (int i = tid; i < n; i += THREADS) { const uint32_t x = key(i); if (x > cut) v += weight(x); }
-            mass = total(v);
-            double same = 0;
-            for (int i = tid; i < n; i += THREADS) same += key(i) == cut;
-            same = total(same);
-            if (same > 0) mass += fmin(same, ties) * weight(cut);
-            const double want = fmax((double)p * mass, 1e-30);
-            const uint32_t c = max(cut, search(weight, fmin(want, mass * 0.9999999999), over));
-            if (c > cut || over >= want) ties = n;
-            cut = c;
-            ties = fmin(ties, fmax(1.0, ceil((want - over) / fmax(weight(cut), 1e-300))));
+    }
+    for (int i = vecs * V + tid; i < ns; i += THREADS) {
+        const float f = plain(logit_f32(logits[i]));
+        mx = fmaxf(mx, f);
+        if (i < held) vals[i] = f;
+    }
+    auto at = [&](int i) { return i < held ? vals[i] : plain(logit_f32(logits[i])); };
+    uint32_t key = __reduce_max_sync(0xffffffffu, order_of(mx));
+    if (lane == 0) sh.warp_u32[warp] = key;
+    __syncthreads();
+    cluster_wait_started();
+    if (tid < ctas) {
+        key = 0;
+        for (int w = 0; w < WARPS; ++w) key = max(key, sh.warp_u32[w]);
+        st_cluster_u32(mapa_shared(smem_u32(&sh.cta_max[rank]), tid), key);
+    }
+    cluster_sync_all();
+    key = 0;
+    for (int c = 0; c < ctas; ++c) key = max(key, sh.cta_max[c]);
+    mx = value_of(key);
+
+    uint32_t cut = 0, ties = 0x7fffffffu;                // kept: keys over cut, and the first `ties` of those that are cut
+    Weights weights = {mx, 0.0f, 0.0f};
+    const bool none = mx == -INFINITY, greedy = !(t > 0.0f);
+    if (none || greedy) {
+        cut = key;
+        ties = 1;
+    } else {
+        weights.set(mx, (double)t);
+        const bool need_k = k > 0 && k < n, need_p = p < 1.0f;
+        if (need_k || need_p) {
+            // a token's bin at level 0, or BINS, and its place in the bin
+            auto bin_of = [&](float v, float& within) {
+                const float x = v == mx ? 0.0f : -16.0f * weights.octaves(v);
+                if (!(x < (float)BINS)) { within = 0.0f; return BINS; }
+                const int b = (int)x;
+                within = x - (float)b;
+                return b;
+            };
+            // delta < 0.0424: a slice's sum of them fits 32 bits
+            const float fixed = slice <= 24000 ? 4194304.0f : slice <= 48000 ? 2097152.0f : 1048576.0f;
+            const double unit = 1.0 / (double)fixed;
+            auto count = [&](int bin, float share) {         // share: w / W
+                atomicAdd(&sh.count[bin], 1u);
+                const uint32_t d = __float2uint_rn((1.0f - share) * fixed);
+                if (d) atomicAdd(&sh.delta[bin], d);
+            };
+            // the cluster's histogram from those of its CTAs: each CTA adds up a share of the bins, two CTAs' a thread, and tells all
+            auto join = [&]() {
+                cluster_sync_all();
+                const int bins = BINS / ctas, b = tid % bins, g = tid / bins, groups = THREADS / bins;       // ctas = 1: two bins a thread
+                if (ctas == 1) {
+                    for (int i = tid; i < BINS; i += THREADS) { sh.all_count[i] = sh.count[i]; sh.all_delta[i] = sh.delta[i]; sh.count[i] = sh.delta[i] = 0; }
+                } else {
+                    const int mine = rank * bins + b;
+                    uint32_t c = 0;
+                    unsigned long long d = 0;
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        const uint32_t from = g * 2 + j;
+                        c += ld_cluster_u32(mapa_shared(smem_u32(&sh.count[mine]), from));
+                        d += ld_cluster_u32(mapa_shared(smem_u32(&sh.delta[mine]), from));
+                    }
+                    sh.part_count[tid] = c;
+                    sh.part_delta[tid] = d;
+                    __syncthreads();
+                    // every group tells two CTAs
+                    c = 0;
+                    d = 0;
+                    for (int x = 0; x < groups; ++x) { c += sh.part_count[x * bins + b]; d += sh.part_delta[x * bins + b]; }
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        st_cluster_u32(mapa_shared(smem_u32(&sh.all_count[mine]), g * 2 + j), c);
+                        st_cluster_u64(mapa_shared(smem_u32(&sh.all_delta[mine]), g * 2 + j), d);
+                    }
+                    cluster_sync_all();
+                    for (int i = tid; i < BINS; i += THREADS) sh.count[i] = sh.delta[i] = 0;
+                }
+                __syncthreads();
+            };
+            // level 0
+            for (int i = tid; i < ns; i += THREADS) {
+                float within;
+                const int b = bin_of(at(i), within);
+                if (b < BINS) count(b, exp2f(within * -0.0625f));
+            }
+            join();
+            const uint32_t c0 = sh.all_count[2 * tid], c1 = sh.all_count[2 * tid + 1];
+            const double w0 = exp2((double)(2 * tid) * -0.0625), w1 = w0 * 0.95760328069857364694;
+            const double m0 = w0 * ((double)c0 - (double)sh.all_delta[2 * tid] * unit), m1 = w1 * ((double)c1 - (double)sh.all_delta[2 * tid + 1] * unit);
+            const Scan first = scan(sh, c0 + c1, m0 + m1);
+            double mass = first.mass_all;                    // of what top-k keeps
+
+            for (int what = need_k ? 0 : 1; what <= (need_p ? 1 : 0); ++what) {
+                const double want = fmax((double)p * mass, 1e-30);       // of mass, for top-p
+                // The bin with the border, from this thread's two: the first whose end reaches what is wanted; the last one with tokens if rounding keeps
+                // all from it.  Its number, tokens and mass, and those ahead of it.
+                auto find = [&](uint32_t over, double over_mass, uint32_t x0, double y0, uint32_t x1, double y1, const Scan& s, uint32_t beyond) {
+                    if (tid == 0) sh.found_bin = BINS;
+                    __syncthreads();
+                    const uint32_t e0 = over + s.before + x0, e1 = e0 + x1;
+                    const double f0 = over_mass + s.mass_before + y0, f1 = f0 + y1;
+                    const bool r0 = what == 0 ? e0 >= (uint32_t)k : x0 > 0 && f0 >= want, r1 = what == 0 ? e1 >= (uint32_t)k : x1 > 0 && f1 >= want;
+                    if (r0) atomicMin(&sh.found_bin, 2u * tid);
+                    else if (r1) atomicMin(&sh.found_bin, 2u * tid + 1);
+                    __syncthreads();
+                    if (what == 1 && sh.found_bin == BINS) {
+                        const bool last = x0 + x1 > 0 && s.before + x0 + x1 == s.all;        // one thread's alone
+                        __syncthreads();
+                        if (last) sh.found_bin = x1 > 0 ? 2u * tid + 1 : 2u * tid;
+                        __syncthreads();
+                    }
+                    const uint32_t b = sh.found_bin;
+                    if (b / 2 == tid) {
+                        const bool odd = b & 1;
+                        sh.found_count = odd ? x1 : x0;
+                        sh.found_mass = odd ? y1 : y0;
+                        sh.found_over = over + s.before + (odd ? x0 : 0u);
+                        sh.found_over_mass = over_mass + s.mass_before + (odd ? y0 : 0.0);
+                    }
+                    if (b == BINS && tid == 0) {             // top-k's border lies beyond the bins
+                        sh.found_count = beyond;
+                        sh.found_mass = 0.0;
+                        sh.found_over = over + s.all;
+                        sh.found_over_mass = over_mass + s.mass_all;
+                    }
+                    __syncthreads();
+                };
+                find(0, 0.0, c0, m0, c1, m1, first, (uint32_t)n - first.all);
+                const int bin = (int)sh.found_bin;
+                uint32_t left = sh.found_count, over = sh.found_over;
+                double over_mass = sh.found_over_mass;
+                int part = -1;
+                if (left > FEW && bin < BINS) {              // level 1
+                    for (int i = tid; i < ns; i += THREADS) {
+                        float within;
+                        if (bin_of(at(i), within) == bin) count(min((int)(within * (float)BINS), BINS - 1), exp2f(within * -0.0625f));
+                    }
+                    join();
+                    const double w = exp2((double)bin * -0.0625);
+                    const uint32_t x0 = sh.all_count[2 * tid], x1 = sh.all_count[2 * tid + 1];
+                    const double y0 = w * ((double)x0 - (double)sh.all_delta[2 * tid] * unit), y1 = w * ((double)x1 - (double)sh.all_delta[2 * tid + 1] * unit);
+                    const Scan s = scan(sh, x0 + x1, y0 + y1);
+                    find(over, over_mass, x0, y0, x1, y1, s, 0);
+                    part = (int)sh.found_bin;
+                    left = sh.found_count;
+                    over = sh.found_over;
+                    over_mass = sh.found_over_mass;
+                }
+                // whether a token is among those that are left
+                uint32_t lo = 0, hi = 0xffffffffu;
+                bool by_key = false;
+                auto in = [&](float v) {
+                    if (by_key) { const uint32_t o = order_of(v); return o >= lo && o <= hi; }
+                    float within;
+                    const int b = bin_of(v, within);
+                    return b == bin && (part < 0 || min((int)(within * (float)BINS), BINS - 1) == part);
+                };
+                for (int turn = 0; left > FEW; ++turn) {
+                    uint32_t l = 0xffffffffu, h = 0;
+                    for (int i = tid; i < ns; i += THREADS) {
+                        const float v = at(i);
+                        if (in(v)) { l = min(l, order_of(v)); h = max(h, order_of(v)); }
+                    }
+                    l = __reduce_min_sync(0xffffffffu, l);
+                    h = __reduce_max_sync(0xffffffffu, h);
+                    if (lane == 0) { sh.part_count[warp] = l; sh.part_count[WARPS + warp] = h; }
+                    __syncthreads();
+                    if (tid < ctas) {
+                        for (int w = 0; w < WARPS; ++w) { l = min(l, sh.part_count[w]); h = max(h, sh.part_count[WARPS + w]); }
+                        st_cluster_u32(mapa_shared(smem_u32(&sh.cta_lo[turn & 1][rank]), tid), l);
+                        st_cluster_u32(mapa_shared(smem_u32(&sh.cta_hi[turn & 1][rank]), tid), h);
+                    }
+                    cluster_sync_all();
+                    lo = 0xffffffffu;
+                    hi = 0;
+                    for (int c = 0; c < ctas; ++c) { lo = min(lo, sh.cta_lo[turn & 1][c]); hi = max(hi, sh.cta_hi[turn & 1][c]); }
+                    by_key = true;
+                    if (lo == hi) break;
+                    const int shift = max(0, 22 - __clz(hi - lo));               // (hi - lo) >> shift < 1024
+                    const float w_top = weights.of(value_of(hi)), back = 1.0f / w_top;           // beyond the bins mass does not count
+                    for (int i = tid; i < ns; i += THREADS) {
+                        const float v = at(i);
+                        if (in(v)) count((int)((hi - order_of(v)) >> shift), bin < BINS ? fminf(weights.of(v) * back, 1.0f) : 1.0f);
+                    }
+                    join();
+                    const uint32_t x0 = sh.all_count[2 * tid], x1 = sh.all_count[2 * tid + 1];
+                    const double w = (double)w_top;
+                    const double y0 = w * ((double)x0 - (double)sh.all_delta[2 * tid] * unit), y1 = w * ((double)x1 - (double)sh.all_delta[2 * tid + 1] * unit);
+                    const Scan s = scan(sh, x0 + x1, y0 + y1);
+                    find(over, over_mass, x0, y0, x1, y1, s, 0);
+                    const uint32_t b = sh.found_bin;
+                    left = sh.found_count;
+                    over = sh.found_over;
+                    over_mass = sh.found_over_mass;
+                    hi -= b << shift;
+                    lo = max(lo, hi - min(hi, (1u << shift) - 1u));
+                }
+                uint32_t border, border_ties;
+                if (left > FEW) {                            // equal ones only
+                    const double w = (double)weights.of(value_of(lo));
+                    border = lo;
+                    border_ties = what == 0 ? (uint32_t)k - over : w > 0.0 ? (uint32_t)fmin(fmax(ceil((want - over_mass) / w), 1.0), (double)left) : left;
+                    mass = over_mass + (double)border_ties * w;
+                } else {
+                    // the last ones, put in order by a warp of every CTA
+                    for (int i = tid; i < ns; i += THREADS) {
+                        const float v = at(i);
+                        if (in(v)) {
+                            const uint32_t slot = atomicAdd(&sh.list_n[what], 1u);
+                            if (slot < FEW) sh.list[what][slot] = order_of(v);
+                        }
+                    }
+                    cluster_sync_all();
+                    if (warp == 0) {
+                        uint32_t mine = 0;
+                        int base = 0;
+                        for (int c = 0; c < ctas; ++c) {
+                            const int m = (int)ld_cluster_u32(mapa_shared(smem_u32(&sh.list_n[what]), c));
+                            if (lane >= base && lane < base + m) mine = ld_cluster_u32(mapa_shared(smem_u32(&sh.list[what][lane - base]), c));
+                            base += m;
+                        }
+                        int place = 0;
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) {
+                            const uint32_t x = __shfl_sync(0xffffffffu, mine, j);
+                            place += x > mine || (x == mine && j < lane);
+                        }
+                        sh.part_count[place] = mine;
+                        __syncwarp();
+                        mine = sh.part_count[lane];                              // falling; lanes from `left` on have none
+                        const double w = lane < (int)left ? (double)weights.of(value_of(mine)) : 0.0;
+                        double upto = w;
+#pragma unroll
+                        for (int o = 1; o < 32; o <<= 1) {
+                            const double x = __shfl_up_sync(0xffffffffu, upto, o);
+                            if (lane >= o) upto += x;
+                        }
+                        const bool kept = lane < (int)left && (what == 0 ? over + lane < (uint32_t)k : lane == 0 || over_mass + (upto - w) < want);
+                        const unsigned int who = __ballot_sync(0xffffffffu, kept);
+                        const int last = 31 - __clz(who | 1u);                   // a head of the order
+                        const uint32_t of_last = __shfl_sync(0xffffffffu, mine, last);
+                        const unsigned int same = __ballot_sync(0xffffffffu, kept && mine == of_last && lane <= last);
+                        const double sum = __shfl_sync(0xffffffffu, upto, last);
+                        if (lane == 0) { sh.cut = of_last; sh.ties = __popc(same); sh.cut_mass = over_mass + sum; }
+                    }
+                    __syncthreads();
+                    border = sh.cut;
+                    border_ties = sh.ties;
+                    mass = sh.cut_mass;
+                }
+                if (border > cut) {                          // top-p's border may be rounded behind top-k's, which then stays
+                    cut = border;
+                    ties = border_ties;
+                } else if (border == cut) {
+                    ties = min(ties, border_ties);
+                }
+            }
         }
         if (mp > 0.0f) {
-            const double least = (double)mx + (double)t * log((double)mp);
-            const float f = __double2float_ru(least);
-            const uint32_t c = order_of(f);
-            if (c > cut) { cut = c; ties = n; }
+            const uint32_t least = order_of(__double2float_ru((double)mx + (double)t * log(fmin((double)mp, 1.0))) + 0.0f);
+            if (least > cut) { cut = least; ties = 0x7fffffffu; }
         }
-        // contiguous ranges a thread: equal keys before it, then running sums
-        const int per = (n + THREADS - 1) / THREADS, i0 = min(n, tid * per), i1 = min(n, i0 + per);
-        auto scan = [&](double v) {                              // prefix[t] = sum of the threads before t
-            __syncthreads();
-            prefix[tid + 1] = v;
-            __syncthreads();
-            if (tid == 0) { prefix[0] = 0; for (int i = 0; i < THREADS; ++i) prefix[i + 1] += prefix[i]; }
-            __syncthreads();
-        };
-        double same = 0;
-        for (int i = i0; i < i1; ++i) same += key(i) == cut;
-        scan(same);
-        const double rank0 = prefix[tid];
-        auto walk = [&](auto each) {
-            double rank = rank0;
-            for (int i = i0; i < i1; ++i) {
-                const uint32_t x = key(i);
-                if (x > cut || (x == cut && rank < ties)) each(i, weight(x));
-                rank += x == cut;
-            }
-        };
-        double sum = 0;
-        walk([&](int, double w) { sum += w; });
-        scan(sum);
-        if (tid == 0) s_token = 0x7fffffff;
-        __syncthreads();
-        int u_at = row;
-        if (a.step) u_at = min(max(a.step[0], 0), a.random_count - 1);
-        const float u = a.random[u_at];
-        const double all = prefix[THREADS], want = fmin(fmax(u, 0.0f), 1.0f) * all;
-        double run = prefix[tid];
-        int found = 0x7fffffff, lastw = -1;
-        walk([&](int i, double w) { run += w; if (w > 0) lastw = i; if (found == 0x7fffffff && w > 0 && run > want) found = i; });
-        if (found != 0x7fffffff) atomicMin(&s_token, found);
-        __syncthreads();
-        if (s_token == 0x7fffffff) {                             // random rounds up to the whole sum: the last one
-            __syncthreads();
-            if (tid == 0) s_token = -1;
-            __syncthreads();
-            if (lastw >= 0) atomicMax(&s_token, lastw);
-            __syncthreads();
-        }
-        token = s_token;
-        prob = (float)(weight(key(token)) / all);
     }
-    if (tid == 0) {
-        a.tokens[row] = token;
-        if (a.prob) a.prob[row] = prob;
+
+    // ---- running sums by index: neighbouring tokens a thread, an odd number of them (no bank conflicts).  Weights as integers, 2^42 the largest:
+    // sums of up to 2^20 of them are exact, and the same whoever adds them up, so that exactly one thread has the token. ----
+    constexpr float ONE = 4398046511104.0f;
+    const int per = ((ns + THREADS - 1) / THREADS) | 1, i0 = min(ns, tid * per), i1 = min(ns, i0 + per);
+    unsigned long long above = 0;
+    uint32_t same = 0;
+    for (int i = i0; i < i1; ++i) {
+        const float v = at(i);
+        const uint32_t o = order_of(v);
+        if (o > cut) above += __float2ull_rn(weights.of(v) * ONE);
+        same += o == cut;
+    }
+    unsigned long long upto = above;
+    uint32_t same_upto = same;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const unsigned long long x = __shfl_up_sync(0xffffffffu, upto, o);
+        const uint32_t y = __shfl_up_sync(0xffffffffu, same_upto, o);
+        if (lane >= o) { upto += x; same_upto += y; }
+    }
+    __syncthreads();
+    if (lane == 31) { sh.part_delta[warp] = upto; sh.part_count[warp] = same_upto; }
+    __syncthreads();
+    unsigned long long cta_above = 0;
+    uint32_t cta_ties = 0;
+    upto -= above;                                       // ahead of this thread
+    same_upto -= same;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) {
+        if (w < warp) { upto += sh.part_delta[w]; same_upto += sh.part_count[w]; }
+        cta_above += sh.part_delta[w];
+        cta_ties += sh.part_count[w];
+    }
+    if (tid < ctas) {
+        st_cluster_u32(mapa_shared(smem_u32(&sh.cta_ties[rank]), tid), cta_ties);
+        st_cluster_u64(mapa_shared(smem_u32(&sh.cta_above[rank]), tid), cta_above);
+    }
+    cluster_sync_all();
+    unsigned long long total = 0;
+    uint32_t all_ties = 0;
+    for (int c = 0; c < ctas; ++c) {
+        if (c < rank) { upto += sh.cta_above[c]; same_upto += sh.cta_ties[c]; }
+        total += sh.cta_above[c];
+        all_ties += sh.cta_ties[c];
+    }
+    const float w_cut = none ? 1.0f : weights.of(value_of(cut));
+    const unsigned long long one_tie = __float2ull_rn(w_cut * ONE);
+    total += one_tie * min(all_ties, ties);
+    const unsigned long long target = min((unsigned long long)(fmin(fmax((double)random, 0.0), 1.0) * (double)total), total - 1);
+    const unsigned long long begin = upto + one_tie * min(same_upto, ties), end = upto + above + one_tie * min(same_upto + same, ties);
+    if (begin <= target && target < end) {
+        unsigned long long run = begin;
+        float w = 0.0f;
+        int i = i0;
+        for (;; ++i) {
+            const float v = at(i);
+            const uint32_t o = order_of(v);
+            if (o > cut || (o == cut && same_upto < ties)) {
+                w = o == cut ? w_cut : weights.of(v);
+                run += __float2ull_rn(w * ONE);
+                if (run > target) break;
+            }
+            same_upto += o == cut;
+        }
+        a.tokens[row] = n0 + i;
+        if (a.prob) a.prob[row] = (float)((double)w * (double)ONE / (double)total);
         if (a.step) {
             const int step = a.step[0];
-            if (a.history && step >= 0 && step < a.history_capacity) a.history[step] = token;
-            a.step[0] += 1;
+            if (a.history && step >= 0 && step < a.history_capacity) a.history[step] = n0 + i;
+            a.step[0] = step + 1;
             a.pos[0] += 1;
             a.len[0] += 1;
         }

@@ -56,7 +56,7 @@ bool make_codes_map(CUtensorMap* map, const twm_cache8* c, void* codes)
 
 // Lets a kernel take more than 48 KB of shared memory on the current device.  The limit belongs to the function: it is set once a device, to what
 // every launch of it asks for.
-twm_status allow_shared(const char* name, const void* kernel, size_t bytes)
+twm_status allow_shared(const char* name, const void* kernel, size_t bytes, bool wide_clusters = false)
 {
     static std::mutex mutex;
     static std::vector<std::pair<const void*, int>> done;
@@ -66,7 +66,9 @@ twm_status allow_shared(const char* name, const void* kernel, size_t bytes)
         std::lock_guard<std::mutex> lock(mutex);
         for (const auto& x : done)
             if (x.first == kernel && x.second == dev) return TWM_OK;
-        if ((e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes)) == cudaSuccess) done.emplace_back(kernel, dev);
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+        if (e == cudaSuccess && wide_clusters) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        if (e == cudaSuccess) done.emplace_back(kernel, dev);
     }
     if (e == cudaSuccess) return TWM_OK;
     set_error(name, e);
@@ -81,6 +83,22 @@ twm_status launch_few(const twm::cache8::AttnArgs& a, const AttnPlan& p, int fla
     const twm_status st = allow_shared("twm_cache8_attention", (const void*)kernel, smem);
     if (st != TWM_OK) return st;
     return launch_op("twm_cache8_attention", kernel, dim3(p.ctas), dim3(twm::cache8::FEW_THREADS), smem, flags, stream, a);
+}
+
+// The CTAs of a row: slices of at most 24000 logits, of which two fit an SM, and where there are few rows more of them, down to 2048 logits.
+template <typename T>
+twm_status launch_sample(const twm_sample_args& a, int flags, void* stream)
+{
+    const int most = a.rows <= 8 ? 16 : a.rows <= 36 ? 8 : 1;
+    int ctas = 1;
+    while (ctas < 16 && (a.vocab > 24000L * ctas || (ctas < most && a.vocab > 2048L * ctas))) ctas *= 2;
+    const int slice = (int)((((long)a.vocab + ctas - 1) / ctas + 15) / 16 * 16);
+    auto* kernel = twm::sample::sample_kernel<T>;
+    static_assert(twm::sample::MAX_SLICE * 4 + sizeof(twm::sample::Shared) + 1024 < 227 * 1024, "shared memory of a CTA");
+    const twm_status st = allow_shared("twm_sample", (const void*)kernel, twm::sample::MAX_SLICE * 4, true);
+    if (st != TWM_OK) return st;
+    return launch_cluster("twm_sample", kernel, dim3(a.rows, ctas), dim3(twm::sample::THREADS), 4 * (size_t)std::min(slice, twm::sample::MAX_SLICE), flags, ctas,
+                          stream, a, slice);
 }
 
 }  // namespace
@@ -143,17 +161,17 @@ twm_status twm_cache8_attention(const twm_cache8* cache, void* out, long ldo, co
 
 twm_status twm_sample(const twm_sample_args* args, int flags, void* stream)
 {
-    if (!args || !args->logits || !args->random || !args->tokens || args->rows < 1 || args->vocab < 1 || args->ld < args->vocab) return TWM_EINVAL;
+    if (!args || !args->logits || !args->random || !args->tokens || args->rows < 1 || args->vocab < 1 || args->vocab > (1 << 20) ||
+        args->ld < args->vocab)
+        return TWM_EINVAL;
     if (args->dtype != TWM_F32 && args->dtype != TWM_F16 && args->dtype != TWM_BF16) return TWM_EINVAL;
     if (args->step && (args->rows != 1 || args->random_count < 1 || !args->pos || !args->len || (args->history && args->history_capacity < 1)))
         return TWM_EINVAL;
     if (reinterpret_cast<uintptr_t>(args->logits) & (args->dtype == TWM_F32 ? 3 : 1)) return TWM_EALIGN;
     const twm_status st = ensure_device(nullptr);
     if (st != TWM_OK) return st;
-    auto* kernel = args->dtype == TWM_F32   ? twm::sample::sample_kernel<float>
-                   : args->dtype == TWM_F16 ? twm::sample::sample_kernel<__half>
-                                            : twm::sample::sample_kernel<__nv_bfloat16>;
-    return launch_op("twm_sample", kernel, dim3(args->rows), dim3(twm::sample::THREADS), 0, flags, stream, *args);
+    if (args->dtype == TWM_F32) return launch_sample<float>(*args, flags, stream);
+    return args->dtype == TWM_F16 ? launch_sample<__half>(*args, flags, stream) : launch_sample<__nv_bfloat16>(*args, flags, stream);
 }
 
 }  // extern "C"

@@ -72,7 +72,7 @@ def sample_args(**kw):
 def test_sampling_that_is_refused(twm_lib):
     assert twm_lib.twm_sample(None, 0, None) == _lib.TWM_EINVAL
     loop = dict(step=0x4000, random_count=3, pos=0x5000, len=0x6000)
-    for bad in (dict(rows=0), dict(vocab=0), dict(dtype=3), dict(logits=None), dict(ld=99), dict(random=None), dict(tokens=None),
+    for bad in (dict(rows=0), dict(vocab=0), dict(vocab=(1 << 20) + 1, ld=1 << 21), dict(dtype=3), dict(logits=None), dict(ld=99), dict(random=None), dict(tokens=None),
                 dict(loop, rows=2), dict(loop, random_count=0), dict(loop, pos=None), dict(loop, len=None), dict(loop, history=0x7000, history_capacity=0)):
         assert twm_lib.twm_sample(sample_args(**bad), 0, None) == _lib.TWM_EINVAL, bad
     assert twm_lib.twm_sample(sample_args(logits=0x1002), 0, None) == _lib.TWM_EALIGN
