@@ -1,0 +1,343 @@
+// twm_cache8_prompt.cuh — softmax attention of many rows over the cache held in 8 bits, on the 5th-generation tensor cores.
+//
+// A tile is 256 rows, two MMA tiles of 128, which share every unit of 64 keys and values; a CTA takes an equal run of all units (see
+// twm_cache8_attn.cuh, also for the mathematics).
+//   warp 12     TMA: the units' codes, into a ring.
+//   warps 8-11  codes to FP16, exactly, into the swizzled layout the MMAs read (rows of 64 elements, 128 bytes); a unit of the tail is copied instead.
+//               Lanes take four chunks of 16 codes of rows r and r ^ 5, so that neither the reads nor the writes meet in a bank.
+//   warp 13     one thread issues tcgen05.mma: the scores of unit u + 1 of both halves, then P V of unit u (P from tensor memory).
+//   warps 0-7   thread = row: maximum, weights, sum; the reference of the exponents moves only when a factor would pass 2^8, and then the row's output is
+//               scaled in tensor memory ahead of the unit's P V.  They bring the rows' queries to shared memory and store the results.
+// Tensor memory: two score buffers of 64 columns and D of output for each half; the factors, FP16, overwrite the scores.
+// Sharing a unit between two halves is what shared memory asks for: a unit costs 16 KB read and 32 KB written by the conversion and 64 KB read by
+// each half's MMAs, 1400 clocks at 128 bytes each for 256 rows against 1024 of MMA and 1024 of exponentials; with 128 rows it would be 1800.
+#pragma once
+
+#include "twm_cache8_attn.cuh"
+#include "twm_gemm_tcw.cuh"
+
+namespace twm {
+namespace cache8 {
+
+constexpr int PROMPT_ROWS = 256, PROMPT_THREADS = 448;
+template <int D>
+struct Prompt {
+    static constexpr int BOXES = D / 64;
+    static constexpr int QBOX = 128 * 128, KBOX = BLOCK * 128;           // bytes of 64 elements of 128 rows, of a unit's keys
+    static constexpr int RAW = 2 * BLOCK * D, RAWS = 3;                  // a unit's codes; units in the ring
+    static constexpr int UNIT = 2 * BOXES * KBOX, UNITS = 3;             // ... as FP16
+    static constexpr int TMEM = 512, HALF = 256, OUT = 128;              // columns: of all, of a half, where its output is
+    static constexpr size_t SMEM = 1024 + 2 * BOXES * (size_t)QBOX + UNITS * (size_t)UNIT + RAWS * (size_t)RAW;
+};
+
+__device__ __forceinline__ uint64_t row_desc(uint32_t addr)             // K-major, 128-byte swizzle
+{
+    return (uint64_t)((addr & 0x3FFFF) >> 4) | ((uint64_t)1 << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+__device__ __forceinline__ uint64_t value_desc(uint32_t addr, uint32_t box)      // columns contiguous, the next 64 in the next box
+{
+    return (uint64_t)((addr & 0x3FFFF) >> 4) | ((uint64_t)(box >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+__device__ __forceinline__ bool elect_one()
+{
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+    return p != 0;
+}
+
+template <int D>
+__global__ void __launch_bounds__(PROMPT_THREADS, 1)
+prompt_kernel(const __grid_constant__ AttnArgs a)
+{
+    using P = Prompt<D>;
+    extern __shared__ uint8_t prompt_raw[];
+    __shared__ uint64_t raw_full[P::RAWS], raw_empty[P::RAWS], unit_full[P::UNITS], unit_empty[P::UNITS], q_full, s_full[2][2], p_full[2], o_done[2];
+    __shared__ uint32_t s_tmem;
+    __shared__ int s_abort;
+    uint8_t* qs = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(prompt_raw) + 1023) & ~(uintptr_t)1023);
+    uint8_t* units = qs + 2 * P::BOXES * P::QBOX;
+    uint8_t* raws = units + P::UNITS * P::UNIT;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    if (tid == 0) {
+        for (int i = 0; i < P::RAWS; ++i) { mbar_init(&raw_full[i], 1); mbar_init(&raw_empty[i], 4); }
+        for (int i = 0; i < P::UNITS; ++i) { mbar_init(&unit_full[i], 4); mbar_init(&unit_empty[i], 1); }
+        mbar_init(&q_full, 8);
+        for (int x = 0; x < 2; ++x) {
+            mbar_init(&s_full[x][0], 1);
+            mbar_init(&s_full[x][1], 1);
+            mbar_init(&p_full[x], 4);
+            mbar_init(&o_done[x], 1);
+        }
+        s_abort = 0;
+        mbar_fence_init();
+    }
+    // tensor memory is asked for once the kernel before has given its own back: an allocation waits without a limit
+    pdl_wait_prior_grids();
+    const Deal deal = {a.num_heads / a.c.kv_heads, PROMPT_ROWS, a.window};
+    const Start start = find_start<PROMPT_THREADS>(a, deal, blockIdx.x, gridDim.x);
+    zero_rows(a, D, blockIdx.x, gridDim.x, tid, PROMPT_THREADS);
+    if (start.units == 0) return;
+    if (warp == 13) {
+        tc::tmem_alloc(&s_tmem, P::TMEM);
+        tc::tc_fence_before();
+    }
+    __syncthreads();
+    tc::tc_fence_after();
+    pdl_launch_dependents();
+    volatile int* abort_flag = &s_abort;
+    const uint32_t tmem = s_tmem;
+    Walk w;
+    w.begin(a, deal, start);
+
+    if (warp == 12) {
+        if (lane == 0) {
+            int i = 0;
+            bool ok = true;
+            do {
+                const int held = (w.sp.pos + w.sp.n) / BLOCK, row0 = (w.seq * a.c.kv_heads + w.head) * a.c.capacity;
+                for (int u = w.u0; u < min(w.u0 + w.n, held) && ok; ++u, ++i) {
+                    const int slot = i % P::RAWS;
+                    if (i >= P::RAWS) ok = mbar_wait_bounded(&raw_empty[slot], (uint32_t)(i / P::RAWS - 1) & 1u, abort_flag);
+                    if (!ok) break;
+                    mbar_arrive_expect_tx(&raw_full[slot], P::RAW);
+                    tma_load_2d(raws + slot * P::RAW, &a.k_map, 0, row0 + u * BLOCK, &raw_full[slot]);
+                    tma_load_2d(raws + slot * P::RAW + BLOCK * D, &a.v_map, 0, row0 + u * BLOCK, &raw_full[slot]);
+                }
+            } while (ok && w.next(a, deal));
+        }
+        __syncwarp();
+    } else if (warp == 13) {
+        if (elect_one()) {
+            constexpr uint32_t idesc_s = (1u << 4) | ((uint32_t)(BLOCK >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);               // D f32, A and B f16
+            constexpr uint32_t idesc_o = (1u << 4) | (1u << 16) | ((uint32_t)(D >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);     // B: columns contiguous
+            int i = 0, tile = 0, n[2] = {0, 0};          // units so far, tiles, units of a half
+            bool ok = true;
+            do {
+                const int halves = min(PROMPT_ROWS, w.sp.n * deal.group - w.t * PROMPT_ROWS) > 128 ? 2 : 1;
+                ok = mbar_wait_bounded(&q_full, (uint32_t)tile & 1u, abort_flag);
+                tc::tc_fence_after();
+                for (int u = 0; u <= w.n && ok; ++u) {
+                    if (u < w.n) {
+                        const int slot = (i + u) % P::UNITS;
+                        ok = mbar_wait_bounded(&unit_full[slot], (uint32_t)((i + u) / P::UNITS) & 1u, abort_flag);
+                        if (!ok) break;
+                        tc::tc_fence_after();
+                        const uint32_t ks = smem_u32(units + slot * P::UNIT);
+                        for (int x = 0; x < halves; ++x) {
+                            const int buffer = (n[x] + u) & 1;
+                            const uint32_t q = smem_u32(qs + x * P::BOXES * P::QBOX);
+#pragma unroll
+                            for (int c = 0; c < D / 16; ++c)
+                                tcw::mma_ss(tmem + x * P::HALF + buffer * BLOCK, row_desc(q + (c >> 2) * P::QBOX + (c & 3) * 32),
+                                            row_desc(ks + (c >> 2) * P::KBOX + (c & 3) * 32), idesc_s, c == 0 ? 0u : 1u);
+                            tc::tc_commit(&s_full[x][buffer]);
+                        }
+                    }
+                    if (u > 0) {
+                        const int slot = (i + u - 1) % P::UNITS;
+                        const uint32_t vs = smem_u32(units + slot * P::UNIT + P::BOXES * P::KBOX);
+                        for (int x = 0; x < halves && ok; ++x) {
+                            const int mine = n[x] + u - 1;
+                            ok = mbar_wait_bounded(&p_full[x], (uint32_t)mine & 1u, abort_flag);
+                            if (!ok) break;
+                            tc::tc_fence_after();
+                            const uint32_t at = tmem + x * P::HALF;
+#pragma unroll
+                            for (int c = 0; c < BLOCK / 16; ++c)
+                                tc::tc_mma_ts(at + P::OUT, at + (mine & 1) * BLOCK + c * 8, value_desc(vs + c * 2048, P::KBOX), idesc_o, (u == 1 && c == 0) ? 0u : 1u);
+                            tc::tc_commit(&o_done[x]);
+                        }
+                        tc::tc_commit(&unit_empty[slot]);
+                    }
+                }
+                i += w.n;
+                for (int x = 0; x < halves; ++x) n[x] += w.n;
+                ++tile;
+            } while (ok && w.next(a, deal));
+        }
+        __syncwarp();
+    } else if (warp >= 8) {
+        // ---- codes to FP16 ----
+        const int me = tid - 256;
+        int i = 0, r = 0;                                 // units, units of codes
+        do {
+            const int length = w.sp.pos + w.sp.n, held = length / BLOCK;
+            const size_t at = (size_t)w.seq * a.c.kv_heads + w.head;
+            for (int u = w.u0; u < w.u0 + w.n; ++u, ++i) {
+                const int slot = i % P::UNITS;
+                if (i >= P::UNITS) tc::wait_uniform(&unit_empty[slot], (uint32_t)(i / P::UNITS - 1) & 1u, abort_flag);
+                uint8_t* dst = units + slot * P::UNIT;
+                auto put = [&](int side, int row, int chunk, const uint4& v) {           // 8 elements
+                    *reinterpret_cast<uint4*>(dst + side * P::BOXES * P::KBOX + (chunk >> 3) * P::KBOX + row * 128 + (((chunk & 7) ^ (row & 7)) << 4)) = v;
+                };
+                if (u < held) {
+                    const int raw = r % P::RAWS;
+                    tc::wait_uniform(&raw_full[raw], (uint32_t)(r / P::RAWS) & 1u, abort_flag);
+                    const uint8_t* src = raws + raw * P::RAW;
+#pragma unroll
+                    for (int j = 0; j < D / 16; ++j) {
+                        // chunk of four, row, keys or values, which four
+                        const int item = j * 128 + me, chunk = (item >> 9) * 4 + (item & 3), side = (item >> 8) & 1, row = (item >> 2) & 63;
+                        // eight lanes take rows r and r ^ 5
+                        const int rr = (row & ~7) | ((row & 1) ? ((row & 7) >> 1) ^ 5 : (row & 7) >> 1);
+                        const uint4 v = D == 128 ? *reinterpret_cast<const uint4*>(src + side * BLOCK * D + rr * 128 + ((chunk ^ (rr & 7)) << 4))
+                                                 : *reinterpret_cast<const uint4*>(src + side * BLOCK * D + rr * 64 + ((chunk ^ ((rr >> 1) & 3)) << 4));
+                        put(side, rr, 2 * chunk, make_uint4(codes_f16(v.x), codes_f16_hi(v.x), codes_f16(v.y), codes_f16_hi(v.y)));
+                        put(side, rr, 2 * chunk + 1, make_uint4(codes_f16(v.z), codes_f16_hi(v.z), codes_f16(v.w), codes_f16_hi(v.w)));
+                    }
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&raw_empty[raw]);
+                    ++r;
+                } else {
+                    const int valid = length - u * BLOCK;
+                    const __half* src[2] = {a.c.k_tail + (at * 2 + (u & 1)) * BLOCK * D, a.c.v_tail + (at * 2 + (u & 1)) * BLOCK * D};
+                    for (int j = me; j < 2 * BLOCK * (D / 8); j += 128) {
+                        const int chunk = j % (D / 8), row = j / (D / 8) % BLOCK, side = j / (D / 8) / BLOCK;
+                        put(side, row, chunk, row < valid ? reinterpret_cast<const uint4*>(src[side] + row * D)[chunk] : make_uint4(0, 0, 0, 0));
+                    }
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&unit_full[slot]);
+            }
+        } while (w.next(a, deal));
+    } else {
+        // ---- rows ----
+        const int x = warp >> 2, row = (warp & 3) * 32 + lane;
+        const uint32_t lane_tmem = tmem + x * P::HALF + ((uint32_t)((warp & 3) * 32) << 16), lane_o = lane_tmem + P::OUT;
+        int n = 0, tile = -1;                             // units of this half; the tile's number
+        do {
+            ++tile;
+            const int row0 = w.t * PROMPT_ROWS, all = min(PROMPT_ROWS, w.sp.n * deal.group - row0);
+            const int r = min(x * 128 + row, all - 1), token = (row0 + r) / deal.group, head = w.head * deal.group + (row0 + r) % deal.group;
+            const bool live = x * 128 + row < all, active = x * 128 < all;
+            const size_t at = (size_t)w.seq * a.c.kv_heads + w.head;
+            if (active) {
+                const uint4* src = reinterpret_cast<const uint4*>(a.q + (size_t)(w.sp.row + token) * a.ldq + head * D);
+                uint8_t* dst = qs + x * P::BOXES * P::QBOX + row * 128;
+#pragma unroll
+                for (int c = 0; c < D / 8; ++c)
+                    *reinterpret_cast<uint4*>(dst + (c >> 3) * P::QBOX + (((c & 7) ^ (row & 7)) << 4)) = live ? src[c] : make_uint4(0, 0, 0, 0);
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            }
+            tc::tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&q_full);
+            if (!active) {                                // not ahead of the others, whose arrivals would be taken for theirs
+                tc::wait_uniform(&q_full, (uint32_t)tile & 1u, abort_flag);
+                continue;
+            }
+            const int held = (w.sp.pos + w.sp.n) / BLOCK, p = w.sp.pos + token;
+            const int first = w.sp.pos + row0 / deal.group, last = w.sp.pos + (row0 + all - 1) / deal.group;       // positions of the tile
+            const float* k_scale = a.c.k_scale + at * (a.c.capacity / BLOCK);
+            const float* v_scale = a.c.v_scale + at * (a.c.capacity / BLOCK);
+            const float base = a.scale * LOG2E;
+            float ks = w.u0 < held ? k_scale[w.u0] : 1.0f, vs = w.u0 < held ? v_scale[w.u0] : 1.0f;
+            float m = -INFINITY, l = 0.0f;
+            for (int j = 0; j < w.n; ++j, ++n) {
+                const int u = w.u0 + j;
+                const float factor = base * ks, inv = power_of_two(-exponent_of(vs)), ev = (float)exponent_of(vs);
+                if (j + 1 < w.n) { ks = u + 1 < held ? k_scale[u + 1] : 1.0f; vs = u + 1 < held ? v_scale[u + 1] : 1.0f; }
+                const uint32_t scores = lane_tmem + (n & 1) * BLOCK;
+                tc::wait_uniform(&s_full[x][n & 1], (uint32_t)(n >> 1) & 1u, abort_flag);
+                tc::tc_fence_after();
+                uint32_t s[4][16];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) tc::tmem_ld<16>(scores + c * 16, s[c]);
+                tc::tmem_wait_ld();
+                if (!((u + 1) * BLOCK - 1 <= first && last - u * BLOCK < a.window)) {
+#pragma unroll
+                    for (int c = 0; c < 4; ++c)
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) {
+                            const int key = u * BLOCK + c * 16 + e;
+                            if (!(key <= p && p - key < a.window)) s[c][e] = __float_as_uint(-INFINITY);
+                        }
+                }
+                float mx[4];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    mx[c] = __uint_as_float(s[c][0]);
+#pragma unroll
+                    for (int e = 1; e < 16; ++e) mx[c] = fmaxf(mx[c], __uint_as_float(s[c][e]));
+                }
+                const float top = fmaf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), factor, ev);
+                float before = 1.0f;
+                const bool moved = top > m + 8.0f;
+                if (moved) {
+                    before = ex2(m - top);
+                    m = top;
+                    l *= before;
+                }
+                const float shift = ev - (m == -INFINITY ? 0.0f : m);
+                float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    uint32_t f[16];
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        const float y = ex2(fmaf(__uint_as_float(s[2 * c + (e >> 3)][2 * e & 15]), factor, shift));
+                        const float z = ex2(fmaf(__uint_as_float(s[2 * c + (e >> 3)][(2 * e & 15) + 1]), factor, shift));
+                        sum[e & 3] += y + z;
+                        f[e] = pack_f16(y, z);
+                    }
+                    tc::tmem_st16(scores + c * 16, f);
+                }
+                l = fmaf((sum[0] + sum[1]) + (sum[2] + sum[3]), inv, l);
+                if (j > 0 && __any_sync(0xffffffffu, moved)) {
+                    // the scores of this unit came after P V of the unit before the last, so the last one's is the phase that is waited for
+                    tc::wait_uniform(&o_done[x], (uint32_t)(n - 1) & 1u, abort_flag);
+                    tc::tc_fence_after();
+                    for (int c = 0; c < D; c += 16) {
+                        uint32_t o[16];
+                        tc::tmem_ld<16>(lane_o + c, o);
+                        tc::tmem_wait_ld();
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * before);
+                        tc::tmem_st16(lane_o + c, o);
+                    }
+                }
+                tc::tmem_wait_st();
+                tc::tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&p_full[x]);
+            }
+            // the last scores say that P V of the unit before the last but one is done; a parity tells only the next phase from it
+            if (n > 1) tc::wait_uniform(&o_done[x], (uint32_t)n & 1u, abort_flag);
+            tc::wait_uniform(&o_done[x], (uint32_t)(n - 1) & 1u, abort_flag);
+            tc::tc_fence_after();
+            const bool alone = w.begins && w.ends, ok = *abort_flag == 0;
+            float* part = a.partial + (2 * (size_t)blockIdx.x + (w.begins ? 1 : 0)) * partial_floats(PROMPT_ROWS, D);
+            __half* out = a.out + (size_t)(w.sp.row + token) * a.ldo + head * D;
+            const float inv_l = 1.0f / l;
+            for (int c = 0; c < D; c += 16) {
+                uint32_t o[16];
+                tc::tmem_ld<16>(lane_o + c, o);
+                tc::tmem_wait_ld();
+                if (!live || !ok) continue;
+                if (alone) {
+#pragma unroll
+                    for (int e = 0; e < 16; e += 8) {
+                        float f[8];
+#pragma unroll
+                        for (int y = 0; y < 8; ++y) f[y] = __uint_as_float(o[e + y]) * inv_l;
+                        *reinterpret_cast<uint4*>(out + c + e) = pack8(f);
+                    }
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 16; e += 4) *reinterpret_cast<uint4*>(part + r * D + c + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                }
+            }
+            if (live && ok && !alone) { part[PROMPT_ROWS * D + r] = m; part[PROMPT_ROWS * (D + 1) + r] = l; }
+        } while (w.next(a, deal));
+    }
+    tc::tc_fence_before();
+    __syncthreads();
+    if (warp == 13) {
+        tc::tc_fence_after();
+        tc::tmem_dealloc(tmem, P::TMEM);
+    }
+}
+
+}  // namespace cache8
+}  // namespace twm

@@ -5,6 +5,7 @@
 
 #include "twm_cache8.cuh"
 #include "twm_cache8_attn.cuh"
+#include "twm_cache8_prompt.cuh"
 #include "twm_sample.cuh"
 
 namespace {
@@ -37,7 +38,7 @@ AttnPlan plan_attention(int group, int max_rows)
     const long rows = (long)max_rows * group;
     if (rows <= 8) return {8, 2 * kDefaultSms};
     if (rows <= 16) return {16, 2 * kDefaultSms};
-    return {32, kDefaultSms};
+    return {twm::cache8::PROMPT_ROWS, kDefaultSms};
 }
 
 // The codes of keys or values as [cached rows][head_dim], a box a block, swizzled over its whole row.
@@ -83,6 +84,17 @@ twm_status launch_few(const twm::cache8::AttnArgs& a, const AttnPlan& p, int fla
     const twm_status st = allow_shared("twm_cache8_attention", (const void*)kernel, smem);
     if (st != TWM_OK) return st;
     return launch_op("twm_cache8_attention", kernel, dim3(p.ctas), dim3(twm::cache8::FEW_THREADS), smem, flags, stream, a);
+}
+
+template <int D>
+twm_status launch_prompt(const twm::cache8::AttnArgs& a, const AttnPlan& p, int flags, void* stream)
+{
+    auto* kernel = twm::cache8::prompt_kernel<D>;
+    constexpr size_t smem = twm::cache8::Prompt<D>::SMEM;
+    static_assert(smem + 1024 < 227 * 1024, "shared memory of a CTA");
+    const twm_status st = allow_shared("twm_cache8_attention", (const void*)kernel, smem);
+    if (st != TWM_OK) return st;
+    return launch_op("twm_cache8_attention", kernel, dim3(p.ctas), dim3(twm::cache8::PROMPT_THREADS), smem, flags, stream, a);
 }
 
 // The CTAs of a row: slices of at most 24000 logits, of which two fit an SM, and where there are few rows more of them, down to 2048 logits.
@@ -150,11 +162,11 @@ twm_status twm_cache8_attention(const twm_cache8* cache, void* out, long ldo, co
         return TWM_ELAUNCH;
     }
     if (D == 64)
-        st = p.tile == 8 ? launch_few<64, 1>(a, p, flags, stream) : p.tile == 16 ? launch_few<64, 2>(a, p, flags, stream) : launch_few<64, 4>(a, p, flags, stream);
+        st = p.tile == 8 ? launch_few<64, 1>(a, p, flags, stream) : p.tile == 16 ? launch_few<64, 2>(a, p, flags, stream) : launch_prompt<64>(a, p, flags, stream);
     else
-        st = p.tile == 8 ? launch_few<128, 1>(a, p, flags, stream) : p.tile == 16 ? launch_few<128, 2>(a, p, flags, stream) : launch_few<128, 4>(a, p, flags, stream);
+        st = p.tile == 8 ? launch_few<128, 1>(a, p, flags, stream) : p.tile == 16 ? launch_few<128, 2>(a, p, flags, stream) : launch_prompt<128>(a, p, flags, stream);
     if (st != TWM_OK) return st;
-    constexpr int each = 1;          // rows of a merging CTA
+    const int each = p.tile == twm::cache8::PROMPT_ROWS ? 16 : 1;        // rows of a merging CTA
     return launch_op("twm_cache8_attention(merge)", D == 64 ? twm::cache8::merge_kernel<64> : twm::cache8::merge_kernel<128>,
                      dim3(p.ctas, (p.tile + each - 1) / each), dim3(twm::cache8::MERGE_THREADS), 0, flags, stream, a, p.tile, each);
 }
