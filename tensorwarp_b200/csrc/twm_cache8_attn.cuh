@@ -19,6 +19,12 @@ namespace cache8 {
 
 constexpr float LOG2E = 1.4426950408889634f;
 
+struct __align__(16) Join {
+    int parts;                   // CTAs that have keys of it; 0: no such tile
+    int rows, row0;              // rows of the tile, and the first of them among those of its sequence and head
+    int head, row;               // key/value head, and the sequence's first row in the call
+    int unused[3];
+};
 struct AttnArgs {
     Cache c;
     Rows r;
@@ -27,6 +33,7 @@ struct AttnArgs {
     long ldo, ldq;
     int num_heads, window;       // window: INT_MAX = all
     float scale;
+    struct Join* joins;          // [CTAs]: the tile that a CTA began and did not end
     float* partial;              // [2 CTAs][tile]: what a CTA has of its first and of its last tile, where others have the rest
     alignas(64) CUtensorMap k_map, v_map;        // bytes [cached rows][D], boxes of a block, swizzled
 };
@@ -42,13 +49,14 @@ __device__ __forceinline__ Tile tile_units(const Span& sp, int t, int tile, int 
     const int rows = sp.n * group, first = sp.pos + t * tile / group, last = sp.pos + (min(rows, (t + 1) * tile) - 1) / group;
     return {(window > first ? 0 : first - window + 1) / BLOCK, last / BLOCK + 1};
 }
+// A tile also takes time of its own, `extra` units' worth, which stand ahead of its units in the line.
 struct Deal {
-    int group, tile, window;
+    int group, tile, window, extra;
     __device__ __forceinline__ int tiles(const Span& sp) const { return (sp.n * group + tile - 1) / tile; }
     __device__ __forceinline__ int units(const Span& sp, int t) const
     {
         const Tile x = tile_units(sp, t, tile, group, window);
-        return x.end - x.lo;
+        return extra + x.end - x.lo;
     }
     // units of one head of a sequence, by all lanes of a warp
     __device__ __forceinline__ long long units_by_warp(const Span& sp) const
@@ -120,9 +128,9 @@ __device__ __forceinline__ Start find_start(const AttnArgs& a, const Deal& deal,
 
 // The tiles of a CTA's run, one after another.
 struct Walk {
-    long long left;              // units of the run behind the current tile
+    long long left;              // of the run, behind the current tile
     int seq, head, t;            // the current tile
-    int u0, n;                   // its first unit and number of units in this run
+    int u0, n;                   // its first unit and number of units in this run; none at all where the run ends with a tile's extra
     bool begins, ends;           // whether the run has the tile's first and last unit
     Span sp;
     Tile whole;
@@ -130,15 +138,17 @@ struct Walk {
     __device__ __forceinline__ void take(const Deal& d, int skip)
     {
         whole = tile_units(sp, t, d.tile, d.group, d.window);
-        u0 = whole.lo + skip;
-        n = (int)min((long long)(whole.end - u0), left);
-        begins = skip == 0;
-        ends = u0 + n == whole.end;
-        left -= n;
+        const int all = d.extra + whole.end - whole.lo, to = (int)min((long long)all, skip + left), from = max(skip - d.extra, 0);
+        u0 = whole.lo + from;
+        n = max(to - d.extra, 0) - from;
+        begins = from == 0;
+        ends = to == all;
+        left -= to - skip;
     }
-    // by all lanes of a warp
-    __device__ __forceinline__ void begin(const AttnArgs& a, const Deal& d, const Start& s)
+    // by all lanes of a warp; false where the run has no unit
+    __device__ __forceinline__ bool begin(const AttnArgs& a, const Deal& d, const Start& s)
     {
+        if (s.units == 0) return false;
         left = s.units;
         seq = s.seq;
         sp = span_of(a.r, seq, a.c.capacity);
@@ -166,6 +176,7 @@ struct Walk {
             t += 32;
         }
         take(d, rest);
+        return n > 0;
     }
     __device__ __forceinline__ bool next(const AttnArgs& a, const Deal& d)
     {
@@ -178,9 +189,17 @@ struct Walk {
             }
         }
         take(d, 0);
-        return true;
+        return n > 0;            // a run that ends with a tile's extra ends ahead of it
     }
 };
+
+// Leaves word for merge_kernel of the run's last tile (`w` stands there), or that there is none.
+__device__ __forceinline__ void leave_word(const AttnArgs& a, const Deal& d, const Walk& w, const Start& s)
+{
+    const int row0 = w.t * d.tile;
+    const bool open = w.n > 0 && w.begins && !w.ends;
+    a.joins[blockIdx.x] = {open ? 1 + (int)((w.whole.end - w.u0 - w.n + s.share - 1) / s.share) : 0, min(d.tile, w.sp.n * d.group - row0), row0, w.head, w.sp.row, {0, 0, 0}};
+}
 
 // Rows of sequences that are out of the call are zeros; CTA `cta` of `ctas` takes its share of the sequences.
 __device__ __forceinline__ void zero_rows(const AttnArgs& a, int D, int cta, int ctas, int tid, int threads)
@@ -210,6 +229,7 @@ __device__ __forceinline__ int exponent_of(float scale) { return (int)(__float_a
 // scores (two 16-byte reads a key, 4 codes a k-step of both registers), and 16 elements of four keys for the output, whose codes
 // are paired by a byte permutation; both reads are free of bank conflicts in the layout that the TMA's swizzle leaves.  P^T needs only a
 // transposition of 8 x 8.  Each warp has its own m; they are joined when the tile ends.
+constexpr int FEW_EXTRA = 1;                                             // a tile's own time, in units
 constexpr int FEW_WARPS = 4, FEW_THREADS = 32 * FEW_WARPS + 32;
 template <int D, int NT>
 struct Few {
@@ -269,13 +289,15 @@ few_kernel(const __grid_constant__ AttnArgs a)
     }
     pdl_launch_dependents();
     pdl_wait_prior_grids();
-    const Deal deal = {a.num_heads / a.c.kv_heads, F::TILE, a.window};
+    const Deal deal = {a.num_heads / a.c.kv_heads, F::TILE, a.window, FEW_EXTRA};
     const Start start = find_start<FEW_THREADS>(a, deal, blockIdx.x, gridDim.x);
     zero_rows(a, D, blockIdx.x, gridDim.x, tid, FEW_THREADS);
-    if (start.units == 0) return;
-    volatile int* abort_flag = &s_abort;
     Walk w;
-    w.begin(a, deal, start);
+    if (!w.begin(a, deal, start)) {
+        if (tid == 0) a.joins[blockIdx.x].parts = 0;
+        return;
+    }
+    volatile int* abort_flag = &s_abort;
 
     if (warp == FEW_WARPS) {
         if (lane == 0) {
@@ -544,11 +566,12 @@ few_kernel(const __grid_constant__ AttnArgs a)
         }
         named_bar_sync(1, 32 * FEW_WARPS);                               // `join` and the statistics are the next tile's
     } while (w.next(a, deal));
+    if (tid == 0) leave_word(a, deal, w, start);
 }
 
 // ------------------------------------------------------------------------------------------------------------- merge --
 // Joins the tiles that several CTAs have keys of: CTA x takes the tile that CTA x of the kernel before began and did not end.  Its parts are
-// the last part of that CTA and the first parts of those behind it, added in that order: the same call gives the same bits.
+// the last part of that CTA and the first parts of those behind it; the same call adds them up in the same order.
 constexpr int MERGE_THREADS = 256;
 template <int D>
 __global__ void __launch_bounds__(MERGE_THREADS)
@@ -559,25 +582,23 @@ merge_kernel(const __grid_constant__ AttnArgs a, int tile, int rows_each)
     __shared__ float red_l[SIDES];
     pdl_launch_dependents();
     pdl_wait_prior_grids();
-    const Deal deal = {a.num_heads / a.c.kv_heads, tile, a.window};
-    const Start start = find_start<MERGE_THREADS>(a, deal, blockIdx.x, gridDim.x);
-    if (start.units == 0) return;
-    Walk w;
-    w.begin(a, deal, start);
-    while (w.left > 0) w.next(a, deal);                                  // the run's last tile
-    if (!w.begins || w.ends) return;
-    const int parts = 1 + (int)((w.whole.end - w.u0 - w.n + start.share - 1) / start.share);
+    const Join w = a.joins[blockIdx.x];
+    const int r0 = blockIdx.y * rows_each, r1 = min(w.rows, r0 + rows_each);
+    if (w.parts == 0 || r0 >= r1) return;
+    const int group = a.num_heads / a.c.kv_heads;
     const size_t each = partial_floats(tile, D);
     const float* base = a.partial + (2 * (size_t)blockIdx.x + 1) * each;         // part j > 0: the first of CTA x + j
     auto part = [&](int j) { return j == 0 ? base : base + (2 * (size_t)j - 1) * each; };
-    const int rows = min(tile, w.sp.n * deal.group - w.t * tile), side = threadIdx.x / LANES, lane = threadIdx.x % LANES;
-    for (int r = blockIdx.y * rows_each; r < min(rows, (blockIdx.y + 1) * rows_each); ++r) {
+    const int side = threadIdx.x / LANES, lane = threadIdx.x % LANES;
+    for (int r = r0; r < r1; ++r) {
         float top = -INFINITY;
-        for (int j = 0; j < parts; ++j) top = fmaxf(top, part(j)[tile * D + r]);
+#pragma unroll 4
+        for (int j = 0; j < w.parts; ++j) top = fmaxf(top, part(j)[tile * D + r]);
         const float ref = top == -INFINITY ? 0.0f : top;
         float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
         float l = 0.0f;
-        for (int j = side; j < parts; j += SIDES) {
+#pragma unroll 4
+        for (int j = side; j < w.parts; j += SIDES) {
             const float* p = part(j);
             const float f = ex2(p[tile * D + r] - ref);
             const float4 x = reinterpret_cast<const float4*>(p + r * D)[lane];
@@ -594,8 +615,8 @@ merge_kernel(const __grid_constant__ AttnArgs a, int tile, int rows_each)
                 l += red_l[x];
             }
             const float n = 1.0f / l;
-            const int row = w.t * tile + r;
-            __half* dst = a.out + (size_t)(w.sp.row + row / deal.group) * a.ldo + (w.head * deal.group + row % deal.group) * D + lane * 4;
+            const int row = w.row0 + r;
+            __half* dst = a.out + (size_t)(w.row + row / group) * a.ldo + (w.head * group + row % group) * D + lane * 4;
             *reinterpret_cast<uint2*>(dst) = make_uint2(pack_f16(v.x * n, v.y * n), pack_f16(v.z * n, v.w * n));
         }
         __syncthreads();

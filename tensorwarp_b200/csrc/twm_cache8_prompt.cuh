@@ -20,6 +20,7 @@ namespace twm {
 namespace cache8 {
 
 constexpr int PROMPT_ROWS = 256, PROMPT_THREADS = 448;
+constexpr int PROMPT_EXTRA = 3;                                          // a tile's own time, in units
 template <int D>
 struct Prompt {
     static constexpr int BOXES = D / 64;
@@ -73,10 +74,14 @@ prompt_kernel(const __grid_constant__ AttnArgs a)
     }
     // tensor memory is asked for once the kernel before has given its own back: an allocation waits without a limit
     pdl_wait_prior_grids();
-    const Deal deal = {a.num_heads / a.c.kv_heads, PROMPT_ROWS, a.window};
+    const Deal deal = {a.num_heads / a.c.kv_heads, PROMPT_ROWS, a.window, PROMPT_EXTRA};
     const Start start = find_start<PROMPT_THREADS>(a, deal, blockIdx.x, gridDim.x);
     zero_rows(a, D, blockIdx.x, gridDim.x, tid, PROMPT_THREADS);
-    if (start.units == 0) return;
+    Walk w;
+    if (!w.begin(a, deal, start)) {
+        if (tid == 0) a.joins[blockIdx.x].parts = 0;
+        return;
+    }
     if (warp == 13) {
         tc::tmem_alloc(&s_tmem, P::TMEM);
         tc::tc_fence_before();
@@ -86,8 +91,6 @@ prompt_kernel(const __grid_constant__ AttnArgs a)
     pdl_launch_dependents();
     volatile int* abort_flag = &s_abort;
     const uint32_t tmem = s_tmem;
-    Walk w;
-    w.begin(a, deal, start);
 
     if (warp == 12) {
         if (lane == 0) {
@@ -205,33 +208,46 @@ prompt_kernel(const __grid_constant__ AttnArgs a)
         // ---- rows ----
         const int x = warp >> 2, row = (warp & 3) * 32 + lane;
         const uint32_t lane_tmem = tmem + x * P::HALF + ((uint32_t)((warp & 3) * 32) << 16), lane_o = lane_tmem + P::OUT;
+        const float base = a.scale * LOG2E;
         int n = 0, tile = -1;                             // units of this half; the tile's number
-        do {
-            ++tile;
-            const int row0 = w.t * PROMPT_ROWS, all = min(PROMPT_ROWS, w.sp.n * deal.group - row0);
-            const int r = min(x * 128 + row, all - 1), token = (row0 + r) / deal.group, head = w.head * deal.group + (row0 + r) % deal.group;
-            const bool live = x * 128 + row < all, active = x * 128 < all;
-            const size_t at = (size_t)w.seq * a.c.kv_heads + w.head;
-            if (active) {
-                const uint4* src = reinterpret_cast<const uint4*>(a.q + (size_t)(w.sp.row + token) * a.ldq + head * D);
+        // The queries of a tile to shared memory: that of the next one while the last products of this one run (its scores are all done).
+        struct Mine { int all, r, token, head; bool live; } now;
+        auto bring = [&](const Walk& w) {
+            const int row0 = w.t * PROMPT_ROWS;
+            Mine v;
+            v.all = min(PROMPT_ROWS, w.sp.n * deal.group - row0);
+            v.r = min(x * 128 + row, v.all - 1);
+            v.token = (row0 + v.r) / deal.group;
+            v.head = w.head * deal.group + (row0 + v.r) % deal.group;
+            v.live = x * 128 + row < v.all;
+            if (x * 128 < v.all) {
+                const uint4* src = reinterpret_cast<const uint4*>(a.q + (size_t)(w.sp.row + v.token) * a.ldq + v.head * D);
                 uint8_t* dst = qs + x * P::BOXES * P::QBOX + row * 128;
 #pragma unroll
                 for (int c = 0; c < D / 8; ++c)
-                    *reinterpret_cast<uint4*>(dst + (c >> 3) * P::QBOX + (((c & 7) ^ (row & 7)) << 4)) = live ? src[c] : make_uint4(0, 0, 0, 0);
+                    *reinterpret_cast<uint4*>(dst + (c >> 3) * P::QBOX + (((c & 7) ^ (row & 7)) << 4)) = v.live ? src[c] : make_uint4(0, 0, 0, 0);
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             }
             tc::tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&q_full);
-            if (!active) {                                // not ahead of the others, whose arrivals would be taken for theirs
+            return v;
+        };
+        now = bring(w);
+        for (bool more = true; more;) {
+            ++tile;
+            const int row0 = w.t * PROMPT_ROWS;
+            const size_t at = (size_t)w.seq * a.c.kv_heads + w.head;
+            if (x * 128 >= now.all) {                     // not ahead of the others, whose arrivals would be taken for this half's
                 tc::wait_uniform(&q_full, (uint32_t)tile & 1u, abort_flag);
+                more = w.next(a, deal);
+                if (more) now = bring(w);
                 continue;
             }
-            const int held = (w.sp.pos + w.sp.n) / BLOCK, p = w.sp.pos + token;
-            const int first = w.sp.pos + row0 / deal.group, last = w.sp.pos + (row0 + all - 1) / deal.group;       // positions of the tile
+            const int held = (w.sp.pos + w.sp.n) / BLOCK, p = w.sp.pos + now.token;
+            const int first = w.sp.pos + row0 / deal.group, last = w.sp.pos + (row0 + now.all - 1) / deal.group;   // positions of the tile
             const float* k_scale = a.c.k_scale + at * (a.c.capacity / BLOCK);
             const float* v_scale = a.c.v_scale + at * (a.c.capacity / BLOCK);
-            const float base = a.scale * LOG2E;
             float ks = w.u0 < held ? k_scale[w.u0] : 1.0f, vs = w.u0 < held ? v_scale[w.u0] : 1.0f;
             float m = -INFINITY, l = 0.0f;
             for (int j = 0; j < w.n; ++j, ++n) {
@@ -284,9 +300,10 @@ prompt_kernel(const __grid_constant__ AttnArgs a)
                     tc::tmem_st16(scores + c * 16, f);
                 }
                 l = fmaf((sum[0] + sum[1]) + (sum[2] + sum[3]), inv, l);
+                // Every phase is waited for, since a parity does not tell a phase from the one after the next; a tile's first scores come behind all
+                // products of the tile before.
+                if (j > 0) tc::wait_uniform(&o_done[x], (uint32_t)(n - 1) & 1u, abort_flag);
                 if (j > 0 && __any_sync(0xffffffffu, moved)) {
-                    // the scores of this unit came after P V of the unit before the last, so the last one's is the phase that is waited for
-                    tc::wait_uniform(&o_done[x], (uint32_t)(n - 1) & 1u, abort_flag);
                     tc::tc_fence_after();
                     for (int c = 0; c < D; c += 16) {
                         uint32_t o[16];
@@ -302,13 +319,16 @@ prompt_kernel(const __grid_constant__ AttnArgs a)
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&p_full[x]);
             }
-            // the last scores say that P V of the unit before the last but one is done; a parity tells only the next phase from it
-            if (n > 1) tc::wait_uniform(&o_done[x], (uint32_t)n & 1u, abort_flag);
+            const bool alone = w.begins && w.ends, live = now.live;
+            const int r = now.r;
+            float* part = a.partial + (2 * (size_t)blockIdx.x + (w.begins ? 1 : 0)) * partial_floats(PROMPT_ROWS, D);
+            __half* out = a.out + (size_t)(w.sp.row + now.token) * a.ldo + now.head * D;
+            more = w.next(a, deal);
+            if (more) now = bring(w);
+            else if (tid == 0) leave_word(a, deal, w, start);
             tc::wait_uniform(&o_done[x], (uint32_t)(n - 1) & 1u, abort_flag);
             tc::tc_fence_after();
-            const bool alone = w.begins && w.ends, ok = *abort_flag == 0;
-            float* part = a.partial + (2 * (size_t)blockIdx.x + (w.begins ? 1 : 0)) * partial_floats(PROMPT_ROWS, D);
-            __half* out = a.out + (size_t)(w.sp.row + token) * a.ldo + head * D;
+            const bool ok = *abort_flag == 0;
             const float inv_l = 1.0f / l;
             for (int c = 0; c < D; c += 16) {
                 uint32_t o[16];
@@ -329,7 +349,7 @@ prompt_kernel(const __grid_constant__ AttnArgs a)
                 }
             }
             if (live && ok && !alone) { part[PROMPT_ROWS * D + r] = m; part[PROMPT_ROWS * (D + 1) + r] = l; }
-        } while (w.next(a, deal));
+        }
     }
     tc::tc_fence_before();
     __syncthreads();

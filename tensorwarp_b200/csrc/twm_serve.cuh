@@ -139,7 +139,7 @@ size_t twm_cache8_attention_bytes(const twm_cache8* c, int num_heads, int max_ro
 {
     if (!c || num_heads < 1 || max_rows < 1 || c->kv_heads < 1 || num_heads % c->kv_heads || (c->head_dim != 64 && c->head_dim != 128)) return 0;
     const AttnPlan p = plan_attention(num_heads / c->kv_heads, max_rows);
-    return 2 * (size_t)p.ctas * twm::cache8::partial_floats(p.tile, c->head_dim) * sizeof(float);
+    return (size_t)p.ctas * (sizeof(twm::cache8::Join) + 2 * twm::cache8::partial_floats(p.tile, c->head_dim) * sizeof(float));
 }
 
 twm_status twm_cache8_attention(const twm_cache8* cache, void* out, long ldo, const void* q, long ldq, int num_heads, int rows, const int* row_start,
@@ -156,7 +156,8 @@ twm_status twm_cache8_attention(const twm_cache8* cache, void* out, long ldo, co
     if ((st = ensure_device(nullptr)) != TWM_OK) return st;
     const AttnPlan p = plan_attention(num_heads / cache->kv_heads, max_rows);
     twm::cache8::AttnArgs a = {device_cache(cache), {row_start, start, rows, max_rows}, (__half*)out, (const __half*)q, ldo, ldq, num_heads,
-                               window ? window : INT_MAX, scale, (float*)workspace, {}, {}};
+                               window ? window : INT_MAX, scale, (twm::cache8::Join*)workspace,
+                               (float*)((twm::cache8::Join*)workspace + p.ctas), {}, {}};
     if (!make_codes_map(&a.k_map, cache, cache->k) || !make_codes_map(&a.v_map, cache, cache->v)) {
         snprintf(t_last_error, sizeof(t_last_error), "cuTensorMapEncodeTiled failed for a cache held in 8 bits");
         return TWM_ELAUNCH;
@@ -168,7 +169,7 @@ twm_status twm_cache8_attention(const twm_cache8* cache, void* out, long ldo, co
     if (st != TWM_OK) return st;
     const int each = p.tile == twm::cache8::PROMPT_ROWS ? 16 : 1;        // rows of a merging CTA
     return launch_op("twm_cache8_attention(merge)", D == 64 ? twm::cache8::merge_kernel<64> : twm::cache8::merge_kernel<128>,
-                     dim3(p.ctas, (p.tile + each - 1) / each), dim3(twm::cache8::MERGE_THREADS), 0, flags, stream, a, p.tile, each);
+                     dim3(p.ctas, (p.tile + each - 1) / each), dim3(twm::cache8::MERGE_THREADS), 0, flags | TWM_FLAG_PDL, stream, a, p.tile, each);
 }
 
 twm_status twm_sample(const twm_sample_args* args, int flags, void* stream)
