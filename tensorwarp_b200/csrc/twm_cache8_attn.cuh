@@ -572,55 +572,72 @@ few_kernel(const __grid_constant__ AttnArgs a)
 // ------------------------------------------------------------------------------------------------------------- merge --
 // Joins the tiles that several CTAs have keys of: CTA x takes the tile that CTA x of the kernel before began and did not end.  Its parts are
 // the last part of that CTA and the first parts of those behind it; the same call adds them up in the same order.
+// A row is LANES threads, four elements each; SIDES groups of them share a row's parts where there are few rows, and so many parts.
 constexpr int MERGE_THREADS = 256;
-template <int D>
+template <int D, int SIDES>
 __global__ void __launch_bounds__(MERGE_THREADS)
-merge_kernel(const __grid_constant__ AttnArgs a, int tile, int rows_each)
+merge_kernel(const __grid_constant__ AttnArgs a, int tile)
 {
-    constexpr int LANES = D / 4, SIDES = MERGE_THREADS / LANES;          // threads of a row; parts taken at once
-    __shared__ float4 red[SIDES][LANES];
-    __shared__ float red_l[SIDES];
+    constexpr int LANES = D / 4, ROWS = MERGE_THREADS / (LANES * SIDES);         // rows of a CTA
+    __shared__ float4 red[SIDES][ROWS][LANES];
+    __shared__ float2 red_ml[SIDES][ROWS];
     pdl_launch_dependents();
     pdl_wait_prior_grids();
     const Join w = a.joins[blockIdx.x];
-    const int r0 = blockIdx.y * rows_each, r1 = min(w.rows, r0 + rows_each);
-    if (w.parts == 0 || r0 >= r1) return;
-    const int group = a.num_heads / a.c.kv_heads;
+    if ((int)blockIdx.y * ROWS >= w.rows || w.parts == 0) return;
+    const int lane = threadIdx.x % LANES, mine = threadIdx.x / LANES % ROWS, side = threadIdx.x / (LANES * ROWS);
+    const int r = min((int)blockIdx.y * ROWS + mine, w.rows - 1);
     const size_t each = partial_floats(tile, D);
     const float* base = a.partial + (2 * (size_t)blockIdx.x + 1) * each;         // part j > 0: the first of CTA x + j
-    auto part = [&](int j) { return j == 0 ? base : base + (2 * (size_t)j - 1) * each; };
-    const int side = threadIdx.x / LANES, lane = threadIdx.x % LANES;
-    for (int r = r0; r < r1; ++r) {
-        float top = -INFINITY;
-#pragma unroll 4
-        for (int j = 0; j < w.parts; ++j) top = fmaxf(top, part(j)[tile * D + r]);
-        const float ref = top == -INFINITY ? 0.0f : top;
-        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-        float l = 0.0f;
-#pragma unroll 4
-        for (int j = side; j < w.parts; j += SIDES) {
-            const float* p = part(j);
-            const float f = ex2(p[tile * D + r] - ref);
-            const float4 x = reinterpret_cast<const float4*>(p + r * D)[lane];
-            v.x = fmaf(x.x, f, v.x); v.y = fmaf(x.y, f, v.y); v.z = fmaf(x.z, f, v.z); v.w = fmaf(x.w, f, v.w);
-            l = fmaf(p[tile * (D + 1) + r], f, l);
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    float top = -INFINITY, l = 0.0f;
+    for (int j0 = side; j0 < w.parts; j0 += 4 * SIDES) {
+        float4 x[4];
+        float m[4], n[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int j = j0 + i * SIDES;
+            const float* p = j == 0 ? base : base + (2 * (size_t)j - 1) * each;
+            const bool there = j < w.parts;
+            x[i] = there ? reinterpret_cast<const float4*>(p + r * D)[lane] : make_float4(0.f, 0.f, 0.f, 0.f);
+            m[i] = there ? p[tile * D + r] : -INFINITY;
+            n[i] = there ? p[tile * (D + 1) + r] : 0.0f;
         }
-        red[side][lane] = v;
-        if (lane == 0) red_l[side] = l;
-        __syncthreads();
-        if (side == 0) {
-            for (int x = 1; x < SIDES; ++x) {
-                const float4 y = red[x][lane];
-                v.x += y.x; v.y += y.y; v.z += y.z; v.w += y.w;
-                l += red_l[x];
-            }
-            const float n = 1.0f / l;
-            const int row = w.row0 + r;
-            __half* dst = a.out + (size_t)(w.row + row / group) * a.ldo + (w.head * group + row % group) * D + lane * 4;
-            *reinterpret_cast<uint2*>(dst) = make_uint2(pack_f16(v.x * n, v.y * n), pack_f16(v.z * n, v.w * n));
+        const float now = fmaxf(fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])), top), ref = now == -INFINITY ? 0.0f : now;
+        const float f = ex2(top - ref);
+        v.x *= f; v.y *= f; v.z *= f; v.w *= f;
+        l *= f;
+        top = now;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float g = ex2(m[i] - ref);
+            v.x = fmaf(x[i].x, g, v.x); v.y = fmaf(x[i].y, g, v.y); v.z = fmaf(x[i].z, g, v.z); v.w = fmaf(x[i].w, g, v.w);
+            l = fmaf(n[i], g, l);
         }
-        __syncthreads();
     }
+    if (SIDES > 1) {
+        red[side][mine][lane] = v;
+        if (lane == 0) red_ml[side][mine] = make_float2(top, l);
+        __syncthreads();
+        if (side > 0) return;
+        for (int x = 0; x < SIDES; ++x) top = fmaxf(top, red_ml[x][mine].x);
+        const float ref = top == -INFINITY ? 0.0f : top;
+        v = make_float4(0.f, 0.f, 0.f, 0.f);
+        l = 0.0f;
+#pragma unroll
+        for (int x = 0; x < SIDES; ++x) {
+            const float2 ml = red_ml[x][mine];
+            const float4 y = red[x][mine][lane];
+            const float g = ex2(ml.x - ref);
+            v.x = fmaf(y.x, g, v.x); v.y = fmaf(y.y, g, v.y); v.z = fmaf(y.z, g, v.z); v.w = fmaf(y.w, g, v.w);
+            l = fmaf(ml.y, g, l);
+        }
+    }
+    if ((int)blockIdx.y * ROWS + mine >= w.rows) return;
+    const float n = 1.0f / l;
+    const int group = a.num_heads / a.c.kv_heads, row = w.row0 + r;
+    __half* dst = a.out + (size_t)(w.row + row / group) * a.ldo + (w.head * group + row % group) * D + lane * 4;
+    *reinterpret_cast<uint2*>(dst) = make_uint2(pack_f16(v.x * n, v.y * n), pack_f16(v.z * n, v.w * n));
 }
 
 }  // namespace cache8

@@ -20,7 +20,7 @@ namespace twm {
 namespace cache8 {
 
 constexpr int PROMPT_ROWS = 256, PROMPT_THREADS = 448;
-constexpr int PROMPT_EXTRA = 3;                                          // a tile's own time, in units
+constexpr int PROMPT_EXTRA = 8;                                          // a tile's own time, in units
 template <int D>
 struct Prompt {
     static constexpr int BOXES = D / 64;

@@ -97,6 +97,16 @@ twm_status launch_prompt(const twm::cache8::AttnArgs& a, const AttnPlan& p, int 
     return launch_op("twm_cache8_attention", kernel, dim3(p.ctas), dim3(twm::cache8::PROMPT_THREADS), smem, flags, stream, a);
 }
 
+// Behind the kernel before whatever the flags: it waits for all of that one.
+template <int D>
+twm_status launch_merge(const twm::cache8::AttnArgs& a, const AttnPlan& p, int flags, void* stream)
+{
+    const bool many = p.tile == twm::cache8::PROMPT_ROWS;
+    const int rows = twm::cache8::MERGE_THREADS / (D / 4) / (many ? 1 : 4);
+    return launch_op("twm_cache8_attention(merge)", many ? twm::cache8::merge_kernel<D, 1> : twm::cache8::merge_kernel<D, 4>,
+                     dim3(p.ctas, (p.tile + rows - 1) / rows), dim3(twm::cache8::MERGE_THREADS), 0, flags | TWM_FLAG_PDL, stream, a, p.tile);
+}
+
 // The CTAs of a row: slices of at most 24000 logits, of which two fit an SM, and where there are few rows more of them, down to 2048 logits.
 template <typename T>
 twm_status launch_sample(const twm_sample_args& a, int flags, void* stream)
@@ -167,9 +177,7 @@ twm_status twm_cache8_attention(const twm_cache8* cache, void* out, long ldo, co
     else
         st = p.tile == 8 ? launch_few<128, 1>(a, p, flags, stream) : p.tile == 16 ? launch_few<128, 2>(a, p, flags, stream) : launch_prompt<128>(a, p, flags, stream);
     if (st != TWM_OK) return st;
-    const int each = p.tile == twm::cache8::PROMPT_ROWS ? 16 : 1;        // rows of a merging CTA
-    return launch_op("twm_cache8_attention(merge)", D == 64 ? twm::cache8::merge_kernel<64> : twm::cache8::merge_kernel<128>,
-                     dim3(p.ctas, (p.tile + each - 1) / each), dim3(twm::cache8::MERGE_THREADS), 0, flags | TWM_FLAG_PDL, stream, a, p.tile, each);
+    return D == 64 ? launch_merge<64>(a, p, flags, stream) : launch_merge<128>(a, p, flags, stream);
 }
 
 twm_status twm_sample(const twm_sample_args* args, int flags, void* stream)
