@@ -46,13 +46,29 @@ __device__ __forceinline__ bool elect_one()
     return p != 0;
 }
 
+// two FP32 operations at once
+__device__ __forceinline__ float2 fma2(float2 x, float2 y, float2 z)
+{
+    float2 r;
+    asm("{\n\t.reg .b64 x, y, z, r;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\tfma.rn.f32x2 r, x, y, z;\n\tmov.b64 {%0, %1}, r;\n\t}"
+        : "=f"(r.x), "=f"(r.y) : "f"(x.x), "f"(x.y), "f"(y.x), "f"(y.y), "f"(z.x), "f"(z.y));
+    return r;
+}
+__device__ __forceinline__ float2 add2(float2 x, float2 y)
+{
+    float2 r;
+    asm("{\n\t.reg .b64 x, y, r;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tadd.rn.f32x2 r, x, y;\n\tmov.b64 {%0, %1}, r;\n\t}"
+        : "=f"(r.x), "=f"(r.y) : "f"(x.x), "f"(x.y), "f"(y.x), "f"(y.y));
+    return r;
+}
+
 template <int D>
 __global__ void __launch_bounds__(PROMPT_THREADS, 1)
 prompt_kernel(const __grid_constant__ AttnArgs a)
 {
     using P = Prompt<D>;
     extern __shared__ uint8_t prompt_raw[];
-    __shared__ uint64_t raw_full[P::RAWS], raw_empty[P::RAWS], unit_full[P::UNITS], unit_empty[P::UNITS], q_full, s_full[2][2], p_full[2], o_done[2];
+    __shared__ uint64_t raw_full[P::RAWS], raw_empty[P::RAWS], unit_full[P::UNITS], unit_empty[P::UNITS], q_full, s_full[2][2], p_full[2][2], o_done[2][2];
     __shared__ uint32_t s_tmem;
     __shared__ int s_abort;
     uint8_t* qs = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(prompt_raw) + 1023) & ~(uintptr_t)1023);
@@ -66,8 +82,10 @@ prompt_kernel(const __grid_constant__ AttnArgs a)
         for (int x = 0; x < 2; ++x) {
             mbar_init(&s_full[x][0], 1);
             mbar_init(&s_full[x][1], 1);
-            mbar_init(&p_full[x], 4);
-            mbar_init(&o_done[x], 1);
+            mbar_init(&p_full[x][0], 4);
+            mbar_init(&p_full[x][1], 4);
+            mbar_init(&o_done[x][0], 1);
+            mbar_init(&o_done[x][1], 1);
         }
         s_abort = 0;
         mbar_fence_init();
@@ -141,14 +159,14 @@ prompt_kernel(const __grid_constant__ AttnArgs a)
                         const uint32_t vs = smem_u32(units + slot * P::UNIT + P::BOXES * P::KBOX);
                         for (int x = 0; x < halves && ok; ++x) {
                             const int mine = n[x] + u - 1;
-                            ok = mbar_wait_bounded(&p_full[x], (uint32_t)mine & 1u, abort_flag);
+                            ok = mbar_wait_bounded(&p_full[x][mine & 1], (uint32_t)(mine >> 1) & 1u, abort_flag);
                             if (!ok) break;
                             tc::tc_fence_after();
                             const uint32_t at = tmem + x * P::HALF;
 #pragma unroll
                             for (int c = 0; c < BLOCK / 16; ++c)
                                 tc::tc_mma_ts(at + P::OUT, at + (mine & 1) * BLOCK + c * 8, value_desc(vs + c * 2048, P::KBOX), idesc_o, (u == 1 && c == 0) ? 0u : 1u);
-                            tc::tc_commit(&o_done[x]);
+                            tc::tc_commit(&o_done[x][mine & 1]);
                         }
                         tc::tc_commit(&unit_empty[slot]);
                     }
@@ -221,11 +239,23 @@ prompt_kernel(const __grid_constant__ AttnArgs a)
             v.head = w.head * deal.group + (row0 + v.r) % deal.group;
             v.live = x * 128 + row < v.all;
             if (x * 128 < v.all) {
-                const uint4* src = reinterpret_cast<const uint4*>(a.q + (size_t)(w.sp.row + v.token) * a.ldq + v.head * D);
-                uint8_t* dst = qs + x * P::BOXES * P::QBOX + row * 128;
+                // a warp's 32 rows, neighbouring lanes along a row; all loads ahead of the first store
+                constexpr int PER = D / 8, AT_ONCE = 32 / PER;
+                const long long mine = (long long)(w.sp.row + v.token) * a.ldq + v.head * D;
+                uint4 q[PER];
 #pragma unroll
-                for (int c = 0; c < D / 8; ++c)
-                    *reinterpret_cast<uint4*>(dst + (c >> 3) * P::QBOX + (((c & 7) ^ (row & 7)) << 4)) = v.live ? src[c] : make_uint4(0, 0, 0, 0);
+                for (int c = 0; c < PER; ++c) {
+                    const int from = c * AT_ONCE + lane / PER;
+                    const long long place = __shfl_sync(0xffffffffu, mine, from);
+                    q[c] = __ldg(reinterpret_cast<const uint4*>(a.q + place) + lane % PER);
+                }
+#pragma unroll
+                for (int c = 0; c < PER; ++c) {
+                    const int from = (warp & 3) * 32 + c * AT_ONCE + lane / PER, chunk = lane % PER;
+                    const bool there = x * 128 + from < v.all;
+                    *reinterpret_cast<uint4*>(qs + x * P::BOXES * P::QBOX + (chunk >> 3) * P::QBOX + from * 128 + (((chunk & 7) ^ (from & 7)) << 4)) =
+                        there ? q[c] : make_uint4(0, 0, 0, 0);
+                }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             }
             tc::tc_fence_before();
@@ -261,14 +291,21 @@ prompt_kernel(const __grid_constant__ AttnArgs a)
 #pragma unroll
                 for (int c = 0; c < 4; ++c) tc::tmem_ld<16>(scores + c * 16, s[c]);
                 tc::tmem_wait_ld();
-                if (!((u + 1) * BLOCK - 1 <= first && last - u * BLOCK < a.window)) {
+                const int lim = p - u * BLOCK;            // the last key of the unit that the row sees
+                if ((u + 1) * BLOCK - 1 > first) {
 #pragma unroll
                     for (int c = 0; c < 4; ++c)
 #pragma unroll
-                        for (int e = 0; e < 16; ++e) {
-                            const int key = u * BLOCK + c * 16 + e;
-                            if (!(key <= p && p - key < a.window)) s[c][e] = __float_as_uint(-INFINITY);
-                        }
+                        for (int e = 0; e < 16; ++e)
+                            if (c * 16 + e > lim) s[c][e] = __float_as_uint(-INFINITY);
+                }
+                if (last - u * BLOCK >= a.window) {
+                    const int low = lim - a.window;       // the last key that is too far behind
+#pragma unroll
+                    for (int c = 0; c < 4; ++c)
+#pragma unroll
+                        for (int e = 0; e < 16; ++e)
+                            if (c * 16 + e <= low) s[c][e] = __float_as_uint(-INFINITY);
                 }
                 float mx[4];
 #pragma unroll
@@ -286,24 +323,28 @@ prompt_kernel(const __grid_constant__ AttnArgs a)
                     l *= before;
                 }
                 const float shift = ev - (m == -INFINITY ? 0.0f : m);
-                float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                const float2 factor2 = make_float2(factor, factor), shift2 = make_float2(shift, shift);
+                float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
                     uint32_t f[16];
 #pragma unroll
                     for (int e = 0; e < 16; ++e) {
-                        const float y = ex2(fmaf(__uint_as_float(s[2 * c + (e >> 3)][2 * e & 15]), factor, shift));
-                        const float z = ex2(fmaf(__uint_as_float(s[2 * c + (e >> 3)][(2 * e & 15) + 1]), factor, shift));
-                        sum[e & 3] += y + z;
-                        f[e] = pack_f16(y, z);
+                        const uint32_t* pair = &s[2 * c + (e >> 3)][2 * e & 15];
+                        float2 y = fma2(make_float2(__uint_as_float(pair[0]), __uint_as_float(pair[1])), factor2, shift2);
+                        y.x = ex2(y.x);
+                        y.y = ex2(y.y);
+                        sum[e & 1] = add2(sum[e & 1], y);
+                        f[e] = pack_f16(y.x, y.y);
                     }
                     tc::tmem_st16(scores + c * 16, f);
                 }
-                l = fmaf((sum[0] + sum[1]) + (sum[2] + sum[3]), inv, l);
-                // Every phase is waited for, since a parity does not tell a phase from the one after the next; a tile's first scores come behind all
-                // products of the tile before.
-                if (j > 0) tc::wait_uniform(&o_done[x], (uint32_t)(n - 1) & 1u, abort_flag);
+                sum[0] = add2(sum[0], sum[1]);
+                l = fmaf(sum[0].x + sum[0].y, inv, l);
+                // A barrier for even and one for odd products: a parity does not tell a phase from the one after the next, and these scores came
+                // behind the products of the unit before the last.
                 if (j > 0 && __any_sync(0xffffffffu, moved)) {
+                    tc::wait_uniform(&o_done[x][(n - 1) & 1], (uint32_t)((n - 1) >> 1) & 1u, abort_flag);
                     tc::tc_fence_after();
                     for (int c = 0; c < D; c += 16) {
                         uint32_t o[16];
@@ -317,7 +358,7 @@ prompt_kernel(const __grid_constant__ AttnArgs a)
                 tc::tmem_wait_st();
                 tc::tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&p_full[x]);
+                if (lane == 0) mbar_arrive(&p_full[x][n & 1]);     // one for even and one for odd units: a warp may be a unit ahead of another
             }
             const bool alone = w.begins && w.ends, live = now.live;
             const int r = now.r;
@@ -326,7 +367,7 @@ prompt_kernel(const __grid_constant__ AttnArgs a)
             more = w.next(a, deal);
             if (more) now = bring(w);
             else if (tid == 0) leave_word(a, deal, w, start);
-            tc::wait_uniform(&o_done[x], (uint32_t)(n - 1) & 1u, abort_flag);
+            tc::wait_uniform(&o_done[x][(n - 1) & 1], (uint32_t)((n - 1) >> 1) & 1u, abort_flag);
             tc::tc_fence_after();
             const bool ok = *abort_flag == 0;
             const float inv_l = 1.0f / l;
@@ -336,13 +377,12 @@ prompt_kernel(const __grid_constant__ AttnArgs a)
                 tc::tmem_wait_ld();
                 if (!live || !ok) continue;
                 if (alone) {
+                    uint32_t h[8];
 #pragma unroll
-                    for (int e = 0; e < 16; e += 8) {
-                        float f[8];
-#pragma unroll
-                        for (int y = 0; y < 8; ++y) f[y] = __uint_as_float(o[e + y]) * inv_l;
-                        *reinterpret_cast<uint4*>(out + c + e) = pack8(f);
-                    }
+                    for (int e = 0; e < 8; ++e) h[e] = pack_f16(__uint_as_float(o[2 * e]) * inv_l, __uint_as_float(o[2 * e + 1]) * inv_l);
+                    uint4* dst = reinterpret_cast<uint4*>(out + c);
+                    dst[0] = make_uint4(h[0], h[1], h[2], h[3]);
+                    dst[1] = make_uint4(h[4], h[5], h[6], h[7]);
                 } else {
 #pragma unroll
                     for (int e = 0; e < 16; e += 4) *reinterpret_cast<uint4*>(part + r * D + c + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
