@@ -4,9 +4,9 @@
 // Nothing is sorted.  The kept tokens are the head of an order, so all cuts come down to one key and how many of the tokens equal to it are
 // kept; that border is found by histograms, narrowing in on the bin it lies in:
 //   level 0   bins of 1/16 octave of weight below the largest logit's, 1024 of them (what is beyond, 2^-64, is one more bin);
-//   level 1   1024 parts of the bin that the border lies in;
-//   then      keys (logits as ordered integers), 1024 parts of what is left, which only many equal or nearly equal logits need;
-// and once 32 tokens or fewer are left they are ordered by one warp.  A bin holds its number of tokens and its mass.  Within a bin weights are
+//   then      1024 equal parts, as ordered integers, of the logits of the bin that the border lies in, and of the part again;
+// and once 32 tokens or fewer are left they are ordered by one warp.  Which logits a bin of level 0 has is found by searching its ends, so that
+// all passes but the first only compare.  A bin holds its number of tokens and its mass.  Within a bin weights are
 // within 2^(1/16) of its largest W: mass = W (count - sum of delta), delta = 1 - w / W in fixed point, so that both are integer sums, the
 // same in any order: the result does not depend on which thread comes first.
 // Then running sums, by index, of the kept weights find the token.
@@ -56,7 +56,6 @@ struct Weights {
         hi = (float)c;
         lo = (float)(c - (double)hi);
     }
-    __device__ __forceinline__ float octaves(float v) const { return (v - top) * hi; }         // <= 0, rising with v; NaN for no number of them
     __device__ __forceinline__ float of(float v) const
     {
         if (v == top) return 1.0f;
@@ -78,7 +77,7 @@ struct Shared {
     uint32_t warp_u32[WARPS];
     double warp_f64[WARPS];
     uint32_t cta_max[MAX_CTAS];
-    uint32_t cta_lo[2][MAX_CTAS], cta_hi[2][MAX_CTAS];   // smallest and largest key of a range, two turns
+    uint32_t ends[2];                                    // the keys at which level 0's bin and the next one begin
     uint32_t cta_ties[MAX_CTAS];
     unsigned long long cta_above[MAX_CTAS];
     uint32_t list_n[2], list[2][FEW];                    // the last tokens of top-k's border, of top-p's
@@ -87,6 +86,13 @@ struct Shared {
     uint32_t cut, ties;
     double cut_mass;
 };
+
+// 2^(-i / 16)
+__device__ __constant__ double c_octave[16] = {
+    1.0, 0.95760328069857364694, 0.91700404320467123174, 0.87812608018664974155, 0.84089641525371454303, 0.80524516597462715409,
+    0.77110541270397041183, 0.73841307296974965570, 0.70710678118654752440, 0.67712777346844636413, 0.64841977732550483296, 0.62092890603674202432,
+    0.59460355750136053336, 0.56939431737834582684, 0.54525386633262882960, 0.52213689121370692017};
+__device__ __forceinline__ double octave_part(int i) { return c_octave[i & 15] * __longlong_as_double((long long)(1023 - (i >> 4)) << 52); }
 
 // counts and masses ahead of this thread's two bins, and of all
 struct Scan { uint32_t before, all; double mass_before, mass_all; };
@@ -160,7 +166,16 @@ sample_kernel(const __grid_constant__ twm_sample_args a, int slice)
         mx = fmaxf(mx, f);
         if (i < held) vals[i] = f;
     }
+    const int quads = (held + 3) / 4;
+    if (tid < 4 * quads - held) vals[held + tid] = NAN;  // compares false with everything
     auto at = [&](int i) { return i < held ? vals[i] : plain(logit_f32(logits[i])); };
+    auto each = [&](auto f) {
+        for (int i = tid; i < quads; i += THREADS) {
+            const float4 q = reinterpret_cast<const float4*>(vals)[i];
+            f(q.x); f(q.y); f(q.z); f(q.w);
+        }
+        for (int i = held + tid; i < ns; i += THREADS) f(plain(logit_f32(logits[i])));
+    };
     uint32_t key = __reduce_max_sync(0xffffffffu, order_of(mx));
     if (lane == 0) sh.warp_u32[warp] = key;
     __syncthreads();
@@ -185,20 +200,16 @@ sample_kernel(const __grid_constant__ twm_sample_args a, int slice)
         weights.set(mx, (double)t);
         const bool need_k = k > 0 && k < n, need_p = p < 1.0f;
         if (need_k || need_p) {
-            // a token's bin at level 0, or BINS, and its place in the bin
-            auto bin_of = [&](float v, float& within) {
-                const float x = v == mx ? 0.0f : -16.0f * weights.octaves(v);
-                if (!(x < (float)BINS)) { within = 0.0f; return BINS; }
-                const int b = (int)x;
-                within = x - (float)b;
-                return b;
-            };
+            // a token's bin at level 0, or BINS; falls with rising logits
+            const float scale16 = -16.0f * weights.hi;
+            auto place_of = [&](float v) { return v == mx ? 0.0f : (v - mx) * scale16; };
+            auto bin_of = [&](float v) { const float x = place_of(v); return x < (float)BINS ? (int)x : BINS; };
             // delta < 0.0424: a slice's sum of them fits 32 bits
             const float fixed = slice <= 24000 ? 4194304.0f : slice <= 48000 ? 2097152.0f : 1048576.0f;
             const double unit = 1.0 / (double)fixed;
-            auto count = [&](int bin, float share) {         // share: w / W
+            auto count = [&](int bin, float delta) {
                 atomicAdd(&sh.count[bin], 1u);
-                const uint32_t d = __float2uint_rn((1.0f - share) * fixed);
+                const uint32_t d = __float_as_uint(fmaf(delta, fixed, 8388608.0f)) - 0x4b000000u;        // the nearest integer
                 if (d) atomicAdd(&sh.delta[bin], d);
             };
             // the cluster's histogram from those of its CTAs: each CTA adds up a share of the bins, two CTAs' a thread, and tells all
@@ -234,15 +245,18 @@ sample_kernel(const __grid_constant__ twm_sample_args a, int slice)
                 }
                 __syncthreads();
             };
-            // level 0
-            for (int i = tid; i < ns; i += THREADS) {
-                float within;
-                const int b = bin_of(at(i), within);
-                if (b < BINS) count(b, exp2f(within * -0.0625f));
-            }
+            // level 0; 1 - 2^(-y/16) = 1 - e^-z by its series, z < 0.0434
+            each([&](float v) {
+                const float x = place_of(v);
+                if (x < (float)BINS) {
+                    const float whole = __fadd_rz(x, 8388608.0f);                // 2^23 + the bin
+                    const float z = (x - (whole - 8388608.0f)) * (0.69314718f / 16.0f);
+                    count((int)(__float_as_uint(whole) - 0x4b000000u), z * fmaf(z, fmaf(z, fmaf(z, -1.0f / 24.0f, 1.0f / 6.0f), -0.5f), 1.0f));
+                }
+            });
             join();
             const uint32_t c0 = sh.all_count[2 * tid], c1 = sh.all_count[2 * tid + 1];
-            const double w0 = exp2((double)(2 * tid) * -0.0625), w1 = w0 * 0.95760328069857364694;
+            const double w0 = octave_part(2 * tid), w1 = octave_part(2 * tid + 1);
             const double m0 = w0 * ((double)c0 - (double)sh.all_delta[2 * tid] * unit), m1 = w1 * ((double)c1 - (double)sh.all_delta[2 * tid + 1] * unit);
             const Scan first = scan(sh, c0 + c1, m0 + m1);
             double mass = first.mass_all;                    // of what top-k keeps
@@ -286,59 +300,32 @@ sample_kernel(const __grid_constant__ twm_sample_args a, int slice)
                 const int bin = (int)sh.found_bin;
                 uint32_t left = sh.found_count, over = sh.found_over;
                 double over_mass = sh.found_over_mass;
-                int part = -1;
-                if (left > FEW && bin < BINS) {              // level 1
-                    for (int i = tid; i < ns; i += THREADS) {
-                        float within;
-                        if (bin_of(at(i), within) == bin) count(min((int)(within * (float)BINS), BINS - 1), exp2f(within * -0.0625f));
-                    }
-                    join();
-                    const double w = exp2((double)bin * -0.0625);
-                    const uint32_t x0 = sh.all_count[2 * tid], x1 = sh.all_count[2 * tid + 1];
-                    const double y0 = w * ((double)x0 - (double)sh.all_delta[2 * tid] * unit), y1 = w * ((double)x1 - (double)sh.all_delta[2 * tid + 1] * unit);
-                    const Scan s = scan(sh, x0 + x1, y0 + y1);
-                    find(over, over_mass, x0, y0, x1, y1, s, 0);
-                    part = (int)sh.found_bin;
-                    left = sh.found_count;
-                    over = sh.found_over;
-                    over_mass = sh.found_over_mass;
+                // the logits that are left, as keys: from the end of the next bin to that of this one, each found by a warp
+                const uint32_t lowest = order_of(-INFINITY);
+                if (warp < 2) {
+                    uint32_t from = lowest, to = key;            // the largest key whose bin is `bin` (or the next one) or behind it
+                    const int b = bin + warp;
+                    if (b == 0) from = key;
+                    else if (b > BINS) from = lowest - 1;
+                    else
+                        while (from < to) {
+                            const uint32_t step = (to - from) / 32 + 1;
+                            const uint32_t mine = from + (lane + 1) * step;
+                            const unsigned int yes = __ballot_sync(0xffffffffu, mine > from && mine <= to && bin_of(value_of(mine)) >= b);
+                            const uint32_t next = from + __popc(yes) * step;
+                            to = min(to, next + (step - 1));
+                            from = next;
+                        }
+                    if (lane == 0) sh.ends[warp] = from;
                 }
-                // whether a token is among those that are left
-                uint32_t lo = 0, hi = 0xffffffffu;
-                bool by_key = false;
-                auto in = [&](float v) {
-                    if (by_key) { const uint32_t o = order_of(v); return o >= lo && o <= hi; }
-                    float within;
-                    const int b = bin_of(v, within);
-                    return b == bin && (part < 0 || min((int)(within * (float)BINS), BINS - 1) == part);
-                };
-                for (int turn = 0; left > FEW; ++turn) {
-                    uint32_t l = 0xffffffffu, h = 0;
-                    for (int i = tid; i < ns; i += THREADS) {
-                        const float v = at(i);
-                        if (in(v)) { l = min(l, order_of(v)); h = max(h, order_of(v)); }
-                    }
-                    l = __reduce_min_sync(0xffffffffu, l);
-                    h = __reduce_max_sync(0xffffffffu, h);
-                    if (lane == 0) { sh.part_count[warp] = l; sh.part_count[WARPS + warp] = h; }
-                    __syncthreads();
-                    if (tid < ctas) {
-                        for (int w = 0; w < WARPS; ++w) { l = min(l, sh.part_count[w]); h = max(h, sh.part_count[WARPS + w]); }
-                        st_cluster_u32(mapa_shared(smem_u32(&sh.cta_lo[turn & 1][rank]), tid), l);
-                        st_cluster_u32(mapa_shared(smem_u32(&sh.cta_hi[turn & 1][rank]), tid), h);
-                    }
-                    cluster_sync_all();
-                    lo = 0xffffffffu;
-                    hi = 0;
-                    for (int c = 0; c < ctas; ++c) { lo = min(lo, sh.cta_lo[turn & 1][c]); hi = max(hi, sh.cta_hi[turn & 1][c]); }
-                    by_key = true;
-                    if (lo == hi) break;
+                __syncthreads();
+                uint32_t hi = sh.ends[0], lo = sh.ends[1] + 1;
+                while (left > FEW && lo < hi) {
                     const int shift = max(0, 22 - __clz(hi - lo));               // (hi - lo) >> shift < 1024
-                    const float w_top = weights.of(value_of(hi)), back = 1.0f / w_top;           // beyond the bins mass does not count
-                    for (int i = tid; i < ns; i += THREADS) {
-                        const float v = at(i);
-                        if (in(v)) count((int)((hi - order_of(v)) >> shift), bin < BINS ? fminf(weights.of(v) * back, 1.0f) : 1.0f);
-                    }
+                    const float w_top = weights.of(value_of(hi)), back = 1.0f / w_top, f_lo = value_of(lo), f_hi = value_of(hi);
+                    each([&](float v) {                          // beyond the bins mass does not count
+                        if (v >= f_lo && v <= f_hi) count((int)((hi - order_of(v)) >> shift), bin < BINS ? fmaxf(fmaf(-weights.of(v), back, 1.0f), 0.0f) : 0.0f);
+                    });
                     join();
                     const uint32_t x0 = sh.all_count[2 * tid], x1 = sh.all_count[2 * tid + 1];
                     const double w = (double)w_top;
@@ -360,28 +347,36 @@ sample_kernel(const __grid_constant__ twm_sample_args a, int slice)
                     mass = over_mass + (double)border_ties * w;
                 } else {
                     // the last ones, put in order by a warp of every CTA
-                    for (int i = tid; i < ns; i += THREADS) {
-                        const float v = at(i);
-                        if (in(v)) {
+                    const float f_lo = value_of(lo), f_hi = value_of(hi);
+                    each([&](float v) {
+                        if (v >= f_lo && v <= f_hi) {
                             const uint32_t slot = atomicAdd(&sh.list_n[what], 1u);
                             if (slot < FEW) sh.list[what][slot] = order_of(v);
                         }
-                    }
+                    });
                     cluster_sync_all();
                     if (warp == 0) {
-                        uint32_t mine = 0;
-                        int base = 0;
-                        for (int c = 0; c < ctas; ++c) {
-                            const int m = (int)ld_cluster_u32(mapa_shared(smem_u32(&sh.list_n[what]), c));
-                            if (lane >= base && lane < base + m) mine = ld_cluster_u32(mapa_shared(smem_u32(&sh.list[what][lane - base]), c));
-                            base += m;
-                        }
-                        int place = 0;
+                        // lane x takes the x-th of the CTAs' lists, one behind another
+                        const int m = lane < ctas ? (int)ld_cluster_u32(mapa_shared(smem_u32(&sh.list_n[what]), lane)) : 0;
+                        int upto_cta = m;
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) {
+                        for (int o = 1; o < MAX_CTAS; o <<= 1) {
+                            const int x = __shfl_up_sync(0xffffffffu, upto_cta, o);
+                            if (lane >= o) upto_cta += x;
+                        }
+                        int from = 0, base = 0;
+                        for (int c = 0; c < ctas; ++c) {
+                            const int x = __shfl_sync(0xffffffffu, upto_cta, c);
+                            if (lane >= x) { from = c + 1; base = x; }
+                        }
+                        uint32_t mine = 0;
+                        if (lane < (int)left) mine = ld_cluster_u32(mapa_shared(smem_u32(&sh.list[what][lane - base]), from));
+                        int place = 0;
+                        for (int j = 0; j < (int)left; ++j) {
                             const uint32_t x = __shfl_sync(0xffffffffu, mine, j);
                             place += x > mine || (x == mine && j < lane);
                         }
+                        if (lane >= (int)left) place = lane;
                         sh.part_count[place] = mine;
                         __syncwarp();
                         mine = sh.part_count[lane];                              // falling; lanes from `left` on have none
@@ -419,18 +414,22 @@ sample_kernel(const __grid_constant__ twm_sample_args a, int slice)
         }
     }
 
-    // ---- running sums by index: neighbouring tokens a thread, an odd number of them (no bank conflicts).  Weights as integers, 2^42 the largest:
+    // ---- running sums by index: neighbouring tokens a thread.  Weights as integers, 2^42 the largest:
     // sums of up to 2^20 of them are exact, and the same whoever adds them up, so that exactly one thread has the token. ----
     constexpr float ONE = 4398046511104.0f;
-    const int per = ((ns + THREADS - 1) / THREADS) | 1, i0 = min(ns, tid * per), i1 = min(ns, i0 + per);
+    const int per = 4 * (((ns + 4 * THREADS - 1) / (4 * THREADS)) | 1), i0 = min(ns, tid * per), i1 = min(ns, i0 + per);
+    const float f_cut = cut < order_of(-INFINITY) ? -INFINITY : value_of(cut);       // all are over 0, but -inf weighs nothing
     unsigned long long above = 0;
     uint32_t same = 0;
-    for (int i = i0; i < i1; ++i) {
-        const float v = at(i);
-        const uint32_t o = order_of(v);
-        if (o > cut) above += __float2ull_rn(weights.of(v) * ONE);
-        same += o == cut;
+    auto weigh = [&](float v) {
+        if (v > f_cut) above += __float2ull_rn(weights.of(v) * ONE);
+        same += v == f_cut;
+    };
+    for (int i = i0; i < min(i1, held); i += 4) {            // an odd number of four each: no bank conflicts
+        const float4 q = *reinterpret_cast<const float4*>(vals + i);
+        weigh(q.x); weigh(q.y); weigh(q.z); weigh(q.w);
     }
+    for (int i = max(i0, held); i < i1; ++i) weigh(plain(logit_f32(logits[i])));
     unsigned long long upto = above;
     uint32_t same_upto = same;
 #pragma unroll
