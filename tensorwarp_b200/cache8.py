@@ -41,7 +41,7 @@ class Cache8:
             if tuple(t.shape) != tuple(shape) or t.dtype not in dtypes or not t.is_contiguous() or t.device != k.device:
                 raise TwmError(_lib.TWM_EINVAL, f"Cache8: expected a contiguous {dtypes[0]} tensor of {tuple(shape)} on {k.device}")
         self.k, self.v, self.k_scale, self.v_scale, self.k_tail, self.v_tail = k, v, k_scale, v_scale, k_tail, v_tail
-        self.device = k.device
+        self.device, self.index = k.device, k.get_device()
         self.desc = _lib.Cache8(self.seqs, self.kv_heads, self.head_dim, self.capacity, k.data_ptr(), v.data_ptr(), k_scale.data_ptr(),
                                 v_scale.data_ptr(), k_tail.data_ptr(), v_tail.data_ptr())
         self._ref = C.addressof(self.desc)
@@ -68,6 +68,7 @@ class Workspace:
     def __init__(self, nbytes: int, device="cuda"):
         self.nbytes = max(int(nbytes), 16)
         self.buf = torch.empty(self.nbytes, dtype=torch.uint8, device=device)
+        self.ptr = self.buf.data_ptr()
 
     @classmethod
     def for_cache(cls, cache: Cache8, num_heads: int, max_rows: int = 1) -> "Workspace":
@@ -75,21 +76,31 @@ class Workspace:
         return cls(_lib.lib().twm_cache8_attention_bytes(cache._ref, num_heads, max_rows), cache.device)
 
 
-def _rows(where: str, cache: Cache8, wide: torch.Tensor, narrow: torch.Tensor, start: torch.Tensor, row_start: Optional[torch.Tensor],
-          max_rows: int, columns: int, out_columns: int) -> None:
-    device = cache.device
+def _refuse(where: str, cache: Cache8, wide: torch.Tensor, narrow: torch.Tensor, start: torch.Tensor, row_start: Optional[torch.Tensor],
+            columns: int, out_columns: int) -> None:
+    """Says what is wrong with a call's rows, which are not as they must be."""
     for t in (wide, narrow, start) if row_start is None else (wide, narrow, start, row_start):
-        if t.device != device:
-            _require_cuda(t)
-            raise TwmError(_lib.TWM_EINVAL, f"{where}: tensors of {t.device} with a cache of {device}")
+        _require_cuda(t)
+        if t.device != cache.device:
+            raise TwmError(_lib.TWM_EINVAL, f"{where}: tensors of {t.device} with a cache of {cache.device}")
     if wide.dtype is not torch.float16 or narrow.dtype is not torch.float16 or wide.dim() != 2 or narrow.dim() != 2:
         raise TwmError(_lib.TWM_EINVAL, f"{where}: rows must be float16 matrices")
-    if wide.shape[1] != columns or narrow.shape[1] != out_columns or narrow.shape[0] < wide.shape[0] or wide.stride(1) != 1 or narrow.stride(1) != 1:
-        raise TwmError(_lib.TWM_EINVAL, f"{where}: expected rows of {columns} and {out_columns} numbers, as many of both")
     if start.dtype is not torch.int32 or start.numel() != cache.seqs or not start.is_contiguous():
         raise TwmError(_lib.TWM_EINVAL, f"{where}: start must be int32 [{cache.seqs}]")
     if row_start is not None and (row_start.dtype is not torch.int32 or row_start.numel() != cache.seqs + 1 or not row_start.is_contiguous()):
         raise TwmError(_lib.TWM_EINVAL, f"{where}: row_start must be int32 [{cache.seqs + 1}]")
+    raise TwmError(_lib.TWM_EINVAL, f"{where}: expected rows of {columns} and {out_columns} numbers, as many of both")
+
+
+def _fits(cache: Cache8, wide: torch.Tensor, narrow: torch.Tensor, start: torch.Tensor, row_start: Optional[torch.Tensor], columns: int,
+          out_columns: int) -> bool:
+    # once per layer and token: integers and identities, no objects made for a comparison
+    index, i32, f16 = cache.index, torch.int32, torch.float16
+    if (wide.get_device() != index or narrow.get_device() != index or start.get_device() != index or wide.dtype is not f16 or narrow.dtype is not f16
+            or wide.dim() != 2 or narrow.dim() != 2 or start.dtype is not i32 or start.numel() != cache.seqs or not start.is_contiguous()
+            or wide.size(1) != columns or narrow.size(1) != out_columns or narrow.size(0) < wide.size(0) or wide.stride(1) != 1 or narrow.stride(1) != 1):
+        return False
+    return row_start is None or (row_start.get_device() == index and row_start.dtype is i32 and row_start.numel() == cache.seqs + 1 and row_start.is_contiguous())
 
 
 def append(cache: Cache8, qkv: torch.Tensor, q_out: torch.Tensor, start: torch.Tensor, *, num_heads: int, row_start: Optional[torch.Tensor] = None,
@@ -100,16 +111,22 @@ def append(cache: Cache8, qkv: torch.Tensor, q_out: torch.Tensor, start: torch.T
     [seqs + 1]: its rows among the call's, at most `max_rows` (None: one row a sequence).  rope: ``rope_table`` of the cache's capacity;
     bias f32 of a whole row."""
     d = cache.head_dim
-    _rows("append", cache, qkv, q_out, start, row_start, max_rows, (num_heads + 2 * cache.kv_heads) * d, num_heads * d)
-    if bias is not None and (bias.dtype is not torch.float32 or bias.numel() != qkv.shape[1] or not bias.is_contiguous() or bias.device != cache.device):
+    columns = (num_heads + 2 * cache.kv_heads) * d
+    if not _fits(cache, qkv, q_out, start, row_start, columns, num_heads * d):
+        _refuse("append", cache, qkv, q_out, start, row_start, columns, num_heads * d)
+    if bias is not None and (bias.dtype is not torch.float32 or bias.numel() != columns or not bias.is_contiguous() or bias.get_device() != cache.index):
         raise TwmError(_lib.TWM_EINVAL, "append: bias must be float32 of a whole row")
-    if rope is not None and (rope.dtype is not torch.float32 or rope.numel() < cache.capacity * d or not rope.is_contiguous() or rope.device != cache.device):
+    if rope is not None and (rope.dtype is not torch.float32 or rope.numel() < cache.capacity * d or not rope.is_contiguous() or rope.get_device() != cache.index):
         raise TwmError(_lib.TWM_EINVAL, "append: rope must be float32 [capacity, head_dim]")
-    with _on(cache.device):
-        check(_lib.lib().twm_cache8_append(cache._ref, q_out.data_ptr(), q_out.stride(0), qkv.data_ptr(), qkv.stride(0),
-                                           bias.data_ptr() if bias is not None else None, rope.data_ptr() if rope is not None else None, num_heads,
-                                           qkv.shape[0], row_start.data_ptr() if row_start is not None else None, max_rows, start.data_ptr(), flags,
-                                           _stream_ptr(stream)), "twm_cache8_append")
+    if torch._C._cuda_getDevice() != cache.index:
+        with torch.cuda.device(cache.index):
+            return append(cache, qkv, q_out, start, num_heads=num_heads, row_start=row_start, max_rows=max_rows, bias=bias, rope=rope, stream=stream, flags=flags)
+    status = _lib.lib().twm_cache8_append(cache._ref, q_out.data_ptr(), q_out.stride(0), qkv.data_ptr(), qkv.stride(0),
+                                          bias.data_ptr() if bias is not None else None, rope.data_ptr() if rope is not None else None, num_heads,
+                                          qkv.size(0), row_start.data_ptr() if row_start is not None else None, max_rows, start.data_ptr(), flags,
+                                          _stream_ptr(stream))
+    if status:
+        check(status, "twm_cache8_append")
 
 
 def attention(cache: Cache8, q: torch.Tensor, out: torch.Tensor, start: torch.Tensor, *, num_heads: int, row_start: Optional[torch.Tensor] = None,
@@ -119,31 +136,20 @@ def attention(cache: Cache8, q: torch.Tensor, out: torch.Tensor, start: torch.Te
     (``append`` with the same start and row_start); out like q.  scale: 1/sqrt(head_dim) if None; window: how many of the newest keys
     a row sees (0: all).  workspace: ``Workspace.for_cache``; without one the call makes its own."""
     d = cache.head_dim
-    _rows("attention", cache, q, out, start, row_start, max_rows, num_heads * d, num_heads * d)
-    with _on(cache.device):
-        if workspace is None:
-            with torch.cuda.stream(stream):
-                workspace = Workspace.for_cache(cache, num_heads, max_rows)
-        elif workspace.buf.device != cache.device:
-            raise TwmError(_lib.TWM_EINVAL, "attention: the workspace is on another device")
-        check(_lib.lib().twm_cache8_attention(cache._ref, out.data_ptr(), out.stride(0), q.data_ptr(), q.stride(0), num_heads, q.shape[0],
-                                              row_start.data_ptr() if row_start is not None else None, max_rows, start.data_ptr(),
-                                              1.0 / math.sqrt(d) if scale is None else scale, window, workspace.buf.data_ptr(), workspace.nbytes,
-                                              flags, _stream_ptr(stream)), "twm_cache8_attention")
-
-
-class _on:
-    """Makes `device` the current one for a launch, where it is not."""
-
-    def __init__(self, device: torch.device):
-        self.index, self.before = device.index, -1
-
-    def __enter__(self):
-        current = torch._C._cuda_getDevice()
-        if self.index != current:
-            torch.cuda.set_device(self.index)
-            self.before = current
-
-    def __exit__(self, *exc):
-        if self.before >= 0:
-            torch.cuda.set_device(self.before)
+    if not _fits(cache, q, out, start, row_start, num_heads * d, num_heads * d):
+        _refuse("attention", cache, q, out, start, row_start, num_heads * d, num_heads * d)
+    if torch._C._cuda_getDevice() != cache.index:
+        with torch.cuda.device(cache.index):
+            return attention(cache, q, out, start, num_heads=num_heads, row_start=row_start, max_rows=max_rows, scale=scale, window=window,
+                             workspace=workspace, stream=stream, flags=flags)
+    if workspace is None:
+        with torch.cuda.stream(stream):
+            workspace = Workspace.for_cache(cache, num_heads, max_rows)
+    elif workspace.buf.get_device() != cache.index:
+        raise TwmError(_lib.TWM_EINVAL, "attention: the workspace is on another device")
+    status = _lib.lib().twm_cache8_attention(cache._ref, out.data_ptr(), out.stride(0), q.data_ptr(), q.stride(0), num_heads, q.size(0),
+                                             row_start.data_ptr() if row_start is not None else None, max_rows, start.data_ptr(),
+                                             1.0 / math.sqrt(d) if scale is None else scale, window, workspace.ptr, workspace.nbytes,
+                                             flags, _stream_ptr(stream))
+    if status:
+        check(status, "twm_cache8_attention")

@@ -3,11 +3,11 @@
 // A row belongs to a cluster of CTAs, each with a slice of it in shared memory: logits are read from memory once, whatever cuts are asked for.
 // Nothing is sorted.  The kept tokens are the head of an order, so all cuts come down to one key and how many of the tokens equal to it are
 // kept; that border is found by histograms, narrowing in on the bin it lies in:
-//   level 0   bins of 1/16 octave of weight below the largest logit's, 1024 of them (what is beyond, 2^-64, is one more bin);
-//   then      1024 equal parts, as ordered integers, of the logits of the bin that the border lies in, and of the part again;
+//   level 0   bins of 1/8 octave of weight below the largest logit's, 512 of them (what is beyond, 2^-64, is one more bin);
+//   then      512 equal parts, as ordered integers, of the logits of the bin that the border lies in, and of the part again;
 // and once 32 tokens or fewer are left they are ordered by one warp.  Which logits a bin of level 0 has is found by searching its ends, so that
 // all passes but the first only compare.  A bin holds its number of tokens and its mass.  Within a bin weights are
-// within 2^(1/16) of its largest W: mass = W (count - sum of delta), delta = 1 - w / W in fixed point, so that both are integer sums, the
+// within 2^(1/8) of its largest W: mass = W (count - sum of delta), delta = 1 - w / W in fixed point, so that both are integer sums, the
 // same in any order: the result does not depend on which thread comes first.
 // Then running sums, by index, of the kept weights find the token.
 // Bound by memory for many rows, by the chain of cluster barriers for one.
@@ -34,7 +34,7 @@ __device__ __forceinline__ uint32_t order_of(float v)
 }
 __device__ __forceinline__ float value_of(uint32_t o) { return __uint_as_float(o & 0x80000000u ? o & 0x7fffffffu : ~o); }
 
-constexpr int THREADS = 512, WARPS = THREADS / 32, BINS = 1024, MAX_CTAS = 16, FEW = 32;
+constexpr int THREADS = 512, WARPS = THREADS / 32, BINS = THREADS, MAX_CTAS = 16, FEW = 32;
 constexpr int MAX_SLICE = 40960;         // logits of a CTA in shared memory; what is beyond is read again
 
 __device__ __forceinline__ void st_cluster_u32(uint32_t at, uint32_t v) { asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(at), "r"(v) : "memory"); }
@@ -56,16 +56,14 @@ struct Weights {
         hi = (float)c;
         lo = (float)(c - (double)hi);
     }
-    __device__ __forceinline__ float of(float v) const
+    __device__ __forceinline__ float of_finite(float v) const           // with a finite largest logit
     {
-        if (v == top) return 1.0f;
-        const float d = v - top, x = d * hi;
-        if (!(x > -140.0f)) return 0.0f;
-        const float rest = fmaf(d, lo, fmaf(d, hi, -x));
+        const float d = v - top, x = d * hi, rest = fmaf(d, lo, fmaf(d, hi, -x));
         float y;
         asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-        return fmaf(y, rest * 0.69314718f, y);
+        return x > -140.0f ? fmaf(y, rest * 0.69314718f, y) : 0.0f;
     }
+    __device__ __forceinline__ float of(float v) const { return v == top ? 1.0f : of_finite(v); }
 };
 
 struct Shared {
@@ -82,19 +80,17 @@ struct Shared {
     unsigned long long cta_above[MAX_CTAS];
     uint32_t list_n[2], list[2][FEW];                    // the last tokens of top-k's border, of top-p's
     uint32_t found_bin, found_count, found_over;
-    double found_mass, found_over_mass;
+    double found_over_mass;
     uint32_t cut, ties;
     double cut_mass;
 };
 
-// 2^(-i / 16)
-__device__ __constant__ double c_octave[16] = {
-    1.0, 0.95760328069857364694, 0.91700404320467123174, 0.87812608018664974155, 0.84089641525371454303, 0.80524516597462715409,
-    0.77110541270397041183, 0.73841307296974965570, 0.70710678118654752440, 0.67712777346844636413, 0.64841977732550483296, 0.62092890603674202432,
-    0.59460355750136053336, 0.56939431737834582684, 0.54525386633262882960, 0.52213689121370692017};
-__device__ __forceinline__ double octave_part(int i) { return c_octave[i & 15] * __longlong_as_double((long long)(1023 - (i >> 4)) << 52); }
+// 2^(-i / 8)
+__device__ __constant__ double c_octave[8] = {1.0, 0.91700404320467123174, 0.84089641525371454303, 0.77110541270397041183, 0.70710678118654752440,
+                                              0.64841977732550483296, 0.59460355750136053336, 0.54525386633262882960};
+__device__ __forceinline__ double octave_part(int i) { return c_octave[i & 7] * __longlong_as_double((long long)(1023 - (i >> 3)) << 52); }
 
-// counts and masses ahead of this thread's two bins, and of all
+// counts and masses ahead of this thread's bin, and of all
 struct Scan { uint32_t before, all; double mass_before, mass_all; };
 __device__ __forceinline__ Scan scan(Shared& sh, uint32_t c, double m)
 {
@@ -110,19 +106,22 @@ __device__ __forceinline__ Scan scan(Shared& sh, uint32_t c, double m)
     __syncthreads();
     if (lane == 31) { sh.warp_u32[warp] = uc; sh.warp_f64[warp] = um; }
     __syncthreads();
-    Scan s = {0, 0, 0.0, 0.0};
-    uint32_t bc = 0;
-    double bm = 0.0;
+    // every warp adds up the warps' sums, a lane each
+    uint32_t tc = lane < WARPS ? sh.warp_u32[lane] : 0u;
+    double tm = lane < WARPS ? sh.warp_f64[lane] : 0.0;
 #pragma unroll
-    for (int w = 0; w < WARPS; ++w) {
-        if (w == warp) { bc = s.all; bm = s.mass_all; }
-        s.all += sh.warp_u32[w];
-        s.mass_all += sh.warp_f64[w];
+    for (int o = 1; o < WARPS; o <<= 1) {
+        const uint32_t xc = __shfl_up_sync(0xffffffffu, tc, o);
+        const double xm = __shfl_up_sync(0xffffffffu, tm, o);
+        if (lane >= o) { tc += xc; tm += xm; }
     }
-    const uint32_t xc = __shfl_up_sync(0xffffffffu, uc, 1);
-    const double xm = __shfl_up_sync(0xffffffffu, um, 1);
-    s.before = bc + (lane ? xc : 0u);
-    s.mass_before = bm + (lane ? xm : 0.0);
+    Scan s;
+    s.all = __shfl_sync(0xffffffffu, tc, WARPS - 1);
+    s.mass_all = __shfl_sync(0xffffffffu, tm, WARPS - 1);
+    const uint32_t bc = __shfl_sync(0xffffffffu, tc, (warp + 31) & 31), xc = __shfl_up_sync(0xffffffffu, uc, 1);
+    const double bm = __shfl_sync(0xffffffffu, tm, (warp + 31) & 31), xm = __shfl_up_sync(0xffffffffu, um, 1);
+    s.before = (warp ? bc : 0u) + (lane ? xc : 0u);
+    s.mass_before = (warp ? bm : 0.0) + (lane ? xm : 0.0);
     return s;
 }
 
@@ -201,102 +200,82 @@ sample_kernel(const __grid_constant__ twm_sample_args a, int slice)
         const bool need_k = k > 0 && k < n, need_p = p < 1.0f;
         if (need_k || need_p) {
             // a token's bin at level 0, or BINS; falls with rising logits
-            const float scale16 = -16.0f * weights.hi;
-            auto place_of = [&](float v) { return v == mx ? 0.0f : (v - mx) * scale16; };
+            const float scale8 = -8.0f * weights.hi;
+            auto place_of = [&](float v) { return v == mx ? 0.0f : (v - mx) * scale8; };
             auto bin_of = [&](float v) { const float x = place_of(v); return x < (float)BINS ? (int)x : BINS; };
-            // delta < 0.0424: a slice's sum of them fits 32 bits
-            const float fixed = slice <= 24000 ? 4194304.0f : slice <= 48000 ? 2097152.0f : 1048576.0f;
+            // delta < 0.0831: a slice's sum of them fits 32 bits
+            const float fixed = slice <= 24000 ? 2097152.0f : slice <= 48000 ? 1048576.0f : 524288.0f;
             const double unit = 1.0 / (double)fixed;
             auto count = [&](int bin, float delta) {
                 atomicAdd(&sh.count[bin], 1u);
                 const uint32_t d = __float_as_uint(fmaf(delta, fixed, 8388608.0f)) - 0x4b000000u;        // the nearest integer
                 if (d) atomicAdd(&sh.delta[bin], d);
             };
-            // the cluster's histogram from those of its CTAs: each CTA adds up a share of the bins, two CTAs' a thread, and tells all
+            // The cluster's histogram from those of its CTAs: each CTA adds up a share of the bins, every thread of one CTA's, and tells all.
             auto join = [&]() {
                 cluster_sync_all();
-                const int bins = BINS / ctas, b = tid % bins, g = tid / bins, groups = THREADS / bins;       // ctas = 1: two bins a thread
                 if (ctas == 1) {
-                    for (int i = tid; i < BINS; i += THREADS) { sh.all_count[i] = sh.count[i]; sh.all_delta[i] = sh.delta[i]; sh.count[i] = sh.delta[i] = 0; }
-                } else {
-                    const int mine = rank * bins + b;
-                    uint32_t c = 0;
-                    unsigned long long d = 0;
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        const uint32_t from = g * 2 + j;
-                        c += ld_cluster_u32(mapa_shared(smem_u32(&sh.count[mine]), from));
-                        d += ld_cluster_u32(mapa_shared(smem_u32(&sh.delta[mine]), from));
-                    }
-                    sh.part_count[tid] = c;
-                    sh.part_delta[tid] = d;
-                    __syncthreads();
-                    // every group tells two CTAs
-                    c = 0;
-                    d = 0;
-                    for (int x = 0; x < groups; ++x) { c += sh.part_count[x * bins + b]; d += sh.part_delta[x * bins + b]; }
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        st_cluster_u32(mapa_shared(smem_u32(&sh.all_count[mine]), g * 2 + j), c);
-                        st_cluster_u64(mapa_shared(smem_u32(&sh.all_delta[mine]), g * 2 + j), d);
-                    }
-                    cluster_sync_all();
-                    for (int i = tid; i < BINS; i += THREADS) sh.count[i] = sh.delta[i] = 0;
+                    sh.all_count[tid] = sh.count[tid];
+                    sh.all_delta[tid] = sh.delta[tid];
+                    sh.count[tid] = sh.delta[tid] = 0;       // the next ones to write there come behind a barrier
+                    return;
                 }
+                const int bins = BINS / ctas, b = tid % bins, g = tid / bins, mine = rank * bins + b;
+                sh.part_count[tid] = ld_cluster_u32(mapa_shared(smem_u32(&sh.count[mine]), g));
+                sh.part_delta[tid] = ld_cluster_u32(mapa_shared(smem_u32(&sh.delta[mine]), g));
                 __syncthreads();
+                uint32_t c = 0;
+                unsigned long long d = 0;
+                for (int x = b; x < BINS; x += bins) { c += sh.part_count[x]; d += sh.part_delta[x]; }
+                st_cluster_u32(mapa_shared(smem_u32(&sh.all_count[mine]), g), c);
+                st_cluster_u64(mapa_shared(smem_u32(&sh.all_delta[mine]), g), d);
+                cluster_sync_all();
+                sh.count[tid] = sh.delta[tid] = 0;
             };
-            // level 0; 1 - 2^(-y/16) = 1 - e^-z by its series, z < 0.0434
-            each([&](float v) {
-                const float x = place_of(v);
+            // level 0; 1 - 2^(-y/8) = 1 - e^-z by its series, z < 0.0867
+            auto put = [&](float x) {
                 if (x < (float)BINS) {
                     const float whole = __fadd_rz(x, 8388608.0f);                // 2^23 + the bin
-                    const float z = (x - (whole - 8388608.0f)) * (0.69314718f / 16.0f);
+                    const float z = (x - (whole - 8388608.0f)) * (0.69314718f / 8.0f);
                     count((int)(__float_as_uint(whole) - 0x4b000000u), z * fmaf(z, fmaf(z, fmaf(z, -1.0f / 24.0f, 1.0f / 6.0f), -0.5f), 1.0f));
                 }
-            });
+            };
+            if (mx < INFINITY) each([&](float v) { put((v - mx) * scale8); });
+            else each([&](float v) { put(place_of(v)); });
             join();
-            const uint32_t c0 = sh.all_count[2 * tid], c1 = sh.all_count[2 * tid + 1];
-            const double w0 = octave_part(2 * tid), w1 = octave_part(2 * tid + 1);
-            const double m0 = w0 * ((double)c0 - (double)sh.all_delta[2 * tid] * unit), m1 = w1 * ((double)c1 - (double)sh.all_delta[2 * tid + 1] * unit);
-            const Scan first = scan(sh, c0 + c1, m0 + m1);
+            const uint32_t c0 = sh.all_count[tid];
+            const double m0 = octave_part(tid) * ((double)c0 - (double)sh.all_delta[tid] * unit);
+            const Scan first = scan(sh, c0, m0);
             double mass = first.mass_all;                    // of what top-k keeps
 
             for (int what = need_k ? 0 : 1; what <= (need_p ? 1 : 0); ++what) {
                 const double want = fmax((double)p * mass, 1e-30);       // of mass, for top-p
-                // The bin with the border, from this thread's two: the first whose end reaches what is wanted; the last one with tokens if rounding keeps
+                // The bin with the border, from this thread's: the first whose end reaches what is wanted; the last one with tokens if rounding keeps
                 // all from it.  Its number, tokens and mass, and those ahead of it.
-                auto find = [&](uint32_t over, double over_mass, uint32_t x0, double y0, uint32_t x1, double y1, const Scan& s, uint32_t beyond) {
+                auto find = [&](uint32_t over, double over_mass, uint32_t x, double y, const Scan& s, uint32_t beyond) {
                     if (tid == 0) sh.found_bin = BINS;
                     __syncthreads();
-                    const uint32_t e0 = over + s.before + x0, e1 = e0 + x1;
-                    const double f0 = over_mass + s.mass_before + y0, f1 = f0 + y1;
-                    const bool r0 = what == 0 ? e0 >= (uint32_t)k : x0 > 0 && f0 >= want, r1 = what == 0 ? e1 >= (uint32_t)k : x1 > 0 && f1 >= want;
-                    if (r0) atomicMin(&sh.found_bin, 2u * tid);
-                    else if (r1) atomicMin(&sh.found_bin, 2u * tid + 1);
+                    if (x > 0 && (what == 0 ? over + s.before + x >= (uint32_t)k : over_mass + s.mass_before + y >= want)) atomicMin(&sh.found_bin, (uint32_t)tid);
                     __syncthreads();
                     if (what == 1 && sh.found_bin == BINS) {
-                        const bool last = x0 + x1 > 0 && s.before + x0 + x1 == s.all;        // one thread's alone
                         __syncthreads();
-                        if (last) sh.found_bin = x1 > 0 ? 2u * tid + 1 : 2u * tid;
+                        if (x > 0 && s.before + x == s.all) sh.found_bin = tid;              // one thread's alone
                         __syncthreads();
                     }
                     const uint32_t b = sh.found_bin;
-                    if (b / 2 == tid) {
-                        const bool odd = b & 1;
-                        sh.found_count = odd ? x1 : x0;
-                        sh.found_mass = odd ? y1 : y0;
-                        sh.found_over = over + s.before + (odd ? x0 : 0u);
-                        sh.found_over_mass = over_mass + s.mass_before + (odd ? y0 : 0.0);
+                    if (b == tid) {
+                        sh.found_count = x;
+                        sh.found_over = over + s.before;
+                        sh.found_over_mass = over_mass + s.mass_before;
                     }
                     if (b == BINS && tid == 0) {             // top-k's border lies beyond the bins
                         sh.found_count = beyond;
-                        sh.found_mass = 0.0;
                         sh.found_over = over + s.all;
                         sh.found_over_mass = over_mass + s.mass_all;
                     }
                     __syncthreads();
                 };
-                find(0, 0.0, c0, m0, c1, m1, first, (uint32_t)n - first.all);
+                find(0, 0.0, c0, m0, first, (uint32_t)n - first.all);
                 const int bin = (int)sh.found_bin;
                 uint32_t left = sh.found_count, over = sh.found_over;
                 double over_mass = sh.found_over_mass;
@@ -307,7 +286,13 @@ sample_kernel(const __grid_constant__ twm_sample_args a, int slice)
                     const int b = bin + warp;
                     if (b == 0) from = key;
                     else if (b > BINS) from = lowest - 1;
-                    else
+                    else {
+                        // next to where the arithmetic without rounding has it, if it is there
+                        const uint32_t near = order_of(fminf(fmaxf(mx + (float)b / scale8, -3.4e38f), mx)), below = near - min(near - lowest, 256u);
+                        if (near > lowest + 512 && bin_of(value_of(below)) >= b && (near + 256 > key || bin_of(value_of(near + 256)) < b)) {
+                            from = below;
+                            to = min(key, near + 255);
+                        }
                         while (from < to) {
                             const uint32_t step = (to - from) / 32 + 1;
                             const uint32_t mine = from + (lane + 1) * step;
@@ -316,22 +301,21 @@ sample_kernel(const __grid_constant__ twm_sample_args a, int slice)
                             to = min(to, next + (step - 1));
                             from = next;
                         }
+                    }
                     if (lane == 0) sh.ends[warp] = from;
                 }
                 __syncthreads();
                 uint32_t hi = sh.ends[0], lo = sh.ends[1] + 1;
                 while (left > FEW && lo < hi) {
-                    const int shift = max(0, 22 - __clz(hi - lo));               // (hi - lo) >> shift < 1024
+                    const int shift = max(0, 23 - __clz(hi - lo));               // (hi - lo) >> shift < 512
                     const float w_top = weights.of(value_of(hi)), back = 1.0f / w_top, f_lo = value_of(lo), f_hi = value_of(hi);
                     each([&](float v) {                          // beyond the bins mass does not count
                         if (v >= f_lo && v <= f_hi) count((int)((hi - order_of(v)) >> shift), bin < BINS ? fmaxf(fmaf(-weights.of(v), back, 1.0f), 0.0f) : 0.0f);
                     });
                     join();
-                    const uint32_t x0 = sh.all_count[2 * tid], x1 = sh.all_count[2 * tid + 1];
-                    const double w = (double)w_top;
-                    const double y0 = w * ((double)x0 - (double)sh.all_delta[2 * tid] * unit), y1 = w * ((double)x1 - (double)sh.all_delta[2 * tid + 1] * unit);
-                    const Scan s = scan(sh, x0 + x1, y0 + y1);
-                    find(over, over_mass, x0, y0, x1, y1, s, 0);
+                    const uint32_t x = sh.all_count[tid];
+                    const double y = (double)w_top * ((double)x - (double)sh.all_delta[tid] * unit);
+                    find(over, over_mass, x, y, scan(sh, x, y), 0);
                     const uint32_t b = sh.found_bin;
                     left = sh.found_count;
                     over = sh.found_over;
@@ -415,21 +399,22 @@ sample_kernel(const __grid_constant__ twm_sample_args a, int slice)
     }
 
     // ---- running sums by index: neighbouring tokens a thread.  Weights as integers, 2^42 the largest:
-    // sums of up to 2^20 of them are exact, and the same whoever adds them up, so that exactly one thread has the token. ----
+    // the threads' sums add up exactly, in any order, so that exactly one thread has the token. ----
     constexpr float ONE = 4398046511104.0f;
     const int per = 4 * (((ns + 4 * THREADS - 1) / (4 * THREADS)) | 1), i0 = min(ns, tid * per), i1 = min(ns, i0 + per);
     const float f_cut = cut < order_of(-INFINITY) ? -INFINITY : value_of(cut);       // all are over 0, but -inf weighs nothing
-    unsigned long long above = 0;
+    float sum = 0.0f;                                    // of a thread's, in FP32, always in the same order
     uint32_t same = 0;
-    auto weigh = [&](float v) {
-        if (v > f_cut) above += __float2ull_rn(weights.of(v) * ONE);
-        same += v == f_cut;
+    auto walk = [&](auto weigh) {
+        for (int i = i0; i < min(i1, held); i += 4) {        // an odd number of four each: no bank conflicts
+            const float4 q = *reinterpret_cast<const float4*>(vals + i);
+            weigh(q.x); weigh(q.y); weigh(q.z); weigh(q.w);
+        }
+        for (int i = max(i0, held); i < i1; ++i) weigh(plain(logit_f32(logits[i])));
     };
-    for (int i = i0; i < min(i1, held); i += 4) {            // an odd number of four each: no bank conflicts
-        const float4 q = *reinterpret_cast<const float4*>(vals + i);
-        weigh(q.x); weigh(q.y); weigh(q.z); weigh(q.w);
-    }
-    for (int i = max(i0, held); i < i1; ++i) weigh(plain(logit_f32(logits[i])));
+    if (mx < INFINITY) walk([&](float v) { if (v > f_cut) sum += weights.of_finite(v); same += v == f_cut; });
+    else walk([&](float v) { if (v > f_cut) sum += weights.of(v); same += v == f_cut; });
+    const unsigned long long above = __float2ull_rn(sum * ONE);
     unsigned long long upto = above;
     uint32_t same_upto = same;
 #pragma unroll
@@ -469,18 +454,14 @@ sample_kernel(const __grid_constant__ twm_sample_args a, int slice)
     const unsigned long long target = min((unsigned long long)(fmin(fmax((double)random, 0.0), 1.0) * (double)total), total - 1);
     const unsigned long long begin = upto + one_tie * min(same_upto, ties), end = upto + above + one_tie * min(same_upto + same, ties);
     if (begin <= target && target < end) {
-        unsigned long long run = begin;
         float w = 0.0f;
         int i = i0;
-        for (;; ++i) {
+        sum = 0.0f;
+        for (;; ++i) {                                       // the same sums again, up to the token whose weight passes the target
             const float v = at(i);
-            const uint32_t o = order_of(v);
-            if (o > cut || (o == cut && same_upto < ties)) {
-                w = o == cut ? w_cut : weights.of(v);
-                run += __float2ull_rn(w * ONE);
-                if (run > target) break;
-            }
-            same_upto += o == cut;
+            if (v > f_cut) sum += w = weights.of(v);
+            else if (v == f_cut && same_upto < ties) { ++same_upto; w = w_cut; }
+            if (upto + __float2ull_rn(sum * ONE) + one_tie * min(same_upto, ties) > target) break;
         }
         a.tokens[row] = n0 + i;
         if (a.prob) a.prob[row] = (float)((double)w * (double)ONE / (double)total);

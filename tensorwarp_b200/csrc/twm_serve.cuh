@@ -16,11 +16,11 @@ bool off16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) != 0; }
 twm_status check_cache8(const twm_cache8* c, int num_heads, int rows, const int* row_start, int max_rows, const int* start)
 {
     if (!c || !c->k || !c->v || !c->k_scale || !c->v_scale || !c->k_tail || !c->v_tail || !start) return TWM_EINVAL;
-    if (c->seqs < 1 || c->seqs > 65535 || c->kv_heads < 1 || c->kv_heads > 65535 || (c->head_dim != 64 && c->head_dim != 128)) return TWM_EINVAL;
+    if (c->seqs < 1 || c->seqs > 65535 || c->kv_heads < 1 || c->kv_heads > 4096 || (c->head_dim != 64 && c->head_dim != 128)) return TWM_EINVAL;
     if (c->capacity < TWM_CACHE8_BLOCK || c->capacity % TWM_CACHE8_BLOCK) return TWM_EINVAL;
     // tensor maps and row numbers count cached rows in 32 bits
     if ((long long)c->seqs * c->kv_heads * c->capacity > INT_MAX) return TWM_EINVAL;
-    if (num_heads < 1 || num_heads % c->kv_heads || rows < 1 || max_rows < 1 || max_rows > rows) return TWM_EINVAL;
+    if (num_heads < 1 || num_heads > 4096 || num_heads % c->kv_heads || rows < 1 || max_rows < 1 || max_rows > rows) return TWM_EINVAL;
     if (!row_start && (rows != c->seqs || max_rows != 1)) return TWM_EINVAL;
     if ((long long)num_heads * c->head_dim > (1 << 20) || (long long)max_rows * num_heads > INT_MAX / 2) return TWM_EINVAL;
     if (off16(c->k) || off16(c->v) || off16(c->k_tail) || off16(c->v_tail)) return TWM_EALIGN;
@@ -107,13 +107,14 @@ twm_status launch_merge(const twm::cache8::AttnArgs& a, const AttnPlan& p, int f
                      dim3(p.ctas, (p.tile + rows - 1) / rows), dim3(twm::cache8::MERGE_THREADS), 0, flags | TWM_FLAG_PDL, stream, a, p.tile);
 }
 
-// The CTAs of a row: slices of at most 24000 logits, of which two fit an SM, and where there are few rows more of them, down to 2048 logits.
+// The CTAs of a row: slices of at most 24000 logits, of which two fit an SM, and where there are few rows as many more of them as the SMs take at
+// once, down to 2048 logits each (64 rows of 32768, two or four CTAs: 28.1 and MEASURED us).
 template <typename T>
 twm_status launch_sample(const twm_sample_args& a, int flags, void* stream)
 {
-    const int most = a.rows <= 8 ? 16 : a.rows <= 36 ? 8 : 1;
+    const int most = 2 * kDefaultSms / std::min(a.rows, 2 * kDefaultSms);
     int ctas = 1;
-    while (ctas < 16 && (a.vocab > 24000L * ctas || (ctas < most && a.vocab > 2048L * ctas))) ctas *= 2;
+    while (ctas < 16 && (a.vocab > 24000L * ctas || (2 * ctas <= most && a.vocab > 2048L * ctas))) ctas *= 2;
     const int slice = (int)((((long)a.vocab + ctas - 1) / ctas + 15) / 16 * 16);
     auto* kernel = twm::sample::sample_kernel<T>;
     static_assert(twm::sample::MAX_SLICE * 4 + sizeof(twm::sample::Shared) + 1024 < 227 * 1024, "shared memory of a CTA");
@@ -138,9 +139,9 @@ twm_status twm_cache8_append(const twm_cache8* cache, void* q_out, long ldq, con
     if (off16(q_out) || off16(qkv) || off16(bias) || off16(rope_table) || (ldq & 7) || (ldqkv & 7)) return TWM_EALIGN;
     if ((st = ensure_device(nullptr)) != TWM_OK) return st;
     const twm::cache8::AppendArgs a = {device_cache(cache), {row_start, start, rows, max_rows}, (__half*)q_out, (const __half*)qkv, bias, rope_table,
-                                       ldq, ldqkv, num_heads};
+                                       ldq, ldqkv, num_heads, max_rows >= TWM_CACHE8_BLOCK / 4 ? 1 : 0};
     // blocks that max_rows tokens can touch, wherever they begin
-    const dim3 grid((unsigned)(((long)max_rows + 2 * TWM_CACHE8_BLOCK - 2) / TWM_CACHE8_BLOCK), cache->kv_heads, cache->seqs);
+    const dim3 grid((unsigned)(((long)max_rows + 2 * TWM_CACHE8_BLOCK - 2) / TWM_CACHE8_BLOCK), cache->kv_heads + (a.apart ? num_heads : 0), cache->seqs);
     return launch_op("twm_cache8_append", cache->head_dim == 64 ? twm::cache8::append_kernel<64> : twm::cache8::append_kernel<128>, grid,
                      dim3(twm::cache8::APPEND_THREADS), 0, flags, stream, a);
 }

@@ -9,7 +9,6 @@ import torch
 
 from . import _lib
 from ._lib import TwmError, check
-from .cache8 import _on
 from .quantize import _require_cuda, _stream_ptr
 
 _DTYPES = {torch.float32: _lib.TWM_F32, torch.float16: _lib.TWM_F16, torch.bfloat16: _lib.TWM_BF16}
@@ -31,13 +30,12 @@ class SamplingParams:
             raise ValueError("top_k must not be negative, top_p in (0, 1] and min_p in [0, 1]")
 
 
-def _column(name: str, t: Optional[torch.Tensor], dtype: torch.dtype, rows: int, device: torch.device) -> Optional[int]:
+def _column(name: str, t: Optional[torch.Tensor], dtype: torch.dtype, rows: int, index: int) -> Optional[int]:
     if t is None:
         return None
-    if t.dtype is not dtype or t.numel() != rows or not t.is_contiguous() or t.device != device:
-        if not t.is_cuda:
-            _require_cuda(t)
-        raise TwmError(_lib.TWM_EINVAL, f"sample: {name} must be {dtype} [{rows}] on {device}")
+    if t.dtype is not dtype or t.numel() != rows or t.get_device() != index or not t.is_contiguous():
+        _require_cuda(t)
+        raise TwmError(_lib.TWM_EINVAL, f"sample: {name} must be {dtype} [{rows}] on the logits' device")
     return t.data_ptr()
 
 
@@ -52,12 +50,16 @@ def sample(logits: torch.Tensor, random: torch.Tensor, tokens: torch.Tensor, *, 
     dtype = _DTYPES.get(logits.dtype)
     if dtype is None or logits.dim() != 2 or logits.stride(1) != 1:
         raise TwmError(_lib.TWM_EINVAL, "sample: logits must be a float32, float16 or bfloat16 matrix with contiguous rows")
-    (rows, vocab), device, f32, i32 = logits.shape, logits.device, torch.float32, torch.int32
+    rows, vocab, index, f32, i32 = logits.size(0), logits.size(1), logits.get_device(), torch.float32, torch.int32
     if rows == 0:
         return
-    args = _lib.SampleArgs(rows, vocab, dtype, logits.data_ptr(), logits.stride(0) if rows > 1 else vocab, _column("random", random, f32, rows, device),
-                           _column("temperature", temperature, f32, rows, device), _column("top_k", top_k, i32, rows, device),
-                           _column("top_p", top_p, f32, rows, device), _column("min_p", min_p, f32, rows, device),
-                           _column("tokens", tokens, i32, rows, device), _column("prob", prob, f32, rows, device))
-    with _on(device):
-        check(_lib.lib().twm_sample(args, flags, _stream_ptr(stream)), "twm_sample")
+    if torch._C._cuda_getDevice() != index:
+        with torch.cuda.device(index):
+            return sample(logits, random, tokens, temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p, prob=prob, stream=stream, flags=flags)
+    args = _lib.SampleArgs(rows, vocab, dtype, logits.data_ptr(), logits.stride(0) if rows > 1 else vocab, _column("random", random, f32, rows, index),
+                           _column("temperature", temperature, f32, rows, index), _column("top_k", top_k, i32, rows, index),
+                           _column("top_p", top_p, f32, rows, index), _column("min_p", min_p, f32, rows, index),
+                           _column("tokens", tokens, i32, rows, index), _column("prob", prob, f32, rows, index))
+    status = _lib.lib().twm_sample(args, flags, _stream_ptr(stream))
+    if status:
+        check(status, "twm_sample")
