@@ -46,13 +46,18 @@ struct AttnArgs {
 struct Tile { int lo, end; };    // first unit, unit behind the last
 __device__ __forceinline__ Tile tile_units(const Span& sp, int t, int tile, int group, int window)
 {
-    const int rows = sp.n * group, first = sp.pos + t * tile / group, last = sp.pos + (min(rows, (t + 1) * tile) - 1) / group;
+    const int rows = sp.n * group;
+    int first = sp.pos, last = sp.pos + sp.n - 1;
+    if (rows > tile) {
+        first = sp.pos + t * tile / group;
+        last = sp.pos + (min(rows, (t + 1) * tile) - 1) / group;
+    }
     return {(window > first ? 0 : first - window + 1) / BLOCK, last / BLOCK + 1};
 }
 // A tile also takes time of its own, `extra` units' worth, which stand ahead of its units in the line.
 struct Deal {
     int group, tile, window, extra;
-    __device__ __forceinline__ int tiles(const Span& sp) const { return (sp.n * group + tile - 1) / tile; }
+    __device__ __forceinline__ int tiles(const Span& sp) const { return sp.n * group <= tile ? 1 : (sp.n * group + tile - 1) / tile; }
     __device__ __forceinline__ int units(const Span& sp, int t) const
     {
         const Tile x = tile_units(sp, t, tile, group, window);
@@ -70,8 +75,12 @@ struct Deal {
     }
 };
 
+// x / y, neither negative; a 64-bit division takes several times as long as a 32-bit one
+__device__ __forceinline__ long long quotient(long long x, long long y) { return ((x | y) >> 32) == 0 ? (long long)((uint32_t)x / (uint32_t)y) : x / y; }
+
 // Where a CTA's run begins, found by the whole CTA.
 struct Start {
+    bool out;                    // whether a sequence is out of the call
     long long units;             // of the CTA
     long long share;             // of every CTA but the last ones
     long long before;            // units of the sequence ahead of the run
@@ -92,7 +101,11 @@ __device__ __forceinline__ Start find_start(const AttnArgs& a, const Deal& deal,
         return (by_warp ? deal.units_by_warp(sp) : sp.n > 0 ? (long long)deal.units(sp, 0) : 0LL) * a.c.kv_heads;
     };
     long long mine = 0;
-    for (int s = s0; s < s1; ++s) mine += units(s);
+    bool out = false;
+    for (int s = s0; s < s1; ++s) {
+        mine += units(s);
+        out |= a.r.start[s] < 0;
+    }
     long long upto = mine;
     if (!by_warp) {
 #pragma unroll
@@ -102,28 +115,30 @@ __device__ __forceinline__ Start find_start(const AttnArgs& a, const Deal& deal,
         }
     }
     if (lane == 31) sums[tid / 32] = upto;
-    if (tid == 0) found = {0, 0, 0, 0};
-    __syncthreads();
+    if (tid == 0) found = {false, 0, 0, 0, 0};
+    out = __syncthreads_or(out);
     long long base = 0, total = 0;
     for (int w = 0; w < THREADS / 32; ++w) {
         if (w < tid / 32) base += sums[w];
         total += sums[w];
     }
     upto += base;
-    const long long share = max(1LL, (total + ctas - 1) / ctas), begin = min(total, share * cta), end = min(total, begin + share);
+    const long long share = max(1LL, quotient(total + ctas - 1, ctas)), begin = min(total, share * cta), end = min(total, begin + share);
     if (begin < end && upto - mine <= begin && begin < upto) {           // the same in all lanes of a warp where warps take sequences
         long long at = upto - mine;
         for (int s = s0; s < s1; ++s) {
             const long long n = units(s);
             if (begin < at + n) {
-                if (!by_warp || lane == 0) found = {end - begin, share, begin - at, s};
+                if (!by_warp || lane == 0) found = {false, end - begin, share, begin - at, s};
                 break;
             }
             at += n;
         }
     }
     __syncthreads();
-    return found;
+    Start start = found;
+    start.out = out;
+    return start;
 }
 
 // The tiles of a CTA's run, one after another.
@@ -154,7 +169,7 @@ struct Walk {
         sp = span_of(a.r, seq, a.c.capacity);
         const int n = d.tiles(sp), lane = threadIdx.x & 31;
         const long long per = n == 1 ? d.units(sp, 0) : d.units_by_warp(sp);
-        head = (int)(s.before / per);
+        head = (int)quotient(s.before, per);
         int rest = (int)(s.before - head * per);
         t = 0;
         while (n > 1) {                                                  // 32 tiles at a time
@@ -222,22 +237,22 @@ __device__ __forceinline__ float ex2(float x) { float y; asm("ex2.approx.ftz.f32
 __device__ __forceinline__ int exponent_of(float scale) { return (int)(__float_as_uint(scale) >> 23) - 127; }
 
 // --------------------------------------------------------------------------------------------- few rows a sequence --
-// Up to 8 NT rows a sequence and key/value head (the query heads that share it, times the new tokens): a tile is all of them, and every key is
-// read once.  Bound by HBM.  Four consumer warps take 16 keys each of a unit, a producer warp brings units by TMA into a ring that runs on over
-// the borders of tiles.  S^T = K Q^T and O^T += V^T P^T as mma.m16n8k16 with the keys, and then the head's elements, as the 16 rows, so that eight
-// rows of queries are a whole operand.  Elements and keys may stand in any order in a sum: lane (g, t) takes 32 elements of keys g and g + 8 for the
-// scores (two 16-byte reads a key, 4 codes a k-step of both registers), and 16 elements of four keys for the output, whose codes
-// are paired by a byte permutation; both reads are free of bank conflicts in the layout that the TMA's swizzle leaves.  P^T needs only a
-// transposition of 8 x 8.  Each warp has its own m; they are joined when the tile ends.
+// Up to 8 NT rows a sequence and key/value head (the query heads that share it, times the new tokens): they are one tile, and every key is
+// read once.  Bound by HBM.  Four consumer warps take 16 keys each of a unit; a producer warp brings units by TMA into a ring that runs on over
+// the borders of tiles, the tail's FP16 rows among them (keys and values in a stage each).  S^T = K Q^T and O^T += V^T P^T as mma.m16n8k16 with
+// the keys, and then the head's elements, as the 16 rows, so that eight rows of queries are a whole operand.  Elements and keys may stand in any
+// order in a sum: lane (g, t) takes D / 4 elements of keys g and g + 8 for the scores (4 codes a k-step of both registers), and D / 8 elements of
+// four keys for the output, whose codes are paired by a byte permutation; at D = 128 both reads are free of bank conflicts in the
+// layout that the TMA's swizzle leaves.  P^T needs only a transposition of 8 x 8.  Each warp has its own m; when the tile ends the four add up in
+// shared memory, while the next tile's queries are on their way.
 constexpr int FEW_EXTRA = 1;                                             // a tile's own time, in units
 constexpr int FEW_WARPS = 4, FEW_THREADS = 32 * FEW_WARPS + 32;
 template <int D, int NT>
 struct Few {
-    static constexpr int STAGE = 2 * BLOCK * D;                          // bytes: keys, values
-    static constexpr int CTAS = NT == 4 ? 1 : 2;                         // to an SM
-    static constexpr int STAGES = NT == 4 ? 10 * 128 / D : 6 * 128 / D;
+    static constexpr int STAGE = 2 * BLOCK * D;                          // bytes: codes of keys and values, or the tail's of one of them
+    static constexpr int STAGES = (NT == 1 ? 5 : 4) * 128 / D;
     static constexpr int TILE = 8 * NT;
-    static constexpr size_t SMEM = 1024 + (size_t)STAGES * STAGE + (size_t)TILE * D * 4;
+    static constexpr size_t SMEM = 1024 + (size_t)STAGES * STAGE + (size_t)FEW_WARPS * TILE * D * 4;
 };
 
 __device__ __forceinline__ uint32_t codes_f16(uint32_t pair)            // two codes in the low half
@@ -270,7 +285,7 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi)
 }
 
 template <int D, int NT>
-__global__ void __launch_bounds__(FEW_THREADS, Few<D, NT>::CTAS)
+__global__ void __launch_bounds__(FEW_THREADS, 2)
 few_kernel(const __grid_constant__ AttnArgs a)
 {
     using F = Few<D, NT>;
@@ -280,18 +295,21 @@ few_kernel(const __grid_constant__ AttnArgs a)
     __shared__ float s_m[FEW_WARPS][F::TILE], s_l[FEW_WARPS][F::TILE];
     __shared__ int s_abort;
     uint8_t* stages = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(few_raw) + 1023) & ~(uintptr_t)1023);
-    float* join = reinterpret_cast<float*>(stages + (size_t)F::STAGES * F::STAGE);
+    float4* join = reinterpret_cast<float4*>(stages + (size_t)F::STAGES * F::STAGE);         // [warp][row][D / 4], a row's turned about by the row
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (tid == 0) {
         for (int i = 0; i < F::STAGES; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], FEW_WARPS); }
         s_abort = 0;
         mbar_fence_init();
+    } else if (tid == 32 * FEW_WARPS) {
+        asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&a.k_map)) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&a.v_map)) : "memory");
     }
     pdl_launch_dependents();
     pdl_wait_prior_grids();
     const Deal deal = {a.num_heads / a.c.kv_heads, F::TILE, a.window, FEW_EXTRA};
     const Start start = find_start<FEW_THREADS>(a, deal, blockIdx.x, gridDim.x);
-    zero_rows(a, D, blockIdx.x, gridDim.x, tid, FEW_THREADS);
+    if (start.out) zero_rows(a, D, blockIdx.x, gridDim.x, tid, FEW_THREADS);
     Walk w;
     if (!w.begin(a, deal, start)) {
         if (tid == 0) a.joins[blockIdx.x].parts = 0;
@@ -303,16 +321,33 @@ few_kernel(const __grid_constant__ AttnArgs a)
         if (lane == 0) {
             int i = 0;
             bool ok = true;
+            auto slot = [&]() {                                          // the next stage, free
+                const int x = i % F::STAGES;
+                if (i >= F::STAGES) ok = ok && mbar_wait_bounded(&empty[x], (uint32_t)(i / F::STAGES - 1) & 1u, abort_flag);
+                ++i;
+                return x;
+            };
             do {
-                const int held = (w.sp.pos + w.sp.n) / BLOCK;           // units that are codes
+                const int length = w.sp.pos + w.sp.n, held = length / BLOCK;         // units that are codes
+                const size_t at = (size_t)w.seq * a.c.kv_heads + w.head;
                 const int row0 = (w.seq * a.c.kv_heads + w.head) * a.c.capacity;
-                for (int u = w.u0; u < min(w.u0 + w.n, held) && ok; ++u, ++i) {
-                    const int slot = i % F::STAGES;
-                    if (i >= F::STAGES) ok = mbar_wait_bounded(&empty[slot], (uint32_t)(i / F::STAGES - 1) & 1u, abort_flag);
-                    if (!ok) break;
-                    mbar_arrive_expect_tx(&full[slot], F::STAGE);
-                    tma_load_2d(stages + slot * F::STAGE, &a.k_map, 0, row0 + u * BLOCK, &full[slot]);
-                    tma_load_2d(stages + slot * F::STAGE + BLOCK * D, &a.v_map, 0, row0 + u * BLOCK, &full[slot]);
+                for (int u = w.u0; u < w.u0 + w.n && ok; ++u) {
+                    if (u < held) {
+                        const int x = slot();
+                        if (!ok) break;
+                        mbar_arrive_expect_tx(&full[x], F::STAGE);
+                        tma_load_2d(stages + x * F::STAGE, &a.k_map, 0, row0 + u * BLOCK, &full[x]);
+                        tma_load_2d(stages + x * F::STAGE + BLOCK * D, &a.v_map, 0, row0 + u * BLOCK, &full[x]);
+                    } else {                                             // the tokens of the tail that are there
+                        const uint32_t bytes = (uint32_t)(length - u * BLOCK) * D * 2;
+                        const size_t from = (at * 2 + (u & 1)) * BLOCK * D;
+                        for (int side = 0; side < 2; ++side) {
+                            const int x = slot();
+                            if (!ok) break;
+                            mbar_arrive_expect_tx(&full[x], bytes);
+                            bulk_g2s(stages + x * F::STAGE, (side ? a.c.v_tail : a.c.k_tail) + from, bytes, &full[x]);
+                        }
+                    }
                 }
             } while (ok && w.next(a, deal));
         }
@@ -334,31 +369,37 @@ few_kernel(const __grid_constant__ AttnArgs a)
         const int row = warp * 16 + 2 * t + (j & 1) + (j >> 1) * 8;
         v_at[j] = BLOCK * D + (D == 128 ? word(row, g) : word(row, g >> 1) + (g & 1) * 8);
     }
-
-    int i = 0;
-    do {                                                                 // a warp whose wait ran out goes on to the end, so that all meet at the barriers
-        const int row0 = w.t * F::TILE, rows = min(F::TILE, w.sp.n * deal.group - row0), length = w.sp.pos + w.sp.n, held = length / BLOCK;
-        const size_t at = (size_t)w.seq * a.c.kv_heads + w.head;
-        uint32_t q[NT][KS][2];
-        int pos[NT][2];                                                  // of the two rows whose scores this lane has
+    int q_token[NT], token[NT][2];                                       // of this lane's row of the queries, and of its two rows of the scores
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+        q_token[nt] = (nt * 8 + g) / deal.group;
+        token[nt][0] = (nt * 8 + 2 * t) / deal.group;
+        token[nt][1] = (nt * 8 + 2 * t + 1) / deal.group;
+    }
+    uint32_t q[NT][KS][2];
+    auto load_queries = [&](const Walk& w, uint32_t (&q)[NT][KS][2]) {   // rows that are not there are zeros
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-            const int r = nt * 8 + g;
-            const bool live = r < rows;
-            const int rq = row0 + min(r, rows - 1);                     // rows that are not there: zeros at the last one's position
-            const __half* src = a.q + (size_t)(w.sp.row + rq / deal.group) * a.ldq + (w.head * deal.group + rq % deal.group) * D + t * (D / 4);
+            const bool live = q_token[nt] < w.sp.n;
+            const __half* src = a.q + (size_t)(w.sp.row + min(q_token[nt], w.sp.n - 1)) * a.ldq +
+                                (w.head * deal.group + nt * 8 + g - q_token[nt] * deal.group) * D + t * (D / 4);
 #pragma unroll
             for (int j = 0; j < D / 32; ++j) {
                 const uint4 v = live ? reinterpret_cast<const uint4*>(src)[j] : make_uint4(0, 0, 0, 0);
                 q[nt][2 * j][0] = v.x; q[nt][2 * j][1] = v.y;
                 q[nt][2 * j + 1][0] = v.z; q[nt][2 * j + 1][1] = v.w;
             }
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                pos[nt][c] = w.sp.pos + (row0 + min(nt * 8 + 2 * t + c, rows - 1)) / deal.group;
-            }
         }
-        const int first = w.sp.pos + row0 / deal.group, last = w.sp.pos + (row0 + rows - 1) / deal.group;
+    };
+    load_queries(w, q);
+
+    int i = 0;
+    for (bool more = true; more;) {                                      // a warp whose wait ran out goes on to the end, so that all meet at the barriers
+        const int first = w.sp.pos, last = w.sp.pos + w.sp.n - 1, length = last + 1, held = length / BLOCK;
+        const size_t at = (size_t)w.seq * a.c.kv_heads + w.head;
+        const float* k_scale = a.c.k_scale + at * (a.c.capacity / BLOCK);
+        const float* v_scale = a.c.v_scale + at * (a.c.capacity / BLOCK);
+        float ks = w.u0 < held ? k_scale[w.u0] : 1.0f, vs = w.u0 < held ? v_scale[w.u0] : 1.0f;
         float o[KS][NT][4], m[NT][2], l[NT][2];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
@@ -370,22 +411,19 @@ few_kernel(const __grid_constant__ AttnArgs a)
                 for (int c = 0; c < 4; ++c) o[mt][nt][c] = 0.0f;
         }
         for (int u = w.u0; u < w.u0 + w.n; ++u) {
-            float s[NT][4];
+            float s[2][NT][4];                                           // two sums, so that a product waits for the one before the last
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                for (int c = 0; c < 4; ++c) s[nt][c] = 0.0f;
-            uint32_t vw[4][DPL / 4];                              // codes of this lane's elements of four keys
-            uint32_t vt[4][DPL / 2];                                     // the tail's, FP16
-            float factor = a.scale * LOG2E, inv = 1.0f;
-            int ev = 0;
+                for (int c = 0; c < 4; ++c) s[0][nt][c] = s[1][nt][c] = 0.0f;
+            uint32_t vw[4][DPL / 4];                                     // codes of this lane's elements of four keys
+            const float factor = a.scale * LOG2E * ks, inv = power_of_two(-exponent_of(vs)), ev = (float)exponent_of(vs);
+            if (u + 1 < w.u0 + w.n) { ks = u + 1 < held ? k_scale[u + 1] : 1.0f; vs = u + 1 < held ? v_scale[u + 1] : 1.0f; }
             const bool codes = u < held;
+            const int valid = length - u * BLOCK;                        // tokens of the tail that are there; what lies behind them is taken as zeros
+            const uint32_t src = base + i % F::STAGES * F::STAGE;
+            tc::wait_uniform(&full[i % F::STAGES], (uint32_t)(i / F::STAGES) & 1u, abort_flag);
             if (codes) {
-                const size_t sc = at * (a.c.capacity / BLOCK) + u;
-                const float ks = a.c.k_scale[sc], vs = a.c.v_scale[sc];
-                const int slot = i % F::STAGES;
-                tc::wait_uniform(&full[slot], (uint32_t)(i / F::STAGES) & 1u, abort_flag);
-                const uint32_t src = base + slot * F::STAGE;
                 uint4 kw[2][WK];
 #pragma unroll
                 for (int j = 0; j < WK; ++j)
@@ -400,9 +438,6 @@ few_kernel(const __grid_constant__ AttnArgs a)
                     else
                         asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(vw[j][0]), "=r"(vw[j][1]) : "r"(src + v_at[j]));
                 }
-                factor *= ks;
-                ev = exponent_of(vs);
-                inv = power_of_two(-ev);
 #pragma unroll
                 for (int j = 0; j < WK; ++j) {
                     const uint32_t x[4] = {kw[0][j].x, kw[0][j].y, kw[0][j].z, kw[0][j].w}, y[4] = {kw[1][j].x, kw[1][j].y, kw[1][j].z, kw[1][j].w};
@@ -410,33 +445,26 @@ few_kernel(const __grid_constant__ AttnArgs a)
                     for (int k = 0; k < 4; ++k) {
                         const uint32_t a0 = codes_f16(x[k]), a1 = codes_f16(y[k]), a2 = codes_f16_hi(x[k]), a3 = codes_f16_hi(y[k]);
 #pragma unroll
-                        for (int nt = 0; nt < NT; ++nt) mma_16x8x16(s[nt], a0, a1, a2, a3, q[nt][j * 4 + k][0], q[nt][j * 4 + k][1]);
+                        for (int nt = 0; nt < NT; ++nt) mma_16x8x16(s[k & 1][nt], a0, a1, a2, a3, q[nt][j * 4 + k][0], q[nt][j * 4 + k][1]);
                     }
                 }
             } else {
-                // the tail, FP16, from its place in memory; rows behind the sequence's end are taken as zeros
-                const __half *kt = a.c.k_tail + (at * 2 + (u & 1)) * BLOCK * D, *vt_ = a.c.v_tail + (at * 2 + (u & 1)) * BLOCK * D;
-                const int valid = length - u * BLOCK;
+                const uint8_t* kt = stages + i % F::STAGES * F::STAGE;
                 const uint4 none = make_uint4(0, 0, 0, 0);
 #pragma unroll
                 for (int j = 0; j < D / 32; ++j) {
-                    const uint4 x = key0 < valid ? reinterpret_cast<const uint4*>(kt + key0 * D + t * (D / 4))[j] : none;
-                    const uint4 y = key1 < valid ? reinterpret_cast<const uint4*>(kt + key1 * D + t * (D / 4))[j] : none;
+                    const uint4 x = key0 < valid ? reinterpret_cast<const uint4*>(kt + key0 * D * 2 + t * (D / 2))[j] : none;
+                    const uint4 y = key1 < valid ? reinterpret_cast<const uint4*>(kt + key1 * D * 2 + t * (D / 2))[j] : none;
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
-                        mma_16x8x16(s[nt], x.x, y.x, x.y, y.y, q[nt][2 * j][0], q[nt][2 * j][1]);
-                        mma_16x8x16(s[nt], x.z, y.z, x.w, y.w, q[nt][2 * j + 1][0], q[nt][2 * j + 1][1]);
+                        mma_16x8x16(s[0][nt], x.x, y.x, x.y, y.y, q[nt][2 * j][0], q[nt][2 * j][1]);
+                        mma_16x8x16(s[1][nt], x.z, y.z, x.w, y.w, q[nt][2 * j + 1][0], q[nt][2 * j + 1][1]);
                     }
                 }
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int row = warp * 16 + 2 * t + (j & 1) + (j >> 1) * 8;
-#pragma unroll
-                    for (int k = 0; k < DPL / 8; ++k) {
-                        const uint4 x = row < valid ? reinterpret_cast<const uint4*>(vt_ + row * D + g * DPL)[k] : none;
-                        vt[j][4 * k] = x.x; vt[j][4 * k + 1] = x.y; vt[j][4 * k + 2] = x.z; vt[j][4 * k + 3] = x.w;
-                    }
-                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&empty[i % F::STAGES]);
+                ++i;
+                tc::wait_uniform(&full[i % F::STAGES], (uint32_t)(i / F::STAGES) & 1u, abort_flag);
             }
             // exponents, masked where not every row sees every key of the unit
             const bool all_seen = (u + 1) * BLOCK - 1 <= first && last - u * BLOCK < a.window;
@@ -445,19 +473,20 @@ few_kernel(const __grid_constant__ AttnArgs a)
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
-                    s[nt][c] = fmaf(s[nt][c], factor, (float)ev);
+                    float x = fmaf(s[0][nt][c] + s[1][nt][c], factor, ev);
                     if (!all_seen) {
-                        const int key = u * BLOCK + (c < 2 ? key0 : key1), p = pos[nt][c & 1];
-                        if (!(key <= p && p - key < a.window)) s[nt][c] = -INFINITY;
+                        const int key = u * BLOCK + (c < 2 ? key0 : key1), p = first + min(token[nt][c & 1], w.sp.n - 1);
+                        if (!(key <= p && p - key < a.window)) x = -INFINITY;
                     }
-                    over |= s[nt][c] > m[nt][c & 1] + 8.0f;
+                    s[0][nt][c] = x;
+                    over |= x > m[nt][c & 1] + 8.0f;
                 }
             if (__any_sync(0xffffffffu, over)) {
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                     for (int c = 0; c < 2; ++c) {
-                        float top = fmaxf(s[nt][c], s[nt][c + 2]);
+                        float top = fmaxf(s[0][nt][c], s[0][nt][c + 2]);
 #pragma unroll
                         for (int x = 4; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
                         if (top > m[nt][c]) {
@@ -474,7 +503,7 @@ few_kernel(const __grid_constant__ AttnArgs a)
             for (int nt = 0; nt < NT; ++nt) {
                 float e[4];
 #pragma unroll
-                for (int c = 0; c < 4; ++c) e[c] = ex2(s[nt][c] - (m[nt][c & 1] == -INFINITY ? 0.0f : m[nt][c & 1]));
+                for (int c = 0; c < 4; ++c) e[c] = ex2(s[0][nt][c] - (m[nt][c & 1] == -INFINITY ? 0.0f : m[nt][c & 1]));
                 l[nt][0] = fmaf(e[0] + e[2], inv, l[nt][0]);
                 l[nt][1] = fmaf(e[1] + e[3], inv, l[nt][1]);
                 p[nt][0] = transposed_8x8(pack_f16(e[0], e[1]));
@@ -493,79 +522,83 @@ few_kernel(const __grid_constant__ AttnArgs a)
                         mma_16x8x16(o[2 * k + 1][nt], b0, b1, b2, b3, p[nt][0], p[nt][1]);
                     }
                 }
-                // Not ahead of the products: words that were only asked for were overtaken by the next copy in a call of forty.
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&empty[i % F::STAGES]);
-                ++i;
             } else {
+                const uint8_t* vt = stages + i % F::STAGES * F::STAGE;
+                const uint4 none = make_uint4(0, 0, 0, 0);
 #pragma unroll
-                for (int mt = 0; mt < KS; ++mt) {
-                    const uint32_t a0 = __byte_perm(vt[0][mt], vt[1][mt], 0x5410), a1 = __byte_perm(vt[0][mt], vt[1][mt], 0x7632);
-                    const uint32_t a2 = __byte_perm(vt[2][mt], vt[3][mt], 0x5410), a3 = __byte_perm(vt[2][mt], vt[3][mt], 0x7632);
+                for (int k = 0; k < DPL / 8; ++k) {                      // eight elements: four m-tiles
+                    uint4 x[4];
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) mma_16x8x16(o[mt][nt], a0, a1, a2, a3, p[nt][0], p[nt][1]);
+                    for (int j = 0; j < 4; ++j) {
+                        const int row = warp * 16 + 2 * t + (j & 1) + (j >> 1) * 8;
+                        x[j] = row < valid ? reinterpret_cast<const uint4*>(vt + row * D * 2 + g * DPL * 2)[k] : none;
+                    }
+                    const uint32_t y[4][4] = {{x[0].x, x[1].x, x[2].x, x[3].x}, {x[0].y, x[1].y, x[2].y, x[3].y}, {x[0].z, x[1].z, x[2].z, x[3].z}, {x[0].w, x[1].w, x[2].w, x[3].w}};
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const uint32_t a0 = __byte_perm(y[e][0], y[e][1], 0x5410), a1 = __byte_perm(y[e][0], y[e][1], 0x7632);
+                        const uint32_t a2 = __byte_perm(y[e][2], y[e][3], 0x5410), a3 = __byte_perm(y[e][2], y[e][3], 0x7632);
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) mma_16x8x16(o[4 * k + e][nt], a0, a1, a2, a3, p[nt][0], p[nt][1]);
+                    }
                 }
             }
+            // Not ahead of the products: words that were only asked for were overtaken by the next copy in a call of forty.
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&empty[i % F::STAGES]);
+            ++i;
         }
-        // ---- the four warps' parts of the tile, in warp order ----
+        // ---- the next tile's queries are asked for, then the four warps' parts of this one are added up ----
+        const int rows = w.sp.n * deal.group;
+        const bool alone = w.begins && w.ends;
+        float* part = a.partial + (2 * (size_t)blockIdx.x + (w.begins ? 1 : 0)) * partial_floats(F::TILE, D);
+        __half* out = a.out + (size_t)w.sp.row * a.ldo + w.head * deal.group * D;
+        more = w.next(a, deal);
+        if (more) load_queries(w, q);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
+            for (int c = 0; c < 2; ++c)
 #pragma unroll
                 for (int x = 4; x < 32; x <<= 1) l[nt][c] += __shfl_xor_sync(0xffffffffu, l[nt][c], x);
-                if (g == 0) { s_m[warp][nt * 8 + 2 * t + c] = m[nt][c]; s_l[warp][nt * 8 + 2 * t + c] = l[nt][c]; }
-            }
-        named_bar_sync(1, 32 * FEW_WARPS);
-        float f[NT][2];
+        named_bar_sync(1, 32 * FEW_WARPS);                               // the tile before has been read
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
                 const int r = nt * 8 + 2 * t + c;
-                const float top = fmaxf(fmaxf(s_m[0][r], s_m[1][r]), fmaxf(s_m[2][r], s_m[3][r]));
-                f[nt][c] = ex2(m[nt][c] - (top == -INFINITY ? 0.0f : top));      // a NaN sum stays one
+                if (g == 0) { s_m[warp][r] = m[nt][c]; s_l[warp][r] = l[nt][c]; }
+                float4* row = join + (warp * F::TILE + r) * (D / 4);     // this lane's elements, DPL of them: m-tile mt has 2 mt and 2 mt + 1
+#pragma unroll
+                for (int j = 0; j < DPL / 4; ++j)
+                    row[(g * (DPL / 4) + j) ^ t] = make_float4(o[2 * j][nt][c], o[2 * j][nt][c + 2], o[2 * j + 1][nt][c], o[2 * j + 1][nt][c + 2]);
             }
-        for (int turn = 0; turn < FEW_WARPS; ++turn) {
-            if (turn == warp) {
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        float* row = join + (nt * 8 + 2 * t + c) * D + g * DPL;      // elements 2 mt, 2 mt + 1 of this lane's
-#pragma unroll
-                        for (int mt = 0; mt < KS; ++mt) {
-                            float2 v = make_float2(o[mt][nt][c] * f[nt][c], o[mt][nt][c + 2] * f[nt][c]);
-                            if (turn > 0) { const float2 x = *reinterpret_cast<float2*>(row + 2 * mt); v.x += x.x; v.y += x.y; }
-                            *reinterpret_cast<float2*>(row + 2 * mt) = v;
-                        }
-                    }
-            }
-            named_bar_sync(1, 32 * FEW_WARPS);
-        }
-        // ---- out, or to the workspace where other CTAs have keys of the tile ----
-        const bool alone = w.begins && w.ends, ok = *abort_flag == 0;
-        float* part = a.partial + (2 * (size_t)blockIdx.x + (w.begins ? 1 : 0)) * partial_floats(F::TILE, D);
+        named_bar_sync(1, 32 * FEW_WARPS);
+        const bool ok = *abort_flag == 0;
         for (int j = tid; j < rows * (D / 4); j += 32 * FEW_WARPS) {
-            const int r = j / (D / 4), d = j % (D / 4) * 4;
-            const float4 v = *reinterpret_cast<const float4*>(join + r * D + d);
-            const float top = fmaxf(fmaxf(s_m[0][r], s_m[1][r]), fmaxf(s_m[2][r], s_m[3][r]));
-            const float ref = top == -INFINITY ? 0.0f : top;
+            const int r = j / (D / 4), d = j % (D / 4);
+            const float top = fmaxf(fmaxf(s_m[0][r], s_m[1][r]), fmaxf(s_m[2][r], s_m[3][r])), ref = top == -INFINITY ? 0.0f : top;
+            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
             float sum = 0.0f;
 #pragma unroll
-            for (int x = 0; x < FEW_WARPS; ++x) sum = fmaf(s_l[x][r], ex2(s_m[x][r] - ref), sum);
+            for (int x = 0; x < FEW_WARPS; ++x) {                        // in warp order; a NaN sum stays one
+                const float f = ex2(s_m[x][r] - ref);
+                const float4 y = join[(x * F::TILE + r) * (D / 4) + (d ^ ((r >> 1) & 3))];
+                v.x = fmaf(y.x, f, v.x); v.y = fmaf(y.y, f, v.y); v.z = fmaf(y.z, f, v.z); v.w = fmaf(y.w, f, v.w);
+                sum = fmaf(s_l[x][r], f, sum);
+            }
             if (!ok) continue;
             if (alone) {
                 const float n = 1.0f / sum;
-                __half* dst = a.out + (size_t)(w.sp.row + (row0 + r) / deal.group) * a.ldo + (w.head * deal.group + (row0 + r) % deal.group) * D + d;
-                *reinterpret_cast<uint2*>(dst) = make_uint2(pack_f16(v.x * n, v.y * n), pack_f16(v.z * n, v.w * n));
+                const int i_token = r / deal.group;
+                *reinterpret_cast<uint2*>(out + (size_t)i_token * a.ldo + (r - i_token * deal.group) * D + d * 4) =
+                    make_uint2(pack_f16(v.x * n, v.y * n), pack_f16(v.z * n, v.w * n));
             } else {
-                *reinterpret_cast<float4*>(part + r * D + d) = v;
+                reinterpret_cast<float4*>(part + r * D)[d] = v;
                 if (d == 0) { part[F::TILE * D + r] = top; part[F::TILE * (D + 1) + r] = sum; }
             }
         }
-        named_bar_sync(1, 32 * FEW_WARPS);                               // `join` and the statistics are the next tile's
-    } while (w.next(a, deal));
+    }
     if (tid == 0) leave_word(a, deal, w, start);
 }
 

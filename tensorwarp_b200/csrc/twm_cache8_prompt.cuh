@@ -94,7 +94,7 @@ prompt_kernel(const __grid_constant__ AttnArgs a)
     pdl_wait_prior_grids();
     const Deal deal = {a.num_heads / a.c.kv_heads, PROMPT_ROWS, a.window, PROMPT_EXTRA};
     const Start start = find_start<PROMPT_THREADS>(a, deal, blockIdx.x, gridDim.x);
-    zero_rows(a, D, blockIdx.x, gridDim.x, tid, PROMPT_THREADS);
+    if (start.out) zero_rows(a, D, blockIdx.x, gridDim.x, tid, PROMPT_THREADS);
     Walk w;
     if (!w.begin(a, deal, start)) {
         if (tid == 0) a.joins[blockIdx.x].parts = 0;
