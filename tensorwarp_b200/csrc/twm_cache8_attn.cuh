@@ -208,6 +208,47 @@ struct Walk {
     }
 };
 
+// The same where every sequence has one tile and there are at most 128 of them: every warp finds the start by itself, a few neighbouring sequences
+// a lane, in 32 bits (units of all sequences: cached rows / 64, and one tile more each).  2.3 + 1.0 thousand clocks of a call for one sequence
+// with find_start and begin, MEASURED this way.
+constexpr int START_BY_WARP = 128;
+__device__ __forceinline__ bool begin_by_warp(const AttnArgs& a, const Deal& d, int cta, int ctas, Start& start, Walk& w)
+{
+    const int lane = threadIdx.x & 31, per = (a.c.seqs + 31) / 32, s0 = min(a.c.seqs, lane * per), s1 = min(a.c.seqs, s0 + per);
+    int mine = 0;
+    bool out = false;
+    for (int s = s0; s < s1; ++s) {
+        const Span sp = span_of(a.r, s, a.c.capacity);
+        if (sp.n > 0) mine += d.units(sp, 0) * a.c.kv_heads;
+        out |= sp.pos < 0;
+    }
+    int upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += v;
+    }
+    const int total = __shfl_sync(0xffffffffu, upto, 31), share = max(1, (total + ctas - 1) / ctas);
+    const int begin = (int)min((long long)share * cta, (long long)total), end = min(total, begin + share);
+    start = {__any_sync(0xffffffffu, out) != 0, end - begin, share, 0, 0};
+    if (begin >= end) return false;
+    const unsigned int in = __ballot_sync(0xffffffffu, begin < upto);
+    const int owner = __ffs(in) - 1;
+    int before = begin - __shfl_sync(0xffffffffu, upto - mine, owner), seq = owner * per, units = 0;
+    for (;; ++seq) {                                                     // every lane along the owner's sequences
+        w.sp = span_of(a.r, seq, a.c.capacity);
+        units = w.sp.n > 0 ? d.units(w.sp, 0) : 0;
+        if (before < units * a.c.kv_heads) break;
+        before -= units * a.c.kv_heads;
+    }
+    w.left = end - begin;
+    w.seq = seq;
+    w.head = before / units;
+    w.t = 0;
+    w.take(d, before - w.head * units);
+    return w.n > 0;
+}
+
 // Leaves word for merge_kernel of the run's last tile (`w` stands there), or that there is none.
 __device__ __forceinline__ void leave_word(const AttnArgs& a, const Deal& d, const Walk& w, const Start& s)
 {
@@ -308,10 +349,18 @@ few_kernel(const __grid_constant__ AttnArgs a)
     pdl_launch_dependents();
     pdl_wait_prior_grids();
     const Deal deal = {a.num_heads / a.c.kv_heads, F::TILE, a.window, FEW_EXTRA};
-    const Start start = find_start<FEW_THREADS>(a, deal, blockIdx.x, gridDim.x);
-    if (start.out) zero_rows(a, D, blockIdx.x, gridDim.x, tid, FEW_THREADS);
+    Start start;
     Walk w;
-    if (!w.begin(a, deal, start)) {
+    bool any;
+    if (a.c.seqs <= START_BY_WARP) {
+        any = begin_by_warp(a, deal, blockIdx.x, gridDim.x, start, w);
+        __syncthreads();                                                 // the barriers are there
+    } else {
+        start = find_start<FEW_THREADS>(a, deal, blockIdx.x, gridDim.x);
+        any = w.begin(a, deal, start);
+    }
+    if (start.out) zero_rows(a, D, blockIdx.x, gridDim.x, tid, FEW_THREADS);
+    if (!any) {
         if (tid == 0) a.joins[blockIdx.x].parts = 0;
         return;
     }
@@ -624,11 +673,12 @@ merge_kernel(const __grid_constant__ AttnArgs a, int tile)
     const float* base = a.partial + (2 * (size_t)blockIdx.x + 1) * each;         // part j > 0: the first of CTA x + j
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
     float top = -INFINITY, l = 0.0f;
-    for (int j0 = side; j0 < w.parts; j0 += 4 * SIDES) {
-        float4 x[4];
-        float m[4], n[4];
+    constexpr int AT_ONCE = 4;
+    for (int j0 = side; j0 < w.parts; j0 += AT_ONCE * SIDES) {
+        float4 x[AT_ONCE];
+        float m[AT_ONCE], n[AT_ONCE];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < AT_ONCE; ++i) {
             const int j = j0 + i * SIDES;
             const float* p = j == 0 ? base : base + (2 * (size_t)j - 1) * each;
             const bool there = j < w.parts;
@@ -636,13 +686,16 @@ merge_kernel(const __grid_constant__ AttnArgs a, int tile)
             m[i] = there ? p[tile * D + r] : -INFINITY;
             n[i] = there ? p[tile * (D + 1) + r] : 0.0f;
         }
-        const float now = fmaxf(fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])), top), ref = now == -INFINITY ? 0.0f : now;
+        float now = top;
+#pragma unroll
+        for (int i = 0; i < AT_ONCE; ++i) now = fmaxf(now, m[i]);
+        const float ref = now == -INFINITY ? 0.0f : now;
         const float f = ex2(top - ref);
         v.x *= f; v.y *= f; v.z *= f; v.w *= f;
         l *= f;
         top = now;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < AT_ONCE; ++i) {
             const float g = ex2(m[i] - ref);
             v.x = fmaf(x[i].x, g, v.x); v.y = fmaf(x[i].y, g, v.y); v.z = fmaf(x[i].z, g, v.z); v.w = fmaf(x[i].w, g, v.w);
             l = fmaf(n[i], g, l);

@@ -102,8 +102,8 @@ template <int D>
 twm_status launch_merge(const twm::cache8::AttnArgs& a, const AttnPlan& p, int flags, void* stream)
 {
     const bool many = p.tile == twm::cache8::PROMPT_ROWS;
-    const int rows = twm::cache8::MERGE_THREADS / (D / 4) / (many ? 1 : 4);
-    return launch_op("twm_cache8_attention(merge)", many ? twm::cache8::merge_kernel<D, 1> : twm::cache8::merge_kernel<D, 4>,
+    const int rows = twm::cache8::MERGE_THREADS / (D / 4) / (many ? 1 : 8);
+    return launch_op("twm_cache8_attention(merge)", many ? twm::cache8::merge_kernel<D, 1> : twm::cache8::merge_kernel<D, 8>,
                      dim3(p.ctas, (p.tile + rows - 1) / rows), dim3(twm::cache8::MERGE_THREADS), 0, flags | TWM_FLAG_PDL, stream, a, p.tile);
 }
 
