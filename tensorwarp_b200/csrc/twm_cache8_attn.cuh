@@ -286,12 +286,13 @@ __device__ __forceinline__ int exponent_of(float scale) { return (int)(__float_a
 // four keys for the output, whose codes are paired by a byte permutation; at D = 128 both reads are free of bank conflicts in the
 // layout that the TMA's swizzle leaves.  P^T needs only a transposition of 8 x 8.  Each warp has its own m; when the tile ends the four add up in
 // shared memory, while the next tile's queries are on their way.
-constexpr int FEW_EXTRA = 1;                                             // a tile's own time, in units
+constexpr int FEW_EXTRA = 4;                                             // a tile's own time, in units (96 sequences: 1 124.5 us, 2 121.9, 4 120.8)
 constexpr int FEW_WARPS = 4, FEW_THREADS = 32 * FEW_WARPS + 32;
 template <int D, int NT>
 struct Few {
     static constexpr int STAGE = 2 * BLOCK * D;                          // bytes: codes of keys and values, or the tail's of one of them
-    static constexpr int STAGES = (NT == 1 ? 5 : 4) * 128 / D;
+    static constexpr int CTAS = D == 64 && NT == 1 ? 3 : 2;              // to an SM, as registers allow (D = 64, 40 sequences: two 22.7 us, three 20.8)
+    static constexpr int STAGES = CTAS == 3 ? 6 : (NT == 1 ? 5 : 4) * 128 / D;
     static constexpr int TILE = 8 * NT;
     static constexpr size_t SMEM = 1024 + (size_t)STAGES * STAGE + (size_t)FEW_WARPS * TILE * D * 4;
 };
@@ -326,7 +327,7 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi)
 }
 
 template <int D, int NT>
-__global__ void __launch_bounds__(FEW_THREADS, 2)
+__global__ void __launch_bounds__(FEW_THREADS, Few<D, NT>::CTAS)
 few_kernel(const __grid_constant__ AttnArgs a)
 {
     using F = Few<D, NT>;
@@ -724,6 +725,49 @@ merge_kernel(const __grid_constant__ AttnArgs a, int tile)
     const int group = a.num_heads / a.c.kv_heads, row = w.row0 + r;
     __half* dst = a.out + (size_t)(w.row + row / group) * a.ldo + (w.head * group + row % group) * D + lane * 4;
     *reinterpret_cast<uint2*>(dst) = make_uint2(pack_f16(v.x * n, v.y * n), pack_f16(v.z * n, v.w * n));
+}
+
+// The same for tiles of PROMPT_ROWS rows, which lie in the workspace by columns, [D / 4][rows] of four, as the kernel before has them: neighbouring
+// threads take neighbouring rows, and 16 columns each.
+constexpr int PROMPT_ROWS = 256, MERGE_ROWS = 32;
+template <int D>
+__global__ void __launch_bounds__(MERGE_ROWS * D / 16)
+merge_columns_kernel(const __grid_constant__ AttnArgs a)
+{
+    pdl_launch_dependents();
+    pdl_wait_prior_grids();
+    const Join w = a.joins[blockIdx.x];
+    const int r = blockIdx.y * MERGE_ROWS + threadIdx.x % MERGE_ROWS, c0 = threadIdx.x / MERGE_ROWS * 4;         // columns 4 c0 ... 4 c0 + 15
+    if (w.parts == 0 || r >= w.rows) return;
+    const size_t each = partial_floats(PROMPT_ROWS, D);
+    const float* base = a.partial + (2 * (size_t)blockIdx.x + 1) * each;         // part j > 0: the first of CTA x + j
+    float4 v[4];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) v[c] = make_float4(0.f, 0.f, 0.f, 0.f);
+    float top = -INFINITY, l = 0.0f;
+#pragma unroll 2
+    for (int j = 0; j < w.parts; ++j) {
+        const float* p = j == 0 ? base : base + (2 * (size_t)j - 1) * each;
+        float4 x[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) x[c] = reinterpret_cast<const float4*>(p)[(c0 + c) * PROMPT_ROWS + r];
+        const float m = p[PROMPT_ROWS * D + r], n = p[PROMPT_ROWS * (D + 1) + r];
+        const float now = fmaxf(top, m), ref = now == -INFINITY ? 0.0f : now, f = ex2(top - ref), g = ex2(m - ref);
+        top = now;
+        l = fmaf(n, g, l * f);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            v[c].x = fmaf(x[c].x, g, v[c].x * f); v[c].y = fmaf(x[c].y, g, v[c].y * f);
+            v[c].z = fmaf(x[c].z, g, v[c].z * f); v[c].w = fmaf(x[c].w, g, v[c].w * f);
+        }
+    }
+    const float n = 1.0f / l;
+    const int group = a.num_heads / a.c.kv_heads, row = w.row0 + r;
+    uint4* dst = reinterpret_cast<uint4*>(a.out + (size_t)(w.row + row / group) * a.ldo + (w.head * group + row % group) * D + c0 * 4);
+#pragma unroll
+    for (int c = 0; c < 4; c += 2)
+        dst[c / 2] = make_uint4(pack_f16(v[c].x * n, v[c].y * n), pack_f16(v[c].z * n, v[c].w * n), pack_f16(v[c + 1].x * n, v[c + 1].y * n),
+                                pack_f16(v[c + 1].z * n, v[c + 1].w * n));
 }
 
 }  // namespace cache8

@@ -19,7 +19,7 @@
 namespace twm {
 namespace cache8 {
 
-constexpr int PROMPT_ROWS = 256, PROMPT_THREADS = 448;
+constexpr int PROMPT_THREADS = 448;
 constexpr int PROMPT_EXTRA = 8;                                          // a tile's own time, in units
 template <int D>
 struct Prompt {
@@ -184,6 +184,13 @@ prompt_kernel(const __grid_constant__ AttnArgs a)
         do {
             const int length = w.sp.pos + w.sp.n, held = length / BLOCK;
             const size_t at = (size_t)w.seq * a.c.kv_heads + w.head;
+            if (i > 0)                                    // these warps are some units ahead: the tile's queries towards L2
+                for (int j = me; j < min(PROMPT_ROWS, w.sp.n * deal.group - w.t * PROMPT_ROWS); j += 128) {
+                    const int r = w.t * PROMPT_ROWS + j, token = r / deal.group;
+                    const __half* q = a.q + (size_t)(w.sp.row + token) * a.ldq + (w.head * deal.group + r - token * deal.group) * D;
+                    l2_prefetch(q);
+                    if (D == 128) l2_prefetch(q + 64);
+                }
             for (int u = w.u0; u < w.u0 + w.n; ++u, ++i) {
                 const int slot = i % P::UNITS;
                 if (i >= P::UNITS) tc::wait_uniform(&unit_empty[slot], (uint32_t)(i / P::UNITS - 1) & 1u, abort_flag);
@@ -227,6 +234,7 @@ prompt_kernel(const __grid_constant__ AttnArgs a)
         const int x = warp >> 2, row = (warp & 3) * 32 + lane;
         const uint32_t lane_tmem = tmem + x * P::HALF + ((uint32_t)((warp & 3) * 32) << 16), lane_o = lane_tmem + P::OUT;
         const float base = a.scale * LOG2E;
+        const bool wide = ((reinterpret_cast<uintptr_t>(a.out) | (uintptr_t)(a.ldo * 2)) & 31) == 0;
         int n = 0, tile = -1;                             // units of this half; the tile's number
         // The queries of a tile to shared memory: that of the next one while the last products of this one run (its scores are all done).
         struct Mine { int all, r, token, head; bool live; } now;
@@ -239,22 +247,24 @@ prompt_kernel(const __grid_constant__ AttnArgs a)
             v.head = w.head * deal.group + (row0 + v.r) % deal.group;
             v.live = x * 128 + row < v.all;
             if (x * 128 < v.all) {
-                // a warp's 32 rows, neighbouring lanes along a row; all loads ahead of the first store
+                // a warp's 32 rows, neighbouring lanes along a row; half of the loads at a time ahead of their stores
                 constexpr int PER = D / 8, AT_ONCE = 32 / PER;
                 const long long mine = (long long)(w.sp.row + v.token) * a.ldq + v.head * D;
-                uint4 q[PER];
 #pragma unroll
-                for (int c = 0; c < PER; ++c) {
-                    const int from = c * AT_ONCE + lane / PER;
-                    const long long place = __shfl_sync(0xffffffffu, mine, from);
-                    q[c] = __ldg(reinterpret_cast<const uint4*>(a.q + place) + lane % PER);
-                }
+                for (int half = 0; half < 2; ++half) {
+                    uint4 q[PER / 2];
 #pragma unroll
-                for (int c = 0; c < PER; ++c) {
-                    const int from = (warp & 3) * 32 + c * AT_ONCE + lane / PER, chunk = lane % PER;
-                    const bool there = x * 128 + from < v.all;
-                    *reinterpret_cast<uint4*>(qs + x * P::BOXES * P::QBOX + (chunk >> 3) * P::QBOX + from * 128 + (((chunk & 7) ^ (from & 7)) << 4)) =
-                        there ? q[c] : make_uint4(0, 0, 0, 0);
+                    for (int c = 0; c < PER / 2; ++c) {
+                        const long long place = __shfl_sync(0xffffffffu, mine, (half * (PER / 2) + c) * AT_ONCE + lane / PER);
+                        q[c] = __ldg(reinterpret_cast<const uint4*>(a.q + place) + lane % PER);
+                    }
+#pragma unroll
+                    for (int c = 0; c < PER / 2; ++c) {
+                        const int from = (warp & 3) * 32 + (half * (PER / 2) + c) * AT_ONCE + lane / PER, chunk = lane % PER;
+                        const bool there = x * 128 + from < v.all;
+                        *reinterpret_cast<uint4*>(qs + x * P::BOXES * P::QBOX + (chunk >> 3) * P::QBOX + from * 128 + (((chunk & 7) ^ (from & 7)) << 4)) =
+                            there ? q[c] : make_uint4(0, 0, 0, 0);
+                    }
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             }
@@ -380,12 +390,17 @@ prompt_kernel(const __grid_constant__ AttnArgs a)
                     uint32_t h[8];
 #pragma unroll
                     for (int e = 0; e < 8; ++e) h[e] = pack_f16(__uint_as_float(o[2 * e]) * inv_l, __uint_as_float(o[2 * e + 1]) * inv_l);
-                    uint4* dst = reinterpret_cast<uint4*>(out + c);
-                    dst[0] = make_uint4(h[0], h[1], h[2], h[3]);
-                    dst[1] = make_uint4(h[4], h[5], h[6], h[7]);
+                    if (wide) {                           // a sector at once
+                        asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(out + c), "r"(h[0]), "r"(h[1]), "r"(h[2]), "r"(h[3]), "r"(h[4]),
+                                     "r"(h[5]), "r"(h[6]), "r"(h[7]) : "memory");
+                    } else {
+                        uint4* dst = reinterpret_cast<uint4*>(out + c);
+                        dst[0] = make_uint4(h[0], h[1], h[2], h[3]);
+                        dst[1] = make_uint4(h[4], h[5], h[6], h[7]);
+                    }
                 } else {
 #pragma unroll
-                    for (int e = 0; e < 16; e += 4) *reinterpret_cast<uint4*>(part + r * D + c + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                    for (int e = 0; e < 16; e += 4) reinterpret_cast<uint4*>(part)[(c + e) / 4 * PROMPT_ROWS + r] = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
                 }
             }
             if (live && ok && !alone) { part[PROMPT_ROWS * D + r] = m; part[PROMPT_ROWS * (D + 1) + r] = l; }

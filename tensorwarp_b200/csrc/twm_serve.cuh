@@ -33,11 +33,11 @@ twm::cache8::Cache device_cache(const twm_cache8* c)
 
 // How attention is launched: the rows of a tile and the CTAs of the grid, whatever the lengths (which are on the device).
 struct AttnPlan { int tile, ctas; };
-AttnPlan plan_attention(int group, int max_rows)
+AttnPlan plan_attention(int group, int max_rows, int head_dim)
 {
     const long rows = (long)max_rows * group;
-    if (rows <= 8) return {8, 2 * kDefaultSms};
-    if (rows <= 16) return {16, 2 * kDefaultSms};
+    if (rows <= 8) return {8, kDefaultSms * (head_dim == 64 ? twm::cache8::Few<64, 1>::CTAS : twm::cache8::Few<128, 1>::CTAS)};
+    if (rows <= 16) return {16, kDefaultSms * (head_dim == 64 ? twm::cache8::Few<64, 2>::CTAS : twm::cache8::Few<128, 2>::CTAS)};
     return {twm::cache8::PROMPT_ROWS, kDefaultSms};
 }
 
@@ -101,10 +101,13 @@ twm_status launch_prompt(const twm::cache8::AttnArgs& a, const AttnPlan& p, int 
 template <int D>
 twm_status launch_merge(const twm::cache8::AttnArgs& a, const AttnPlan& p, int flags, void* stream)
 {
-    const bool many = p.tile == twm::cache8::PROMPT_ROWS;
-    const int rows = twm::cache8::MERGE_THREADS / (D / 4) / (many ? 1 : 8);
-    return launch_op("twm_cache8_attention(merge)", many ? twm::cache8::merge_kernel<D, 1> : twm::cache8::merge_kernel<D, 8>,
-                     dim3(p.ctas, (p.tile + rows - 1) / rows), dim3(twm::cache8::MERGE_THREADS), 0, flags | TWM_FLAG_PDL, stream, a, p.tile);
+    flags |= TWM_FLAG_PDL;
+    if (p.tile == twm::cache8::PROMPT_ROWS)
+        return launch_op("twm_cache8_attention(merge)", twm::cache8::merge_columns_kernel<D>, dim3(p.ctas, p.tile / twm::cache8::MERGE_ROWS),
+                         dim3(twm::cache8::MERGE_ROWS * D / 16), 0, flags, stream, a);
+    const int rows = twm::cache8::MERGE_THREADS / (D / 4) / 8;
+    return launch_op("twm_cache8_attention(merge)", twm::cache8::merge_kernel<D, 8>, dim3(p.ctas, (p.tile + rows - 1) / rows),
+                     dim3(twm::cache8::MERGE_THREADS), 0, flags, stream, a, p.tile);
 }
 
 // The CTAs of a row: slices of at most 24000 logits, of which two fit an SM, and where there are few rows as many more of them as the SMs take at
@@ -149,7 +152,7 @@ twm_status twm_cache8_append(const twm_cache8* cache, void* q_out, long ldq, con
 size_t twm_cache8_attention_bytes(const twm_cache8* c, int num_heads, int max_rows)
 {
     if (!c || num_heads < 1 || max_rows < 1 || c->kv_heads < 1 || num_heads % c->kv_heads || (c->head_dim != 64 && c->head_dim != 128)) return 0;
-    const AttnPlan p = plan_attention(num_heads / c->kv_heads, max_rows);
+    const AttnPlan p = plan_attention(num_heads / c->kv_heads, max_rows, c->head_dim);
     return (size_t)p.ctas * (sizeof(twm::cache8::Join) + 2 * twm::cache8::partial_floats(p.tile, c->head_dim) * sizeof(float));
 }
 
@@ -165,7 +168,7 @@ twm_status twm_cache8_attention(const twm_cache8* cache, void* out, long ldo, co
     if (off16(out) || off16(q) || off16(workspace) || (ldo & 7) || (ldq & 7)) return TWM_EALIGN;
     if (workspace_bytes < twm_cache8_attention_bytes(cache, num_heads, max_rows)) return TWM_EWORKSPACE;
     if ((st = ensure_device(nullptr)) != TWM_OK) return st;
-    const AttnPlan p = plan_attention(num_heads / cache->kv_heads, max_rows);
+    const AttnPlan p = plan_attention(num_heads / cache->kv_heads, max_rows, D);
     twm::cache8::AttnArgs a = {device_cache(cache), {row_start, start, rows, max_rows}, (__half*)out, (const __half*)q, ldo, ldq, num_heads,
                                window ? window : INT_MAX, scale, (twm::cache8::Join*)workspace,
                                (float*)((twm::cache8::Join*)workspace + p.ctas), {}, {}};
