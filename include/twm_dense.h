@@ -31,6 +31,7 @@
 #define TWM_DENSE_H
 
 #include "twmarlin.h"
+#include "twm_serve.h"
 
 #ifdef __cplusplus
 extern "C" {
@@ -159,6 +160,10 @@ twm_status twm_dense_set_step(const twm_dense_buffers* b, int first_pos, int slo
 size_t twm_dense_argmax_scratch_bytes(void);
 twm_status twm_dense_argmax_advance(const twm_dense_buffers* b, int vocab, int row, int* history,
                                     int history_capacity, void* scratch, size_t scratch_bytes, int flags, void* stream);
+
+/* twm_sample (twm_serve.h) of this library; with buffers->meta, meta + 2 and meta + 3 as pos, len and step it takes the place of
+ * twm_dense_argmax_advance. */
+twm_status twm_dense_sample(const twm_sample_args* args, int flags, void* stream);
 
 /* ---- single operations, as the step uses them ---- */
 enum { TWM_EPI_STORE = 0, TWM_EPI_STORE_F32 = 1, TWM_EPI_GELU_GLU = 2, TWM_EPI_RELU2 = 3 };

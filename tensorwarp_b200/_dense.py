@@ -4,7 +4,7 @@ from __future__ import annotations
 import ctypes as C
 
 from .build import build_library
-from ._lib import TWM_FLAG_PDL, TWM_OK  # noqa: F401
+from ._lib import TWM_F32, TWM_FLAG_PDL, TWM_OK, SampleArgs  # noqa: F401
 
 TWM_DENSE_F32, TWM_DENSE_BF16 = 0, 2
 MIX_SIGMOID, MIX_LATENT, MIX_GLA = 0, 1, 2
@@ -52,6 +52,7 @@ SIGNATURES = {
     "twm_dense_set_step": (C.c_int, [_B, C.c_int, C.c_int, C.c_int, _P]),
     "twm_dense_argmax_scratch_bytes": (C.c_size_t, []),
     "twm_dense_argmax_advance": (C.c_int, [_B, C.c_int, C.c_int, _P, C.c_int, _P, C.c_size_t, C.c_int, _P]),
+    "twm_dense_sample": (C.c_int, [C.POINTER(SampleArgs), C.c_int, _P]),
     "twm_dense_gemm": (C.c_int, [C.c_int, _P, C.c_int, _P, C.c_int, _P, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int,
                                  C.c_int, _P]),
     "twm_dense_route": (C.c_int, [_P, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, _P, _P, C.c_int, _P]),

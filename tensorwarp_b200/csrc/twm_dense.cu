@@ -24,6 +24,7 @@
 #include "twm_dense_tc2.cuh"
 #include "twm_dense_experts_tc.cuh"
 #include "twm_dense_tcs.cuh"
+#include "twm_sample.cuh"
 
 namespace {
 
@@ -1250,6 +1251,21 @@ twm_status twm_dense_argmax_advance(const twm_dense_buffers* b, int vocab, int r
                (const float*)b->logits + (size_t)row * vocab, vocab));
     return launch("argmax(final)", ops::argmax_final_kernel, dim3(1), 256, 0, flags, stream, 0, b->tokens, history, history_capacity,
                   b->meta, b->meta + 2, b->meta + 3, (const float*)pval, (const int*)pidx, kArgmaxParts, vocab);
+}
+
+twm_status twm_dense_sample(const twm_sample_args* args, int flags, void* stream)
+{
+    const twm_status st = sample::check(args);
+    if (st != TWM_OK) {
+        invalid("sample");
+        return st;
+    }
+    int sms = 0;
+    TRY(device(&sms));
+    const cudaError_t e = sample::launch(*args, sms, flags, stream);
+    if (e != cudaSuccess) return fail("sample", e);
+    ++t_launches;
+    return TWM_OK;
 }
 
 twm_status twm_dense_gemm(int dtype, const void* a, int lda, const void* w, int ldw, void* c, int ldc, int M, int N, int K,

@@ -13,6 +13,8 @@
 // Bound by memory for many rows, by the chain of cluster barriers for one.
 #pragma once
 
+#include <algorithm>
+
 #include <cuda_bf16.h>
 
 #include "../../include/twm_serve.h"
@@ -127,13 +129,13 @@ __device__ __forceinline__ Scan scan(Shared& sh, uint32_t c, double m)
 
 template <typename T>
 __global__ void __launch_bounds__(THREADS, 2)
-sample_kernel(const __grid_constant__ twm_sample_args a, int slice)
+sample_kernel(const __grid_constant__ twm_sample_args a, int slice, int ctas)
 {
     extern __shared__ __align__(16) float vals[];
     __shared__ Shared sh;
     cluster_started();
     pdl_launch_dependents();
-    const int row = blockIdx.x, rank = blockIdx.y, ctas = gridDim.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int row = blockIdx.x / ctas, rank = blockIdx.x % ctas, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int n = a.vocab, n0 = min(n, rank * slice), ns = min(n - n0, slice);
     for (int i = tid; i < BINS; i += THREADS) sh.count[i] = sh.delta[i] = 0;
     if (tid < 2) sh.list_n[tid] = 0;
@@ -473,6 +475,52 @@ sample_kernel(const __grid_constant__ twm_sample_args a, int slice)
             a.len[0] += 1;
         }
     }
+}
+
+// ---------------------------------------------------------------------------------------------------------- launch --
+
+inline twm_status check(const twm_sample_args* a)
+{
+    if (!a || !a->logits || !a->random || !a->tokens || a->rows < 1 || a->rows > (1 << 26) || a->vocab < 1 || a->vocab > (1 << 20) || a->ld < a->vocab) return TWM_EINVAL;
+    if (a->dtype != TWM_F32 && a->dtype != TWM_F16 && a->dtype != TWM_BF16) return TWM_EINVAL;
+    if (a->step && (a->rows != 1 || a->random_count < 1 || !a->pos || !a->len || (a->history && a->history_capacity < 1))) return TWM_EINVAL;
+    return reinterpret_cast<uintptr_t>(a->logits) & (a->dtype == TWM_F32 ? 3 : 1) ? TWM_EALIGN : TWM_OK;
+}
+
+// The CTAs of a row: slices of at most 24000 logits, of which two fit an SM, and where there are few rows as many more of them as `sms` SMs take at
+// once, down to 2048 logits each (64 rows of 32768, two or four CTAs: 28.1 and 25.5 us).
+template <typename T>
+cudaError_t launch_as(const twm_sample_args& a, int sms, int flags, cudaStream_t stream)
+{
+    const int most = 2 * sms / std::min(a.rows, 2 * sms);
+    int ctas = 1;
+    while (ctas < MAX_CTAS && (a.vocab > 24000L * ctas || (2 * ctas <= most && a.vocab > 2048L * ctas))) ctas *= 2;
+    const int slice = (int)((((long)a.vocab + ctas - 1) / ctas + 15) / 16 * 16);
+    static_assert(MAX_SLICE * 4 + sizeof(Shared) + 1024 < 227 * 1024, "shared memory of a CTA");
+    auto* kernel = sample_kernel<T>;
+    cudaError_t e;
+    // both belong to the function and only ever get these values
+    if ((e = cudaFuncSetAttribute((const void*)kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, MAX_SLICE * 4)) != cudaSuccess) return e;
+    if ((e = cudaFuncSetAttribute((const void*)kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1)) != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)a.rows * ctas);
+    cfg.blockDim = dim3(THREADS);
+    cfg.dynamicSmemBytes = 4 * (size_t)std::min(slice, MAX_SLICE);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = ctas;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = flags & TWM_FLAG_PDL ? 2 : 1;
+    return cudaLaunchKernelEx(&cfg, kernel, a, slice, ctas);
+}
+inline cudaError_t launch(const twm_sample_args& a, int sms, int flags, void* stream)
+{
+    if (a.dtype == TWM_F32) return launch_as<float>(a, sms, flags, (cudaStream_t)stream);
+    return a.dtype == TWM_F16 ? launch_as<__half>(a, sms, flags, (cudaStream_t)stream) : launch_as<__nv_bfloat16>(a, sms, flags, (cudaStream_t)stream);
 }
 
 }  // namespace sample

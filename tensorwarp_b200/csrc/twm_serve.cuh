@@ -57,7 +57,7 @@ bool make_codes_map(CUtensorMap* map, const twm_cache8* c, void* codes)
 
 // Lets a kernel take more than 48 KB of shared memory on the current device.  The limit belongs to the function: it is set once a device, to what
 // every launch of it asks for.
-twm_status allow_shared(const char* name, const void* kernel, size_t bytes, bool wide_clusters = false)
+twm_status allow_shared(const char* name, const void* kernel, size_t bytes)
 {
     static std::mutex mutex;
     static std::vector<std::pair<const void*, int>> done;
@@ -68,7 +68,6 @@ twm_status allow_shared(const char* name, const void* kernel, size_t bytes, bool
         for (const auto& x : done)
             if (x.first == kernel && x.second == dev) return TWM_OK;
         e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
-        if (e == cudaSuccess && wide_clusters) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
         if (e == cudaSuccess) done.emplace_back(kernel, dev);
     }
     if (e == cudaSuccess) return TWM_OK;
@@ -108,23 +107,6 @@ twm_status launch_merge(const twm::cache8::AttnArgs& a, const AttnPlan& p, int f
     const int rows = twm::cache8::MERGE_THREADS / (D / 4) / 8;
     return launch_op("twm_cache8_attention(merge)", twm::cache8::merge_kernel<D, 8>, dim3(p.ctas, (p.tile + rows - 1) / rows),
                      dim3(twm::cache8::MERGE_THREADS), 0, flags, stream, a, p.tile);
-}
-
-// The CTAs of a row: slices of at most 24000 logits, of which two fit an SM, and where there are few rows as many more of them as the SMs take at
-// once, down to 2048 logits each (64 rows of 32768, two or four CTAs: 28.1 and MEASURED us).
-template <typename T>
-twm_status launch_sample(const twm_sample_args& a, int flags, void* stream)
-{
-    const int most = 2 * kDefaultSms / std::min(a.rows, 2 * kDefaultSms);
-    int ctas = 1;
-    while (ctas < 16 && (a.vocab > 24000L * ctas || (2 * ctas <= most && a.vocab > 2048L * ctas))) ctas *= 2;
-    const int slice = (int)((((long)a.vocab + ctas - 1) / ctas + 15) / 16 * 16);
-    auto* kernel = twm::sample::sample_kernel<T>;
-    static_assert(twm::sample::MAX_SLICE * 4 + sizeof(twm::sample::Shared) + 1024 < 227 * 1024, "shared memory of a CTA");
-    const twm_status st = allow_shared("twm_sample", (const void*)kernel, twm::sample::MAX_SLICE * 4, true);
-    if (st != TWM_OK) return st;
-    return launch_cluster("twm_sample", kernel, dim3(a.rows, ctas), dim3(twm::sample::THREADS), 4 * (size_t)std::min(slice, twm::sample::MAX_SLICE), flags, ctas,
-                          stream, a, slice);
 }
 
 }  // namespace
@@ -186,17 +168,12 @@ twm_status twm_cache8_attention(const twm_cache8* cache, void* out, long ldo, co
 
 twm_status twm_sample(const twm_sample_args* args, int flags, void* stream)
 {
-    if (!args || !args->logits || !args->random || !args->tokens || args->rows < 1 || args->vocab < 1 || args->vocab > (1 << 20) ||
-        args->ld < args->vocab)
-        return TWM_EINVAL;
-    if (args->dtype != TWM_F32 && args->dtype != TWM_F16 && args->dtype != TWM_BF16) return TWM_EINVAL;
-    if (args->step && (args->rows != 1 || args->random_count < 1 || !args->pos || !args->len || (args->history && args->history_capacity < 1)))
-        return TWM_EINVAL;
-    if (reinterpret_cast<uintptr_t>(args->logits) & (args->dtype == TWM_F32 ? 3 : 1)) return TWM_EALIGN;
-    const twm_status st = ensure_device(nullptr);
-    if (st != TWM_OK) return st;
-    if (args->dtype == TWM_F32) return launch_sample<float>(*args, flags, stream);
-    return args->dtype == TWM_F16 ? launch_sample<__half>(*args, flags, stream) : launch_sample<__nv_bfloat16>(*args, flags, stream);
+    twm_status st = twm::sample::check(args);
+    if (st != TWM_OK || (st = ensure_device(nullptr)) != TWM_OK) return st;
+    const cudaError_t e = twm::sample::launch(*args, kDefaultSms, flags, stream);
+    if (e == cudaSuccess) return TWM_OK;
+    set_error("twm_sample", e);
+    return TWM_ELAUNCH;
 }
 
 }  // extern "C"

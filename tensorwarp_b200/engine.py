@@ -3,7 +3,7 @@
 An engine keeps the state of several sequences and runs one sequence's step at a time: a portion of
 its prompt of any size, or one decoded token.  Prompt portions are enqueued by one native call; a
 decoded token replays a captured CUDA graph whose position, slot and token live in device memory,
-so one graph serves every sequence.  Sampling stays on the device (greedy).
+so one graph serves every sequence.  Tokens are chosen on the device, greedily or by drawing from given random numbers.
 """
 from __future__ import annotations
 
@@ -14,6 +14,7 @@ import torch
 
 from . import _dense
 from ._dense import check
+from .sampling import LoopState, SamplingParams
 from .state import SequenceState
 
 
@@ -31,6 +32,9 @@ class StepEngine(Protocol):
         ...
     def greedy(self, seq: int, tokens: Sequence[int], count: int) -> List[int]:
         """Run the sequence's next tokens, then generate `count` tokens; the last one is not yet run."""
+        ...
+    def sample(self, seq: int, tokens: Sequence[int], count: int, params: SamplingParams, generator: torch.Generator) -> List[int]:
+        """As greedy, with tokens drawn by `params` from the generator's next `count` random numbers."""
         ...
 
 
@@ -99,6 +103,7 @@ class DenseEngine:
             setattr(b, name, t.data_ptr())
         self._b = b
         self.history = zeros(max(self.capacity, 1), dtype=i32)
+        self._loop = LoopState(self.capacity, dev)
         self._argmax_scratch = zeros(_dense.lib().twm_dense_argmax_scratch_bytes(), dtype=torch.uint8)
 
     @property
@@ -183,15 +188,23 @@ class DenseEngine:
 
     # ------------------------------------------------------------------ decode --
     def _enqueue_decode(self, kind: str) -> None:
-        """One decoded token on the engine's stream.  kind: "silent" (state only), "logits", "greedy" (logits, arg-max,
-        and position and token advanced on the device)."""
+        """One decoded token on the engine's stream.  kind: "silent" (state only), "logits", "greedy" and "sample" (logits, arg-max
+        or a token drawn, and position and token advanced on the device)."""
         lib, s = _dense.lib(), self.stream.cuda_stream
         check(lib.twm_dense_decode(C.byref(self._desc), C.byref(self._b), 0 if kind == "silent" else 1, self.flags, s),
               "twm_dense_decode")
         self.launches_per_step = lib.twm_dense_launches()
+        if kind in ("greedy", "sample"):
+            self._choose(kind)
+            self.launches_per_step = lib.twm_dense_launches()
+
+    def _choose(self, kind: str) -> None:
         if kind == "greedy":
             self._argmax()
-            self.launches_per_step = lib.twm_dense_launches()
+            return
+        meta = self._b.meta                                         # position, slot, position + 1, step
+        check(_dense.lib().twm_dense_sample(self._loop.args(self.logits, self.vocab, self._b.tokens, meta + 12, self.history, meta, meta + 8), self.flags,
+                                            self.stream.cuda_stream), "twm_dense_sample")
 
     def _argmax(self) -> None:
         check(_dense.lib().twm_dense_argmax_advance(C.byref(self._b), self.vocab, 0, self.history.data_ptr(), self.history.numel(),
@@ -216,6 +229,15 @@ class DenseEngine:
                 self._enqueue_decode(kind)
 
     def greedy(self, seq: int, tokens: Sequence[int], count: int) -> List[int]:
+        return self._generate("greedy", seq, tokens, count)
+
+    def sample(self, seq: int, tokens: Sequence[int], count: int, params: SamplingParams, generator: torch.Generator) -> List[int]:
+        random = torch.rand(max(count, 0), generator=generator)
+        with torch.cuda.stream(self.stream):
+            self._loop.set(params, random[:self.capacity])          # more than that are refused below
+        return self._generate("sample", seq, tokens, count)
+
+    def _generate(self, kind: str, seq: int, tokens: Sequence[int], count: int) -> List[int]:
         if count < 1:
             return []
         tokens = list(tokens)
@@ -228,13 +250,13 @@ class DenseEngine:
             self._buf["meta"][3:4].zero_()                          # the step counter indexes the history
             if len(tokens) > 1:
                 self.step(seq, tokens, [len(tokens) - 1])
-                self._set_step(first + len(tokens) - 1, seq)        # the arg-max advances the position by one
-                self._argmax()
+                self._set_step(first + len(tokens) - 1, seq)        # the choice advances the position by one
+                self._choose(kind)
                 replays -= 1
             else:
                 self._set_step(first, seq, tokens[0])
         for _ in range(replays):
-            self._decode("greedy")
+            self._decode(kind)
         if len(tokens) > 1:
             self.state.advance(seq, replays)
         else:

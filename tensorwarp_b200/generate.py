@@ -18,8 +18,10 @@ from typing import List, Optional
 import torch
 
 from . import _lib
+from . import cache8 as c8
 from . import quantize as q
 from ._lib import check
+from .sampling import LoopState, SamplingParams
 
 
 @dataclass
@@ -111,7 +113,7 @@ class Q4DecodeBuffers:
     """Every buffer one decode step touches, allocated once (Q4DecodeBuffers::allocate,
     generate.rs:1382-1416)."""
 
-    def __init__(self, cfg: TransformerConfig, device):
+    def __init__(self, cfg: TransformerConfig, device, kv_cache: str = "f16"):
         f16, f32, i32 = torch.float16, torch.float32, torch.int32
         dev = device
         self.x = torch.zeros(cfg.hidden, dtype=f32, device=dev)                  # residual stream
@@ -126,11 +128,18 @@ class Q4DecodeBuffers:
         self.cache_len = torch.zeros(1, dtype=i32, device=dev)                    # cache_len_buf (generate.rs:1415)
         self.step = torch.zeros(1, dtype=i32, device=dev)
         self.history = torch.zeros(cfg.max_seq, dtype=i32, device=dev)
-        self.k_cache = [torch.zeros((cfg.max_seq, cfg.kv_dim), dtype=f16, device=dev) for _ in range(cfg.layers)]
-        self.v_cache = [torch.zeros((cfg.max_seq, cfg.kv_dim), dtype=f16, device=dev) for _ in range(cfg.layers)]
         lib = _lib.lib()
-        self.attn_scratch = torch.zeros(lib.twm_attn_scratch_bytes(1, cfg.num_heads, cfg.head_dim, cfg.max_seq),
-                                        dtype=torch.uint8, device=dev)
+        if kv_cache == "f16":
+            self.k_cache = [torch.zeros((cfg.max_seq, cfg.kv_dim), dtype=f16, device=dev) for _ in range(cfg.layers)]
+            self.v_cache = [torch.zeros((cfg.max_seq, cfg.kv_dim), dtype=f16, device=dev) for _ in range(cfg.layers)]
+            self.attn_scratch = torch.zeros(lib.twm_attn_scratch_bytes(1, cfg.num_heads, cfg.head_dim, cfg.max_seq),
+                                            dtype=torch.uint8, device=dev)
+        else:
+            self.cache8 = [c8.Cache8.empty(1, cfg.max_seq, cfg.num_kv_heads, cfg.head_dim, dev) for _ in range(cfg.layers)]
+            self.rope = c8.rope_table(self.cache8[0].capacity if cfg.layers else 0, cfg.head_dim, cfg.rope_theta, dev)
+            self.query = torch.zeros((1, cfg.q_dim), dtype=f16, device=dev)
+            self.attn_workspace = c8.Workspace.for_cache(self.cache8[0], cfg.num_heads) if cfg.layers else None
+        self.loop = LoopState(cfg.max_seq, dev)
         self.argmax_scratch = torch.zeros(lib.twm_argmax_scratch_bytes(), dtype=torch.uint8, device=dev)
         shapes = [(1, cfg.q_dim + 2 * cfg.kv_dim, cfg.hidden, cfg.group_size), (1, cfg.hidden, cfg.q_dim, cfg.group_size),
                   (1, 2 * cfg.ffn, cfg.hidden, cfg.group_size), (1, cfg.hidden, cfg.ffn, cfg.group_size)]
@@ -140,17 +149,23 @@ class Q4DecodeBuffers:
 class QuantizedGenerationEngine:
     """Decode engine on TW-Marlin weights (generate.rs:1191-2547, Q4 + marlin + graph path)."""
 
-    def __init__(self, model: Q4Model, use_pdl: bool = True, q4_lm_head: bool = False):
-        self.model = model
+    def __init__(self, model: Q4Model, use_pdl: bool = True, q4_lm_head: bool = False, kv_cache: str = "f16"):
+        """kv_cache: "f16", or "e4m3" for keys and values held in 8 bits (half the memory; ``cache8``)."""
+        if kv_cache not in ("f16", "e4m3"):
+            raise _lib.TwmError(_lib.TWM_EINVAL, f"QuantizedGenerationEngine: kv_cache {kv_cache!r} is neither 'f16' nor 'e4m3'")
+        if kv_cache == "e4m3" and model.cfg.head_dim not in (64, 128):
+            raise _lib.TwmError(_lib.TWM_EINVAL, "QuantizedGenerationEngine: a cache held in 8 bits wants heads of 64 or 128")
+        self.model, self.kv_cache = model, kv_cache
         # the reference's graph path keeps the LM head outside the graph in FP32/FP16 (generate.rs:2530-2534)
         # and has a Q4 one as an option (forward_lm_head_tw_marlin, generate.rs:1750-1761): same here
         self.q4_lm_head = q4_lm_head
         if q4_lm_head:
             model.quantize_lm_head()
         self.cfg = model.cfg
-        self.buf = Q4DecodeBuffers(model.cfg, model.device)
+        self.buf = Q4DecodeBuffers(model.cfg, model.device, kv_cache)
         self.flags = _lib.TWM_FLAG_PDL if use_pdl else 0
         self.graph: Optional[torch.cuda.CUDAGraph] = None
+        self.sample_graph: Optional[torch.cuda.CUDAGraph] = None
         self.stream = torch.cuda.Stream(model.device)
         self.launches_per_step = 0
 
@@ -158,6 +173,15 @@ class QuantizedGenerationEngine:
     def prefill_random_kv(self, length: int, seed: int = 2) -> None:
         """KV cache holding `length` tokens of FP16 N(0,1) (the benchmark's stand-in for a prefill)."""
         gen = torch.Generator(device=self.model.device).manual_seed(seed)
+        if self.kv_cache == "e4m3":
+            kv = 2 * self.cfg.kv_dim
+            qkv = torch.zeros((length, self.cfg.q_dim + kv), dtype=torch.float16, device=self.model.device)
+            start, rows = torch.zeros(1, dtype=torch.int32, device=self.model.device), torch.tensor([0, length], dtype=torch.int32, device=self.model.device)
+            for cache in self.buf.cache8 if length else ():
+                qkv[:, self.cfg.q_dim:] = torch.randn((length, kv), generator=gen, device=self.model.device)
+                c8.append(cache, qkv, torch.empty_like(qkv[:, :self.cfg.q_dim]), start, num_heads=self.cfg.num_heads, row_start=rows, max_rows=length)
+            self.set_position(length)
+            return
         for kc, vc in zip(self.buf.k_cache, self.buf.v_cache):
             kc[:length] = torch.randn((length, self.cfg.kv_dim), generator=gen, device=self.model.device).half()
             vc[:length] = torch.randn((length, self.cfg.kv_dim), generator=gen, device=self.model.device).half()
@@ -176,7 +200,18 @@ class QuantizedGenerationEngine:
         self.buf.step.zero_()
 
     # ------------------------------------------------------------------- step --
-    def _step_ops(self, stream_ptr: int):
+    def _cache8_ops(self, cache, lw, stream_ptr: int):
+        """A layer's append to, and attention over, its cache held in 8 bits."""
+        lib, cfg, b, fl = _lib.lib(), self.cfg, self.buf, self.flags
+        append = lambda: check(lib.twm_cache8_append(  # noqa: E731
+            cache._ref, b.query.data_ptr(), cfg.q_dim, b.qkv.data_ptr(), b.qkv.numel(), lw.bqkv.data_ptr() if lw.bqkv is not None else None,
+            b.rope.data_ptr(), cfg.num_heads, 1, None, 1, b.pos.data_ptr(), fl, stream_ptr), "twm_cache8_append")
+        attend = lambda: check(lib.twm_cache8_attention(  # noqa: E731
+            cache._ref, b.attn.data_ptr(), cfg.q_dim, b.query.data_ptr(), cfg.q_dim, cfg.num_heads, 1, None, 1, b.pos.data_ptr(), cfg.head_dim ** -0.5, 0,
+            b.attn_workspace.ptr, b.attn_workspace.nbytes, fl, stream_ptr), "twm_cache8_attention")
+        return [("kv_append", 1, append), ("attention", 2, attend)]
+
+    def _step_ops(self, stream_ptr: int, sample: bool = False):
         """One decode step as an ordered list of (category, launches, enqueue) triples: the launch
         order of generate.rs:2149-2206 with the split/add passes folded into their neighbours.  The
         categories are the rows of the reference's profile table (generate.rs:2380-2396)."""
@@ -199,8 +234,9 @@ class QuantizedGenerationEngine:
             return lambda: check(lib.twm_gemm_w4a16(C.byref(args), stream_ptr), "twm_gemm_w4a16")
 
         # cos/sin of this step's position, once for all layers
-        ops.append(("rope_table", 1, lambda: check(lib.twm_rope_table(b.rope_table.data_ptr(), b.pos.data_ptr(), cfg.head_dim,
-                                                                      cfg.rope_theta, fl, stream_ptr), "twm_rope_table")))
+        if self.kv_cache == "f16":
+            ops.append(("rope_table", 1, lambda: check(lib.twm_rope_table(b.rope_table.data_ptr(), b.pos.data_ptr(), cfg.head_dim,
+                                                                          cfg.rope_theta, fl, stream_ptr), "twm_rope_table")))
         ops.append(("embedding", 1, lambda: check(lib.twm_embed(b.x.data_ptr(), self.model.embed.data_ptr(), b.token.data_ptr(),
                                                                  1, cfg.hidden, fl, stream_ptr), "twm_embed")))
         for li, lw in enumerate(self.model.layers):
@@ -209,11 +245,14 @@ class QuantizedGenerationEngine:
             ops.append(("qkv_gemm", 1, gemm(b.normed, lw.wqkv, b.qkv, cfg.q_dim + 2 * cfg.kv_dim, cfg.hidden)))
             # bias + RoPE on q and k, the KV append and the attention itself: the attention kernel takes the fused
             # QKV output (fused_bias_rope_append_device_pos + decode_attention_flash_device_len, generate.rs:2164-2178)
-            ops.append(("attention", 2, lambda li=li, lw=lw: check(lib.twm_attn_decode_rope(
-                b.attn.data_ptr(), b.qkv.data_ptr(), lw.bqkv.data_ptr() if lw.bqkv is not None else None,
-                b.rope_table.data_ptr(), b.k_cache[li].data_ptr(), b.v_cache[li].data_ptr(), 1, cfg.num_heads,
-                cfg.num_kv_heads, cfg.head_dim, b.pos.data_ptr(), b.cache_len.data_ptr(), cfg.max_seq,
-                b.attn_scratch.data_ptr(), b.attn_scratch.numel(), fl, stream_ptr), "twm_attn_decode_rope")))
+            if self.kv_cache == "f16":
+                ops.append(("attention", 2, lambda li=li, lw=lw: check(lib.twm_attn_decode_rope(
+                    b.attn.data_ptr(), b.qkv.data_ptr(), lw.bqkv.data_ptr() if lw.bqkv is not None else None,
+                    b.rope_table.data_ptr(), b.k_cache[li].data_ptr(), b.v_cache[li].data_ptr(), 1, cfg.num_heads,
+                    cfg.num_kv_heads, cfg.head_dim, b.pos.data_ptr(), b.cache_len.data_ptr(), cfg.max_seq,
+                    b.attn_scratch.data_ptr(), b.attn_scratch.numel(), fl, stream_ptr), "twm_attn_decode_rope")))
+            else:
+                ops += self._cache8_ops(b.cache8[li], lw, stream_ptr)
             ops.append(("out_gemm", 1, gemm(b.attn, lw.wo, b.x, cfg.hidden, cfg.q_dim, accumulate=True)))          # x += o(attn)
             ops.append(("ffn_rmsnorm", 1, lambda lw=lw: check(lib.twm_rmsnorm(
                 b.normed.data_ptr(), b.x.data_ptr(), lw.ffn_norm.data_ptr(), 1, cfg.hidden, cfg.eps, fl, stream_ptr), "twm_rmsnorm")))
@@ -230,19 +269,23 @@ class QuantizedGenerationEngine:
             ops.append(("lm_head", 1, lambda: check(lib.twm_lm_head(b.logits.data_ptr(), b.normed.data_ptr(),
                                                                     self.model.lm_head.data_ptr(), cfg.hidden, cfg.vocab, fl,
                                                                     stream_ptr), "twm_lm_head")))
-        ops.append(("argmax_advance", 2, lambda: check(lib.twm_argmax_advance(
-            b.token.data_ptr(), b.history.data_ptr(), b.history.numel(), b.pos.data_ptr(), b.cache_len.data_ptr(),
-            b.step.data_ptr(), b.logits.data_ptr(), cfg.vocab, b.argmax_scratch.data_ptr(), b.argmax_scratch.numel(), fl,
-            stream_ptr), "twm_argmax_advance")))
+        if sample:
+            args = b.loop.args(b.logits, cfg.vocab, b.token.data_ptr(), b.step.data_ptr(), b.history, b.pos.data_ptr(), b.cache_len.data_ptr())
+            ops.append(("sample", 1, lambda: check(lib.twm_sample(args, fl, stream_ptr), "twm_sample")))
+        else:
+            ops.append(("argmax_advance", 2, lambda: check(lib.twm_argmax_advance(
+                b.token.data_ptr(), b.history.data_ptr(), b.history.numel(), b.pos.data_ptr(), b.cache_len.data_ptr(),
+                b.step.data_ptr(), b.logits.data_ptr(), cfg.vocab, b.argmax_scratch.data_ptr(), b.argmax_scratch.numel(), fl,
+                stream_ptr), "twm_argmax_advance")))
         if len(pending) > 1:
             pending[-1].next = C.addressof(pending[0])       # the next token's first GEMM
         return ops
 
-    def forward_decode_tw_marlin_graph(self, stream_ptr: int) -> int:
-        """Enqueue one decode step (embedding .. arg-max) on the stream; returns the number of
+    def forward_decode_tw_marlin_graph(self, stream_ptr: int, sample: bool = False) -> int:
+        """Enqueue one decode step (embedding .. arg-max, or a token drawn) on the stream; returns the number of
         kernel launches (forward_decode_tw_marlin_graph, generate.rs:2124-2211)."""
         n = 0
-        for _, launches, enqueue in self._step_ops(stream_ptr):
+        for _, launches, enqueue in self._step_ops(stream_ptr, sample):
             enqueue()
             n += launches
         self.launches_per_step = n
@@ -274,7 +317,7 @@ class QuantizedGenerationEngine:
             torch.cuda.synchronize()
         per_step = {k: v / steps for k, v in acc.items()}
         total = sum(per_step.values())
-        layered = {"attn_rmsnorm", "qkv_gemm", "attention", "out_gemm", "ffn_rmsnorm", "gate_up_gemm", "down_gemm"}
+        layered = {"attn_rmsnorm", "qkv_gemm", "kv_append", "attention", "out_gemm", "ffn_rmsnorm", "gate_up_gemm", "down_gemm"}
         nl = max(len(self.model.layers), 1)
         table = {k: {"us": round(v, 1), "us_per_layer": round(v / nl, 2) if k in layered else None,
                      "pct": round(100.0 * v / total, 1)} for k, v in per_step.items()}
@@ -287,30 +330,36 @@ class QuantizedGenerationEngine:
         with torch.cuda.stream(self.stream):
             self.forward_decode_tw_marlin_graph(self.stream.cuda_stream)
 
-    def capture(self) -> None:
-        """Capture one step (GraphCapture::record_with_device, cuda_graph.rs:85-111).  One eager
+    def capture(self, sample: bool = False) -> None:
+        """Capture one step, or the one that samples (GraphCapture::record_with_device, cuda_graph.rs:85-111).  One eager
         step runs first (it initialises per-device state), then its effects on the position
         buffers and the cache are undone, as the reference does (generate.rs:2491-2500)."""
         b = self.buf
         saved = (b.pos.clone(), b.cache_len.clone(), b.step.clone(), b.token.clone())
         with torch.cuda.stream(self.stream):
-            self.forward_decode_tw_marlin_graph(self.stream.cuda_stream)
+            self.forward_decode_tw_marlin_graph(self.stream.cuda_stream, sample)
             torch.cuda.synchronize()
             b.pos.copy_(saved[0]); b.cache_len.copy_(saved[1]); b.step.copy_(saved[2]); b.token.copy_(saved[3])
             torch.cuda.synchronize()
-            self.graph = torch.cuda.CUDAGraph()
-            with torch.cuda.graph(self.graph, stream=self.stream):
-                self.forward_decode_tw_marlin_graph(self.stream.cuda_stream)
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=self.stream):
+                self.forward_decode_tw_marlin_graph(self.stream.cuda_stream, sample)
+            if sample:
+                self.sample_graph = graph
+            else:
+                self.graph = graph
         torch.cuda.synchronize()
 
     def replay(self) -> None:
         self.graph.replay()
 
-    def generate_tw_marlin_graph(self, first_token: int, max_tokens: int) -> List[int]:
-        """Greedy decode `max_tokens` tokens from `first_token` by replaying the captured step
-        (generate.rs:2512-2536 without the per-token host round trip)."""
-        if self.graph is None:
-            self.capture()
+    def generate_tw_marlin_graph(self, first_token: int, max_tokens: int, sampling: Optional[SamplingParams] = None,
+                                 random: Optional[torch.Tensor] = None) -> List[int]:
+        """Decode `max_tokens` tokens from `first_token` by replaying the captured step
+        (generate.rs:2512-2536 without the per-token host round trip): greedily, or drawn by `sampling` from `random`, a number
+        in [0, 1) a token (those of the settings' seed if None)."""
+        if (self.graph if sampling is None else self.sample_graph) is None:
+            self.capture(sampling is not None)
         self.set_token(first_token)
         start = int(self.buf.step.item())
         pos = int(self.buf.pos.item())
@@ -320,7 +369,15 @@ class QuantizedGenerationEngine:
         if start + max_tokens > self.buf.history.numel():
             raise _lib.TwmError(_lib.TWM_EINVAL, f"generate_tw_marlin_graph: {start} + {max_tokens} tokens do not fit the "
                                                  f"token list ({self.buf.history.numel()} entries); reset_history() first")
+        if sampling is not None:
+            if random is None:
+                random = torch.rand(max_tokens, generator=sampling.generator())
+            if random.numel() < max_tokens:
+                raise _lib.TwmError(_lib.TWM_EINVAL, f"generate_tw_marlin_graph: {random.numel()} random numbers for {max_tokens} tokens")
+            self.buf.loop.set(sampling, random[:max_tokens], start)
+            torch.cuda.synchronize()
+        graph = self.graph if sampling is None else self.sample_graph
         for _ in range(max_tokens):
-            self.graph.replay()
+            graph.replay()
         torch.cuda.synchronize()
         return self.buf.history[start:start + max_tokens].tolist()

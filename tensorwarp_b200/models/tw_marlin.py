@@ -13,6 +13,7 @@ import torch
 from ..checkpoint import CheckpointError
 from ..generate import Q4Model, QuantizedGenerationEngine, TransformerConfig
 from ..registry import register
+from ..sampling import SamplingParams
 from ..state import StateError
 
 
@@ -72,6 +73,12 @@ class Q4StepEngine:
         return torch.stack(rows) if rows else None
 
     def greedy(self, seq: int, tokens: Sequence[int], count: int) -> List[int]:
+        return self._generate(seq, tokens, count, {})
+
+    def sample(self, seq: int, tokens: Sequence[int], count: int, params: SamplingParams, generator: torch.Generator) -> List[int]:
+        return self._generate(seq, tokens, count, {"sampling": params, "random": torch.rand(max(count, 0), generator=generator)})
+
+    def _generate(self, seq: int, tokens: Sequence[int], count: int, how: dict) -> List[int]:
         self._reserve(seq, tokens, max(count - 1, 0))
         if count < 1:
             return []
@@ -79,14 +86,14 @@ class Q4StepEngine:
             self._run(token)
         self.engine.reset_history()
         self.engine.set_position(self._length)
-        out = self.engine.generate_tw_marlin_graph(tokens[-1], count)
+        out = self.engine.generate_tw_marlin_graph(tokens[-1], count, **how)
         self._length += count
         return out
 
 
 @register("TWMarlinQ4")
 def build(config: dict, weights, dtype: torch.dtype = torch.bfloat16, device="cuda", max_tokens: Optional[int] = None,
-          **_) -> Q4StepEngine:
+          kv_cache: str = "f16", **_) -> Q4StepEngine:
     if weights is not None:
         raise CheckpointError("TWMarlinQ4 has no checkpoint format here; remove model.safetensors to run synthetic weights")
     if dtype == torch.float32:
@@ -94,4 +101,4 @@ def build(config: dict, weights, dtype: torch.dtype = torch.bfloat16, device="cu
     cfg = parse_config(config)
     if max_tokens:
         cfg.max_seq = min(cfg.max_seq, max_tokens)
-    return Q4StepEngine(QuantizedGenerationEngine(Q4Model(cfg, device, seed=int(config.get("seed", 0)))))
+    return Q4StepEngine(QuantizedGenerationEngine(Q4Model(cfg, device, seed=int(config.get("seed", 0))), kv_cache=kv_cache))

@@ -30,6 +30,32 @@ class SamplingParams:
             raise ValueError("top_k must not be negative, top_p in (0, 1] and min_p in [0, 1]")
 
 
+    def generator(self) -> torch.Generator:
+        """Random numbers of a request: the same ones for the same seed, however its tokens are dealt to calls."""
+        return torch.Generator().manual_seed(self.seed)
+
+
+class LoopState:
+    """Device memory of a decode loop of one row that samples: its settings, which a captured step reads, and the random numbers of
+    its steps."""
+
+    def __init__(self, steps: int, device):
+        self._settings = torch.zeros(4, dtype=torch.float32, device=device)
+        self.random = torch.zeros(max(steps, 1), dtype=torch.float32, device=device)
+
+    def set(self, params: SamplingParams, random: torch.Tensor, at: int = 0) -> None:
+        """On the current stream: the settings of the steps to come, and the numbers of steps at, at + 1, ..."""
+        top_k = torch.tensor([min(params.top_k, 1 << 30)], dtype=torch.int32).view(torch.float32)
+        self._settings.copy_(torch.cat((torch.tensor([params.temperature, params.top_p, params.min_p]), top_k)))
+        self.random[at:at + random.numel()].copy_(random)
+
+    def args(self, logits: torch.Tensor, vocab: int, token: int, step: int, history: torch.Tensor, pos: int, length: int) -> _lib.SampleArgs:
+        """The call of a step: f32 logits of one row; token, step, pos and length as addresses."""
+        p = self._settings.data_ptr()
+        return _lib.SampleArgs(1, vocab, _lib.TWM_F32, logits.data_ptr(), vocab, self.random.data_ptr(), p, p + 12, p + 4, p + 8, token, None, step,
+                               self.random.numel(), history.data_ptr(), history.numel(), pos, length)
+
+
 def _column(name: str, t: Optional[torch.Tensor], dtype: torch.dtype, rows: int, index: int) -> Optional[int]:
     if t is None:
         return None

@@ -1,8 +1,8 @@
 """Serves requests on a step engine: first come, first served admission into the engine's free sequences,
 prompts in portions, live sequences in turn.
 
-Each turn runs one sequence: the next portion of its prompt, or a burst of greedily decoded tokens
-(one host synchronisation a burst).  A sequence's slot goes back to the engine when it has finished.
+Each turn runs one sequence: the next portion of its prompt, or a burst of decoded tokens, greedily or
+drawn as the request says (one host synchronisation a burst).  A sequence's slot goes back to the engine when it has finished.
 """
 from __future__ import annotations
 
@@ -18,6 +18,8 @@ class Request:
     stop_token: Optional[int] = None
     generated: List[int] = field(default_factory=list)
     done: bool = False
+    sampling: Optional["SamplingParams"] = None         # noqa: F821  (sampling.SamplingParams; None: greedily)
+    generator: object = None                            # of its random numbers
 
 
 @dataclass
@@ -35,15 +37,18 @@ class Scheduler:
         self._waiting: Deque[Request] = deque()
         self._live: Deque[_Live] = deque()
 
-    def submit(self, tokens: Sequence[int], max_new_tokens: int, stop_token: Optional[int] = None) -> Request:
+    def submit(self, tokens: Sequence[int], max_new_tokens: int, stop_token: Optional[int] = None, sampling=None) -> Request:
+        """sampling: a ``sampling.SamplingParams``; None decodes greedily."""
         tokens = list(tokens)
+        if sampling is not None and not hasattr(self.engine, "sample"):
+            raise ValueError("the engine decodes greedily only")
         if not tokens or max_new_tokens < 1:
             raise ValueError("a request has at least one token and asks for at least one")
         if len(tokens) + max_new_tokens - 1 > self.engine.capacity:
             raise ValueError(f"{len(tokens)} tokens and {max_new_tokens} new ones do not fit the {self.engine.capacity} of a sequence")
         if min(tokens) < 0 or max(tokens) >= self.engine.vocab:
             raise ValueError(f"token outside the vocabulary of {self.engine.vocab}")
-        request = Request(tokens, max_new_tokens, stop_token)
+        request = Request(tokens, max_new_tokens, stop_token, sampling=sampling, generator=sampling.generator() if sampling is not None else None)
         self._waiting.append(request)
         return request
 
@@ -65,7 +70,10 @@ class Scheduler:
                 del live.pending[:self.portion]
             else:
                 count = min(self.burst, request.max_new_tokens - len(request.generated))
-                new = self.engine.greedy(live.seq, live.pending, count)
+                if request.sampling is None:
+                    new = self.engine.greedy(live.seq, live.pending, count)
+                else:
+                    new = self.engine.sample(live.seq, live.pending, count, request.sampling, request.generator)
                 if request.stop_token is not None and request.stop_token in new:
                     new = new[:new.index(request.stop_token) + 1]
                     request.done = True

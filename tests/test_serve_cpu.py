@@ -5,6 +5,7 @@ import pytest
 import torch
 
 from tensorwarp_b200 import _lib, cache8, sampling
+from tensorwarp_b200.scheduler import Scheduler
 
 
 def cache(**kw):
@@ -91,3 +92,63 @@ def test_sampling_params():
                 dict(min_p=-0.1), dict(min_p=1.1)):
         with pytest.raises(ValueError):
             sampling.SamplingParams(**bad)
+
+
+class Drawing:
+    """An engine whose tokens are its sequence's random numbers."""
+    vocab, capacity, max_live = 1000, 64, 2
+
+    def __init__(self):
+        self.calls, self.live = [], {}
+
+    def open(self):
+        seq = min(set(range(self.max_live)) - set(self.live))
+        self.live[seq] = 0
+        return seq
+
+    def close(self, seq):
+        del self.live[seq]
+
+    def step(self, seq, tokens, want=()):
+        self.live[seq] += len(tokens)
+
+    def greedy(self, seq, tokens, count):
+        self.calls.append(("greedy", count))
+        self.live[seq] += len(tokens) + count - 1
+        return [7] * count
+
+    def sample(self, seq, tokens, count, params, generator):
+        self.calls.append(("sample", count, params))
+        self.live[seq] += len(tokens) + count - 1
+        return (torch.rand(count, generator=generator) * self.vocab).int().tolist()
+
+
+def test_scheduler_hands_sampling_on():
+    """Settings and generator go with the request: other bursts, the same tokens; a request without settings is greedy."""
+    params, seen = sampling.SamplingParams(temperature=0.5, seed=5), []
+    for burst in (1, 4, 16):
+        sch = Scheduler(Drawing(), portion=4, burst=burst)
+        requests = [sch.submit([1, 2, 3, 4, 5, 6], 10, sampling=params), sch.submit([9], 4), sch.submit([1], 10, sampling=params)]
+        assert len(list(sch.run())) == 3
+        assert {c[0] for c in sch.engine.calls} == {"greedy", "sample"} and all(c[2] is params for c in sch.engine.calls if c[0] == "sample")
+        seen.append([r.generated for r in requests])
+        assert requests[1].generated == [7] * 4 and requests[0].generated == requests[2].generated
+    assert seen[0] == seen[1] == seen[2]
+
+
+def test_scheduler_refuses_sampling_on_engines_without_it():
+    class Greedy(Drawing):
+        sample = property(lambda self: (_ for _ in ()).throw(AttributeError()))
+    sch = Scheduler(Greedy())
+    sch.submit([1], 2)
+    with pytest.raises(ValueError):
+        sch.submit([1], 2, sampling=sampling.SamplingParams())
+
+
+def test_command_line_takes_settings():
+    """Bad settings are refused before a model is loaded."""
+    from tensorwarp_b200.__main__ import main
+    with pytest.raises(ValueError):
+        main(["generate", "--model", "/nowhere", "--tokens", "1", "--temperature", "-1"])
+    with pytest.raises(SystemExit):
+        main(["generate", "--model", "/nowhere", "--tokens", "1", "--kv-cache", "int4"])
