@@ -46,9 +46,19 @@ typedef struct twm_cache8 {
  * stride ldqkv), q_out the rotated queries [rows][q] (f16, row stride ldq).  rope_table: f32 [capacity][head_dim], cosines then
  * sines of every position, or NULL for none; bias: f32 [q | k | v] or NULL.  What twm_rope_append is to the FP16 cache.
  * Pointers on 16 bytes, row strides multiples of 8. */
-twm_status twm_cache8_append(const twm_cache8* cache, void* q_out_f16, long ldq, const void* qkv_f16, long ldqkv, const float* bias,
-                             const float* rope_table, int num_heads, int rows, const int* row_start, int max_rows, const int* start,
-                             int flags, void* stream);
+typedef struct twm_cache8_append_args {
+    void* q_out;
+    long ldq;
+    const void* qkv;
+    long ldqkv;
+    const float* bias;
+    const float* rope_table;
+    int num_heads;
+    int rows, max_rows;
+    const int* row_start;
+    const int* start;
+} twm_cache8_append_args;
+twm_status twm_cache8_append(const twm_cache8* cache, const twm_cache8_append_args* args, int flags, void* stream);
 
 /* Bytes of workspace twm_cache8_attention needs.  Nothing in it is kept from call to call. */
 size_t twm_cache8_attention_bytes(const twm_cache8* cache, int num_heads, int max_rows);
@@ -56,10 +66,23 @@ size_t twm_cache8_attention_bytes(const twm_cache8* cache, int num_heads, int ma
 /* Softmax attention of the rows of a call over the cache, which already holds their own keys and values: the row at position p
  * sees the keys j <= p with p - j < window (window 0: all).  A sequence taken out of the call gets zeros.
  * out and q: f16 [rows][num_heads * head_dim], row strides ldo and ldq; query head h reads key/value head
- * h / (num_heads / kv_heads).  Pointers on 16 bytes, row strides multiples of 8.  Calls that share a workspace must not overlap. */
-twm_status twm_cache8_attention(const twm_cache8* cache, void* out_f16, long ldo, const void* q_f16, long ldq, int num_heads, int rows,
-                                const int* row_start, int max_rows, const int* start, float scale, int window, void* workspace,
-                                size_t workspace_bytes, int flags, void* stream);
+ * h / (num_heads / kv_heads); scale is positive.  Pointers on 16 bytes, row strides multiples of 8.  Calls that share a workspace must
+ * not overlap. */
+typedef struct twm_cache8_attention_args {
+    void* out;
+    long ldo;
+    const void* q;
+    long ldq;
+    int num_heads;
+    int rows, max_rows;
+    int window;
+    const int* row_start;
+    const int* start;
+    void* workspace;
+    size_t workspace_bytes;
+    float scale;
+} twm_cache8_attention_args;
+twm_status twm_cache8_attention(const twm_cache8* cache, const twm_cache8_attention_args* args, int flags, void* stream);
 
 /* One token of every row of logits.  With w_i = exp((l_i - max l) / temperature) and the order of falling l, equal ones by
  * rising index:

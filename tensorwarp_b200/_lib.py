@@ -68,12 +68,36 @@ class Cache8(C.Structure):
                 ("k_tail", C.c_void_p), ("v_tail", C.c_void_p)]
 
 
+class Cache8AppendArgs(C.Structure):
+    """``twm_cache8_append_args``."""
+    _fields_ = [("q_out", C.c_void_p), ("ldq", C.c_long), ("qkv", C.c_void_p), ("ldqkv", C.c_long), ("bias", C.c_void_p), ("rope_table", C.c_void_p),
+                ("num_heads", C.c_int), ("rows", C.c_int), ("max_rows", C.c_int), ("row_start", C.c_void_p), ("start", C.c_void_p)]
+
+
+class Cache8AttentionArgs(C.Structure):
+    """``twm_cache8_attention_args``."""
+    _fields_ = [("out", C.c_void_p), ("ldo", C.c_long), ("q", C.c_void_p), ("ldq", C.c_long), ("num_heads", C.c_int), ("rows", C.c_int),
+                ("max_rows", C.c_int), ("window", C.c_int), ("row_start", C.c_void_p), ("start", C.c_void_p), ("workspace", C.c_void_p),
+                ("workspace_bytes", C.c_size_t), ("scale", C.c_float)]
+
+
+# the same structures as bytes, from all fields in order
+_append_args, _attention_args = struct.Struct("@PlPlPP3iPP"), struct.Struct("@PlPl4iPPPNf4x")
+assert _append_args.size == C.sizeof(Cache8AppendArgs) and _attention_args.size == C.sizeof(Cache8AttentionArgs)
+pack_append_args, pack_attention_args = _append_args.pack, _attention_args.pack
+
+
 class SampleArgs(C.Structure):
     """``twm_sample_args``."""
     _fields_ = [("rows", C.c_int), ("vocab", C.c_int), ("dtype", C.c_int), ("logits", C.c_void_p), ("ld", C.c_long),
                 ("random", C.c_void_p), ("temperature", C.c_void_p), ("top_k", C.c_void_p), ("top_p", C.c_void_p), ("min_p", C.c_void_p),
                 ("tokens", C.c_void_p), ("prob", C.c_void_p), ("step", C.c_void_p), ("random_count", C.c_int), ("history", C.c_void_p),
                 ("history_capacity", C.c_int), ("pos", C.c_void_p), ("len", C.c_void_p)]
+
+
+_sample_args = struct.Struct("@3iPlPPPPPPPPiPiPP")
+assert _sample_args.size == C.sizeof(SampleArgs)
+pack_sample_args = _sample_args.pack
 
 
 class ChainOp(C.Structure):
@@ -148,13 +172,11 @@ SIGNATURES = {
     "twm_argmax_scratch_bytes": (C.c_size_t, []),
     "twm_argmax_advance": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int,
                                      C.c_void_p, C.c_size_t, C.c_int, C.c_void_p]),
-    # include/twm_serve.h (a twm_cache8 by address)
-    "twm_cache8_append": (C.c_int, [C.c_void_p, C.c_void_p, C.c_long, C.c_void_p, C.c_long, C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_void_p,
-                                    C.c_int, C.c_void_p, C.c_int, C.c_void_p]),
+    # include/twm_serve.h (a twm_cache8 by address, the arguments by reference, or as bytes)
+    "twm_cache8_append": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.c_void_p]),
     "twm_cache8_attention_bytes": (C.c_size_t, [C.c_void_p, C.c_int, C.c_int]),
-    "twm_cache8_attention": (C.c_int, [C.c_void_p, C.c_void_p, C.c_long, C.c_void_p, C.c_long, C.c_int, C.c_int, C.c_void_p, C.c_int, C.c_void_p,
-                                       C.c_float, C.c_int, C.c_void_p, C.c_size_t, C.c_int, C.c_void_p]),
-    "twm_sample": (C.c_int, [C.POINTER(SampleArgs), C.c_int, C.c_void_p]),
+    "twm_cache8_attention": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.c_void_p]),
+    "twm_sample": (C.c_int, [C.c_void_p, C.c_int, C.c_void_p]),
     "twm_status_string": (C.c_char_p, [C.c_int]),
     "twm_last_error": (C.c_char_p, []),
     "twm_version": (C.c_char_p, []),

@@ -68,7 +68,7 @@ class Workspace:
     def __init__(self, nbytes: int, device="cuda"):
         self.nbytes = max(int(nbytes), 16)
         self.buf = torch.empty(self.nbytes, dtype=torch.uint8, device=device)
-        self.ptr = self.buf.data_ptr()
+        self.ptr, self.index = self.buf.data_ptr(), self.buf.get_device()
 
     @classmethod
     def for_cache(cls, cache: Cache8, num_heads: int, max_rows: int = 1) -> "Workspace":
@@ -92,15 +92,16 @@ def _refuse(where: str, cache: Cache8, wide: torch.Tensor, narrow: torch.Tensor,
     raise TwmError(_lib.TWM_EINVAL, f"{where}: expected rows of {columns} and {out_columns} numbers, as many of both")
 
 
-def _fits(cache: Cache8, wide: torch.Tensor, narrow: torch.Tensor, start: torch.Tensor, row_start: Optional[torch.Tensor], columns: int,
-          out_columns: int) -> bool:
-    # once per layer and token: integers and identities, no objects made for a comparison
-    index, i32, f16 = cache.index, torch.int32, torch.float16
-    if (wide.get_device() != index or narrow.get_device() != index or start.get_device() != index or wide.dtype is not f16 or narrow.dtype is not f16
-            or wide.dim() != 2 or narrow.dim() != 2 or start.dtype is not i32 or start.numel() != cache.seqs or not start.is_contiguous()
-            or wide.size(1) != columns or narrow.size(1) != out_columns or narrow.size(0) < wide.size(0) or wide.stride(1) != 1 or narrow.stride(1) != 1):
-        return False
-    return row_start is None or (row_start.get_device() == index and row_start.dtype is i32 and row_start.numel() == cache.seqs + 1 and row_start.is_contiguous())
+def _pointer(cache: Cache8, start: torch.Tensor, row_start: Optional[torch.Tensor]) -> Optional[int]:
+    """Address of row_start (0: none); None if it or start is not what a call takes."""
+    i32, index = torch.int32, cache.index
+    if start.dtype is not i32 or start.get_device() != index or start.numel() != cache.seqs or not start.is_contiguous():
+        return None
+    if row_start is None:
+        return 0
+    if row_start.dtype is not i32 or row_start.get_device() != index or row_start.numel() != cache.seqs + 1 or not row_start.is_contiguous():
+        return None
+    return row_start.data_ptr()
 
 
 def append(cache: Cache8, qkv: torch.Tensor, q_out: torch.Tensor, start: torch.Tensor, *, num_heads: int, row_start: Optional[torch.Tensor] = None,
@@ -110,21 +111,28 @@ def append(cache: Cache8, qkv: torch.Tensor, q_out: torch.Tensor, start: torch.T
     values to the cache.  start int32 [seqs]: tokens of each sequence before the call (< 0: not in the call); row_start int32
     [seqs + 1]: its rows among the call's, at most `max_rows` (None: one row a sequence).  rope: ``rope_table`` of the cache's capacity;
     bias f32 of a whole row."""
-    d = cache.head_dim
-    columns = (num_heads + 2 * cache.kv_heads) * d
-    if not _fits(cache, qkv, q_out, start, row_start, columns, num_heads * d):
-        _refuse("append", cache, qkv, q_out, start, row_start, columns, num_heads * d)
-    if bias is not None and (bias.dtype is not torch.float32 or bias.numel() != columns or not bias.is_contiguous() or bias.get_device() != cache.index):
-        raise TwmError(_lib.TWM_EINVAL, "append: bias must be float32 of a whole row")
-    if rope is not None and (rope.dtype is not torch.float32 or rope.numel() < cache.capacity * d or not rope.is_contiguous() or rope.get_device() != cache.index):
-        raise TwmError(_lib.TWM_EINVAL, "append: rope must be float32 [capacity, head_dim]")
-    if torch._C._cuda_getDevice() != cache.index:
-        with torch.cuda.device(cache.index):
+    # Once per layer and token, and as long as the call itself takes: sizes and strides are read at once, and the arguments packed by struct.
+    d, index, f16 = cache.head_dim, cache.index, torch.float16
+    columns, out_columns = (num_heads + 2 * cache.kv_heads) * d, num_heads * d
+    size, ld, out_size, out_ld = qkv.size(), qkv.stride(), q_out.size(), q_out.stride()
+    at = _pointer(cache, start, row_start)
+    if (at is None or len(size) != 2 or len(out_size) != 2 or size[1] != columns or out_size[1] != out_columns or out_size[0] < size[0] or ld[1] != 1
+            or out_ld[1] != 1 or qkv.dtype is not f16 or q_out.dtype is not f16 or qkv.get_device() != index or q_out.get_device() != index):
+        _refuse("append", cache, qkv, q_out, start, row_start, columns, out_columns)
+    bias_at = rope_at = 0
+    if bias is not None:
+        if bias.dtype is not torch.float32 or bias.numel() != columns or not bias.is_contiguous() or bias.get_device() != index:
+            raise TwmError(_lib.TWM_EINVAL, "append: bias must be float32 of a whole row")
+        bias_at = bias.data_ptr()
+    if rope is not None:
+        if rope.dtype is not torch.float32 or rope.numel() < cache.capacity * d or not rope.is_contiguous() or rope.get_device() != index:
+            raise TwmError(_lib.TWM_EINVAL, "append: rope must be float32 [capacity, head_dim]")
+        rope_at = rope.data_ptr()
+    if torch._C._cuda_getDevice() != index:
+        with torch.cuda.device(index):
             return append(cache, qkv, q_out, start, num_heads=num_heads, row_start=row_start, max_rows=max_rows, bias=bias, rope=rope, stream=stream, flags=flags)
-    status = _lib.lib().twm_cache8_append(cache._ref, q_out.data_ptr(), q_out.stride(0), qkv.data_ptr(), qkv.stride(0),
-                                          bias.data_ptr() if bias is not None else None, rope.data_ptr() if rope is not None else None, num_heads,
-                                          qkv.size(0), row_start.data_ptr() if row_start is not None else None, max_rows, start.data_ptr(), flags,
-                                          _stream_ptr(stream))
+    args = _lib.pack_append_args(q_out.data_ptr(), out_ld[0], qkv.data_ptr(), ld[0], bias_at, rope_at, num_heads, size[0], max_rows, at, start.data_ptr())
+    status = _lib.lib().twm_cache8_append(cache._ref, args, flags, _stream_ptr(stream))
     if status:
         check(status, "twm_cache8_append")
 
@@ -135,21 +143,24 @@ def attention(cache: Cache8, q: torch.Tensor, out: torch.Tensor, start: torch.Te
     """Causal softmax attention of q f16 [rows, num_heads * head_dim] over the cache, which holds the rows' own keys and values already
     (``append`` with the same start and row_start); out like q.  scale: 1/sqrt(head_dim) if None; window: how many of the newest keys
     a row sees (0: all).  workspace: ``Workspace.for_cache``; without one the call makes its own."""
-    d = cache.head_dim
-    if not _fits(cache, q, out, start, row_start, num_heads * d, num_heads * d):
-        _refuse("attention", cache, q, out, start, row_start, num_heads * d, num_heads * d)
-    if torch._C._cuda_getDevice() != cache.index:
-        with torch.cuda.device(cache.index):
+    d, index, f16 = cache.head_dim, cache.index, torch.float16
+    columns = num_heads * d
+    size, ld, out_size, out_ld = q.size(), q.stride(), out.size(), out.stride()
+    at = _pointer(cache, start, row_start)
+    if (at is None or len(size) != 2 or len(out_size) != 2 or size[1] != columns or out_size[1] != columns or out_size[0] < size[0] or ld[1] != 1
+            or out_ld[1] != 1 or q.dtype is not f16 or out.dtype is not f16 or q.get_device() != index or out.get_device() != index):
+        _refuse("attention", cache, q, out, start, row_start, columns, columns)
+    if torch._C._cuda_getDevice() != index:
+        with torch.cuda.device(index):
             return attention(cache, q, out, start, num_heads=num_heads, row_start=row_start, max_rows=max_rows, scale=scale, window=window,
                              workspace=workspace, stream=stream, flags=flags)
     if workspace is None:
         with torch.cuda.stream(stream):
             workspace = Workspace.for_cache(cache, num_heads, max_rows)
-    elif workspace.buf.get_device() != cache.index:
+    elif workspace.index != index:
         raise TwmError(_lib.TWM_EINVAL, "attention: the workspace is on another device")
-    status = _lib.lib().twm_cache8_attention(cache._ref, out.data_ptr(), out.stride(0), q.data_ptr(), q.stride(0), num_heads, q.size(0),
-                                             row_start.data_ptr() if row_start is not None else None, max_rows, start.data_ptr(),
-                                             1.0 / math.sqrt(d) if scale is None else scale, window, workspace.ptr, workspace.nbytes,
-                                             flags, _stream_ptr(stream))
+    args = _lib.pack_attention_args(out.data_ptr(), out_ld[0], q.data_ptr(), ld[0], num_heads, size[0], max_rows, window, at, start.data_ptr(), workspace.ptr,
+                                    workspace.nbytes, 1.0 / math.sqrt(d) if scale is None else scale)
+    status = _lib.lib().twm_cache8_attention(cache._ref, args, flags, _stream_ptr(stream))
     if status:
         check(status, "twm_cache8_attention")

@@ -2,6 +2,7 @@
 #pragma once
 
 #include <climits>
+#include <cmath>
 
 #include "twm_cache8.cuh"
 #include "twm_cache8_attn.cuh"
@@ -113,20 +114,20 @@ twm_status launch_merge(const twm::cache8::AttnArgs& a, const AttnPlan& p, int f
 
 extern "C" {
 
-twm_status twm_cache8_append(const twm_cache8* cache, void* q_out, long ldq, const void* qkv, long ldqkv, const float* bias,
-                             const float* rope_table, int num_heads, int rows, const int* row_start, int max_rows, const int* start,
-                             int flags, void* stream)
+twm_status twm_cache8_append(const twm_cache8* cache, const twm_cache8_append_args* x, int flags, void* stream)
 {
-    twm_status st = check_cache8(cache, num_heads, rows, row_start, max_rows, start);
+    if (!x) return TWM_EINVAL;
+    twm_status st = check_cache8(cache, x->num_heads, x->rows, x->row_start, x->max_rows, x->start);
     if (st == TWM_EINVAL) return st;
-    if (!q_out || !qkv || ldq < (long)num_heads * cache->head_dim || ldqkv < (long)(num_heads + 2 * cache->kv_heads) * cache->head_dim) return TWM_EINVAL;
+    if (!x->q_out || !x->qkv || x->ldq < (long)x->num_heads * cache->head_dim || x->ldqkv < (long)(x->num_heads + 2 * cache->kv_heads) * cache->head_dim)
+        return TWM_EINVAL;
     if (st != TWM_OK) return st;
-    if (off16(q_out) || off16(qkv) || off16(bias) || off16(rope_table) || (ldq & 7) || (ldqkv & 7)) return TWM_EALIGN;
+    if (off16(x->q_out) || off16(x->qkv) || off16(x->bias) || off16(x->rope_table) || (x->ldq & 7) || (x->ldqkv & 7)) return TWM_EALIGN;
     if ((st = ensure_device(nullptr)) != TWM_OK) return st;
-    const twm::cache8::AppendArgs a = {device_cache(cache), {row_start, start, rows, max_rows}, (__half*)q_out, (const __half*)qkv, bias, rope_table,
-                                       ldq, ldqkv, num_heads, max_rows >= TWM_CACHE8_BLOCK / 4 ? 1 : 0};
+    const twm::cache8::AppendArgs a = {device_cache(cache), {x->row_start, x->start, x->rows, x->max_rows}, (__half*)x->q_out, (const __half*)x->qkv, x->bias,
+                                       x->rope_table, x->ldq, x->ldqkv, x->num_heads, x->max_rows >= TWM_CACHE8_BLOCK / 4 ? 1 : 0};
     // blocks that max_rows tokens can touch, wherever they begin
-    const dim3 grid((unsigned)(((long)max_rows + 2 * TWM_CACHE8_BLOCK - 2) / TWM_CACHE8_BLOCK), cache->kv_heads + (a.apart ? num_heads : 0), cache->seqs);
+    const dim3 grid((unsigned)(((long)x->max_rows + 2 * TWM_CACHE8_BLOCK - 2) / TWM_CACHE8_BLOCK), cache->kv_heads + (a.apart ? x->num_heads : 0), cache->seqs);
     return launch_op("twm_cache8_append", cache->head_dim == 64 ? twm::cache8::append_kernel<64> : twm::cache8::append_kernel<128>, grid,
                      dim3(twm::cache8::APPEND_THREADS), 0, flags, stream, a);
 }
@@ -138,22 +139,23 @@ size_t twm_cache8_attention_bytes(const twm_cache8* c, int num_heads, int max_ro
     return (size_t)p.ctas * (sizeof(twm::cache8::Join) + 2 * twm::cache8::partial_floats(p.tile, c->head_dim) * sizeof(float));
 }
 
-twm_status twm_cache8_attention(const twm_cache8* cache, void* out, long ldo, const void* q, long ldq, int num_heads, int rows, const int* row_start,
-                                int max_rows, const int* start, float scale, int window, void* workspace, size_t workspace_bytes, int flags,
-                                void* stream)
+twm_status twm_cache8_attention(const twm_cache8* cache, const twm_cache8_attention_args* x, int flags, void* stream)
 {
-    twm_status st = check_cache8(cache, num_heads, rows, row_start, max_rows, start);
+    if (!x) return TWM_EINVAL;
+    twm_status st = check_cache8(cache, x->num_heads, x->rows, x->row_start, x->max_rows, x->start);
     if (st == TWM_EINVAL) return st;
     const int D = cache->head_dim;
-    if (!out || !q || !workspace || window < 0 || !(scale > 0.0f) || ldo < (long)num_heads * D || ldq < (long)num_heads * D) return TWM_EINVAL;
+    if (!x->out || !x->q || !x->workspace || x->window < 0 || !(x->scale > 0.0f) || !(x->scale < INFINITY) || x->ldo < (long)x->num_heads * D ||
+        x->ldq < (long)x->num_heads * D)
+        return TWM_EINVAL;
     if (st != TWM_OK) return st;
-    if (off16(out) || off16(q) || off16(workspace) || (ldo & 7) || (ldq & 7)) return TWM_EALIGN;
-    if (workspace_bytes < twm_cache8_attention_bytes(cache, num_heads, max_rows)) return TWM_EWORKSPACE;
+    if (off16(x->out) || off16(x->q) || off16(x->workspace) || (x->ldo & 7) || (x->ldq & 7)) return TWM_EALIGN;
+    if (x->workspace_bytes < twm_cache8_attention_bytes(cache, x->num_heads, x->max_rows)) return TWM_EWORKSPACE;
     if ((st = ensure_device(nullptr)) != TWM_OK) return st;
-    const AttnPlan p = plan_attention(num_heads / cache->kv_heads, max_rows, D);
-    twm::cache8::AttnArgs a = {device_cache(cache), {row_start, start, rows, max_rows}, (__half*)out, (const __half*)q, ldo, ldq, num_heads,
-                               window ? window : INT_MAX, scale, (twm::cache8::Join*)workspace,
-                               (float*)((twm::cache8::Join*)workspace + p.ctas), {}, {}};
+    const AttnPlan p = plan_attention(x->num_heads / cache->kv_heads, x->max_rows, D);
+    auto* joins = (twm::cache8::Join*)x->workspace;
+    twm::cache8::AttnArgs a = {device_cache(cache), {x->row_start, x->start, x->rows, x->max_rows}, (__half*)x->out, (const __half*)x->q, x->ldo, x->ldq,
+                               x->num_heads, x->window ? x->window : INT_MAX, x->scale, joins, (float*)(joins + p.ctas), {}, {}};
     if (!make_codes_map(&a.k_map, cache, cache->k) || !make_codes_map(&a.v_map, cache, cache->v)) {
         snprintf(t_last_error, sizeof(t_last_error), "cuTensorMapEncodeTiled failed for a cache held in 8 bits");
         return TWM_ELAUNCH;

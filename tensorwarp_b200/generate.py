@@ -203,12 +203,12 @@ class QuantizedGenerationEngine:
     def _cache8_ops(self, cache, lw, stream_ptr: int):
         """A layer's append to, and attention over, its cache held in 8 bits."""
         lib, cfg, b, fl = _lib.lib(), self.cfg, self.buf, self.flags
-        append = lambda: check(lib.twm_cache8_append(  # noqa: E731
-            cache._ref, b.query.data_ptr(), cfg.q_dim, b.qkv.data_ptr(), b.qkv.numel(), lw.bqkv.data_ptr() if lw.bqkv is not None else None,
-            b.rope.data_ptr(), cfg.num_heads, 1, None, 1, b.pos.data_ptr(), fl, stream_ptr), "twm_cache8_append")
-        attend = lambda: check(lib.twm_cache8_attention(  # noqa: E731
-            cache._ref, b.attn.data_ptr(), cfg.q_dim, b.query.data_ptr(), cfg.q_dim, cfg.num_heads, 1, None, 1, b.pos.data_ptr(), cfg.head_dim ** -0.5, 0,
-            b.attn_workspace.ptr, b.attn_workspace.nbytes, fl, stream_ptr), "twm_cache8_attention")
+        appended = _lib.Cache8AppendArgs(b.query.data_ptr(), cfg.q_dim, b.qkv.data_ptr(), b.qkv.numel(), lw.bqkv.data_ptr() if lw.bqkv is not None else None,
+                                         b.rope.data_ptr(), cfg.num_heads, 1, 1, None, b.pos.data_ptr())
+        attended = _lib.Cache8AttentionArgs(b.attn.data_ptr(), cfg.q_dim, b.query.data_ptr(), cfg.q_dim, cfg.num_heads, 1, 1, 0, None, b.pos.data_ptr(),
+                                            b.attn_workspace.ptr, b.attn_workspace.nbytes, cfg.head_dim ** -0.5)
+        append = lambda: check(lib.twm_cache8_append(cache._ref, C.addressof(appended), fl, stream_ptr), "twm_cache8_append")  # noqa: E731
+        attend = lambda: check(lib.twm_cache8_attention(cache._ref, C.addressof(attended), fl, stream_ptr), "twm_cache8_attention")  # noqa: E731
         return [("kv_append", 1, append), ("attention", 2, attend)]
 
     def _step_ops(self, stream_ptr: int, sample: bool = False):
@@ -271,7 +271,7 @@ class QuantizedGenerationEngine:
                                                                     stream_ptr), "twm_lm_head")))
         if sample:
             args = b.loop.args(b.logits, cfg.vocab, b.token.data_ptr(), b.step.data_ptr(), b.history, b.pos.data_ptr(), b.cache_len.data_ptr())
-            ops.append(("sample", 1, lambda: check(lib.twm_sample(args, fl, stream_ptr), "twm_sample")))
+            ops.append(("sample", 1, lambda: check(lib.twm_sample(C.addressof(args), fl, stream_ptr), "twm_sample")))
         else:
             ops.append(("argmax_advance", 2, lambda: check(lib.twm_argmax_advance(
                 b.token.data_ptr(), b.history.data_ptr(), b.history.numel(), b.pos.data_ptr(), b.cache_len.data_ptr(),

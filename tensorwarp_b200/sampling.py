@@ -56,9 +56,9 @@ class LoopState:
                                self.random.numel(), history.data_ptr(), history.numel(), pos, length)
 
 
-def _column(name: str, t: Optional[torch.Tensor], dtype: torch.dtype, rows: int, index: int) -> Optional[int]:
+def _column(name: str, t: Optional[torch.Tensor], dtype: torch.dtype, rows: int, index: int) -> int:
     if t is None:
-        return None
+        return 0
     if t.dtype is not dtype or t.numel() != rows or t.get_device() != index or not t.is_contiguous():
         _require_cuda(t)
         raise TwmError(_lib.TWM_EINVAL, f"sample: {name} must be {dtype} [{rows}] on the logits' device")
@@ -71,21 +71,22 @@ def sample(logits: torch.Tensor, random: torch.Tensor, tokens: torch.Tensor, *, 
     """tokens int32 [rows]: one of each row of logits (f32, f16 or bf16 [rows, vocab]), chosen by random f32 [rows] in [0, 1).
     temperature, top_p, min_p f32 [rows] and top_k int32 [rows], None to leave one out (1 for the temperature); prob f32 [rows]
     gets what the kept tokens' distribution gave the token.  ``include/twm_serve.h`` has the definition."""
-    if not logits.is_cuda:
+    index = logits.get_device()
+    if index < 0:
         _require_cuda(logits)
-    dtype = _DTYPES.get(logits.dtype)
-    if dtype is None or logits.dim() != 2 or logits.stride(1) != 1:
+    dtype, size, ld = _DTYPES.get(logits.dtype), logits.size(), logits.stride()
+    if dtype is None or len(size) != 2 or ld[1] != 1:
         raise TwmError(_lib.TWM_EINVAL, "sample: logits must be a float32, float16 or bfloat16 matrix with contiguous rows")
-    rows, vocab, index, f32, i32 = logits.size(0), logits.size(1), logits.get_device(), torch.float32, torch.int32
+    (rows, vocab), f32, i32 = size, torch.float32, torch.int32
     if rows == 0:
         return
     if torch._C._cuda_getDevice() != index:
         with torch.cuda.device(index):
             return sample(logits, random, tokens, temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p, prob=prob, stream=stream, flags=flags)
-    args = _lib.SampleArgs(rows, vocab, dtype, logits.data_ptr(), logits.stride(0) if rows > 1 else vocab, _column("random", random, f32, rows, index),
-                           _column("temperature", temperature, f32, rows, index), _column("top_k", top_k, i32, rows, index),
-                           _column("top_p", top_p, f32, rows, index), _column("min_p", min_p, f32, rows, index),
-                           _column("tokens", tokens, i32, rows, index), _column("prob", prob, f32, rows, index))
+    args = _lib.pack_sample_args(rows, vocab, dtype, logits.data_ptr(), ld[0] if rows > 1 else vocab, _column("random", random, f32, rows, index),
+                                 _column("temperature", temperature, f32, rows, index), _column("top_k", top_k, i32, rows, index),
+                                 _column("top_p", top_p, f32, rows, index), _column("min_p", min_p, f32, rows, index),
+                                 _column("tokens", tokens, i32, rows, index), _column("prob", prob, f32, rows, index), 0, 0, 0, 0, 0, 0)
     status = _lib.lib().twm_sample(args, flags, _stream_ptr(stream))
     if status:
         check(status, "twm_sample")

@@ -198,7 +198,7 @@ def test_decode_loop_form():
                            history.data_ptr(), 3, pos.data_ptr(), length.data_ptr())
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
-        _lib.check(_lib.lib().twm_sample(args, _lib.TWM_FLAG_PDL, torch.cuda.current_stream().cuda_stream), "twm_sample")
+        _lib.check(_lib.lib().twm_sample(_lib.C.addressof(args), _lib.TWM_FLAG_PDL, torch.cuda.current_stream().cuda_stream), "twm_sample")
     want = [chosen(logits[0].double().cpu().numpy(), float(u[min(i, 2)]), 1.0)[0] for i in range(steps)]
     for i in range(steps):
         graph.replay()

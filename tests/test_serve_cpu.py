@@ -15,13 +15,14 @@ def cache(**kw):
 
 
 def append(lib, c, q=0x1000, ldq=1024, qkv=0x2000, ldqkv=2048, bias=None, rope=None, heads=8, rows=2, row_start=None, max_rows=1, start=0x3000):
-    return lib.twm_cache8_append(C.addressof(c) if c is not None else None, q, ldq, qkv, ldqkv, bias, rope, heads, rows, row_start, max_rows, start, 0, None)
+    args = _lib.Cache8AppendArgs(q, ldq, qkv, ldqkv, bias, rope, heads, rows, max_rows, row_start, start)
+    return lib.twm_cache8_append(C.addressof(c) if c is not None else None, C.addressof(args), 0, None)
 
 
 def attention(lib, c, out=0x1000, ldo=1024, q=0x2000, ldq=1024, heads=8, rows=2, row_start=None, max_rows=1, start=0x3000, scale=0.1, window=0, ws=0x4000,
               nbytes=1 << 40):
-    return lib.twm_cache8_attention(C.addressof(c) if c is not None else None, out, ldo, q, ldq, heads, rows, row_start, max_rows, start, scale, window, ws,
-                                    nbytes, 0, None)
+    args = _lib.Cache8AttentionArgs(out, ldo, q, ldq, heads, rows, max_rows, window, row_start, start, ws, nbytes, scale)
+    return lib.twm_cache8_attention(C.addressof(c) if c is not None else None, C.addressof(args), 0, None)
 
 
 BAD_CACHES = [dict(seqs=0), dict(seqs=65536), dict(kv_heads=0), dict(head_dim=96), dict(head_dim=0), dict(capacity=100), dict(capacity=0), dict(k=None), dict(v=None),
@@ -51,11 +52,16 @@ def test_other_refusals(twm_lib):
         assert append(twm_lib, cache(), **bad) == _lib.TWM_EINVAL, bad
     for bad in (dict(qkv=0x2002), dict(ldqkv=2052), dict(bias=0x7004), dict(rope=0x7008)):
         assert append(twm_lib, cache(), **bad) == _lib.TWM_EALIGN, bad
-    for bad in (dict(out=None), dict(ldo=1000), dict(scale=0.0), dict(scale=-1.0), dict(scale=float("nan")), dict(window=-1), dict(ws=None)):
+    for bad in (dict(out=None), dict(ldo=1000), dict(scale=0.0), dict(scale=-1.0), dict(scale=float("nan")), dict(scale=float("inf")), dict(window=-1), dict(ws=None)):
         assert attention(twm_lib, cache(), **bad) == _lib.TWM_EINVAL, bad
     for bad in (dict(out=0x1001), dict(ldo=1028), dict(ws=0x4008)):
         assert attention(twm_lib, cache(), **bad) == _lib.TWM_EALIGN, bad
     assert attention(twm_lib, cache(), nbytes=8) == _lib.TWM_EWORKSPACE
+
+
+def test_no_arguments(twm_lib):
+    assert twm_lib.twm_cache8_append(C.addressof(cache()), None, 0, None) == _lib.TWM_EINVAL
+    assert twm_lib.twm_cache8_attention(C.addressof(cache()), None, 0, None) == _lib.TWM_EINVAL
 
 
 def test_workspace_sizes(twm_lib):
@@ -75,8 +81,8 @@ def test_sampling_that_is_refused(twm_lib):
     loop = dict(step=0x4000, random_count=3, pos=0x5000, len=0x6000)
     for bad in (dict(rows=0), dict(vocab=0), dict(vocab=(1 << 20) + 1, ld=1 << 21), dict(dtype=3), dict(logits=None), dict(ld=99), dict(random=None), dict(tokens=None),
                 dict(loop, rows=2), dict(loop, random_count=0), dict(loop, pos=None), dict(loop, len=None), dict(loop, history=0x7000, history_capacity=0)):
-        assert twm_lib.twm_sample(sample_args(**bad), 0, None) == _lib.TWM_EINVAL, bad
-    assert twm_lib.twm_sample(sample_args(logits=0x1002), 0, None) == _lib.TWM_EALIGN
+        assert twm_lib.twm_sample(C.addressof(sample_args(**bad)), 0, None) == _lib.TWM_EINVAL, bad
+    assert twm_lib.twm_sample(C.addressof(sample_args(logits=0x1002)), 0, None) == _lib.TWM_EALIGN
 
 
 def test_host_tensors_are_refused():
