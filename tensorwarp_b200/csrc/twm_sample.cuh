@@ -5,7 +5,8 @@
 // kept; that border is found by histograms, narrowing in on the bin it lies in:
 //   level 0   bins of 1/8 octave of weight below the largest logit's, 512 of them (what is beyond, 2^-64, is one more bin);
 //   then      512 equal parts, as ordered integers, of the logits of the bin that the border lies in, and of the part again;
-// and once 32 tokens or fewer are left they are ordered by one warp.  Which logits a bin of level 0 has is found by searching its ends, so that
+// and once 32 tokens or fewer are left they are ordered by one warp.  Where those of level 0's bin and all ahead of it are 128 at most, as for a small
+// top-k or a sharp row, they go to the first CTA, which orders them and does the rest alone.  Which logits a bin of level 0 has is found by searching its ends, so that
 // all passes but the first only compare.  A bin holds its number of tokens and its mass.  Within a bin weights are
 // within 2^(1/8) of its largest W: mass = W (count - sum of delta), delta = 1 - w / W in fixed point, so that both are integer sums, the
 // same in any order: the result does not depend on which thread comes first.
@@ -37,6 +38,7 @@ __device__ __forceinline__ uint32_t order_of(float v)
 __device__ __forceinline__ float value_of(uint32_t o) { return __uint_as_float(o & 0x80000000u ? o & 0x7fffffffu : ~o); }
 
 constexpr int THREADS = 512, WARPS = THREADS / 32, BINS = THREADS, MAX_CTAS = 16, FEW = 32;
+constexpr int ALL = 128;                 // tokens that the first CTA orders by itself
 constexpr int MAX_SLICE = 40960;         // logits of a CTA in shared memory; what is beyond is read again
 
 __device__ __forceinline__ void st_cluster_u32(uint32_t at, uint32_t v) { asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(at), "r"(v) : "memory"); }
@@ -68,6 +70,13 @@ struct Weights {
     __device__ __forceinline__ float of(float v) const { return v == top ? 1.0f : of_finite(v); }
 };
 
+__device__ __forceinline__ uint32_t count_cluster(uint32_t at)          // adds one to a counter and gives what it was
+{
+    uint32_t v;
+    asm volatile("atom.shared::cluster.add.u32 %0, [%1], 1;" : "=r"(v) : "r"(at) : "memory");
+    return v;
+}
+
 struct Shared {
     uint32_t count[BINS], delta[BINS];                   // this CTA's, as it counts
     uint32_t all_count[BINS];                            // the cluster's
@@ -81,6 +90,11 @@ struct Shared {
     uint32_t cta_ties[MAX_CTAS];
     unsigned long long cta_above[MAX_CTAS];
     uint32_t list_n[2], list[2][FEW];                    // the last tokens of top-k's border, of top-p's
+    uint32_t own_n;                                      // the slice's logits in the border's bin, if a thread has one at most
+    float own[THREADS];
+    uint32_t all_n, all_key[ALL], all_index[ALL];        // the first CTA's: all tokens down to the end of the border's bin
+    uint32_t key[ALL], index[ALL], kept;                 // ... in order
+    unsigned long long weight[ALL];
     uint32_t found_bin, found_count, found_over;
     double found_over_mass;
     uint32_t cut, ties;
@@ -139,6 +153,7 @@ sample_kernel(const __grid_constant__ twm_sample_args a, int slice, int ctas)
     const int n = a.vocab, n0 = min(n, rank * slice), ns = min(n - n0, slice);
     for (int i = tid; i < BINS; i += THREADS) sh.count[i] = sh.delta[i] = 0;
     if (tid < 2) sh.list_n[tid] = 0;
+    if (tid == 0) sh.all_n = 0;
     pdl_wait_prior_grids();
     const T* logits = reinterpret_cast<const T*>(a.logits) + (size_t)row * a.ld + n0;
     const float t = a.temperature ? a.temperature[row] : 1.0f;
@@ -190,6 +205,21 @@ sample_kernel(const __grid_constant__ twm_sample_args a, int slice, int ctas)
     key = 0;
     for (int c = 0; c < ctas; ++c) key = max(key, sh.cta_max[c]);
     mx = value_of(key);
+
+    constexpr float ONE = 4398046511104.0f;              // 2^42
+    auto answer = [&](int token, float prob) {           // by one thread of the cluster
+        a.tokens[row] = token;
+        if (a.prob) a.prob[row] = prob;
+        if (a.step) {
+            const int step = a.step[0];
+            if (a.history && step >= 0 && step < a.history_capacity) a.history[step] = token;
+            a.step[0] = step + 1;
+            a.pos[0] += 1;
+            a.len[0] += 1;
+        }
+    };
+    // the lowest key that min_p keeps
+    auto least_key = [&]() { return mp > 0.0f ? order_of(__double2float_ru((double)mx + (double)t * log(fmin((double)mp, 1.0))) + 0.0f) : 0u; };
 
     uint32_t cut = 0, ties = 0x7fffffffu;                // kept: keys over cut, and the first `ties` of those that are cut
     Weights weights = {mx, 0.0f, 0.0f};
@@ -250,6 +280,80 @@ sample_kernel(const __grid_constant__ twm_sample_args a, int slice, int ctas)
             const Scan first = scan(sh, c0, m0);
             double mass = first.mass_all;                    // of what top-k keeps
 
+            // All tokens from key `lo` on, n of them, to the first CTA, which orders them by value and index: top-k, top-p and min-p all keep a head of
+            // that order.  A token's running sum is that of the kept ones with lower indexes.
+            auto finish_alone = [&](uint32_t lo, uint32_t n_all, bool need_k, double mass) {
+                const float f_lo = value_of(lo);
+                const uint32_t to_n = mapa_shared(smem_u32(&sh.all_n), 0), to_key = mapa_shared(smem_u32(sh.all_key), 0), to_index = mapa_shared(smem_u32(sh.all_index), 0);
+                auto offer = [&](float v, int i) {
+                    if (v >= f_lo) {
+                        const uint32_t slot = count_cluster(to_n);
+                        if (slot < ALL) { st_cluster_u32(to_key + 4 * slot, order_of(v)); st_cluster_u32(to_index + 4 * slot, (uint32_t)(n0 + i)); }
+                    }
+                };
+                for (int i = tid; i < quads; i += THREADS) {
+                    const float4 q = reinterpret_cast<const float4*>(vals)[i];
+                    if (fmaxf(fmaxf(q.x, q.y), fmaxf(q.z, q.w)) >= f_lo) { offer(q.x, 4 * i); offer(q.y, 4 * i + 1); offer(q.z, 4 * i + 2); offer(q.w, 4 * i + 3); }
+                }
+                for (int i = held + tid; i < ns; i += THREADS) offer(plain(logit_f32(logits[i])), i);
+                cluster_sync_all();
+                if (rank != 0) return;
+                const int m = (int)min(n_all, (uint32_t)ALL);
+                if (tid < m) {
+                    const uint32_t mine = sh.all_key[tid], index = sh.all_index[tid];
+                    int place = 0;
+                    for (int j = 0; j < m; ++j) place += sh.all_key[j] > mine || (sh.all_key[j] == mine && sh.all_index[j] < index);
+                    sh.key[place] = mine;
+                    sh.index[place] = index;
+                }
+                __syncthreads();
+                if (warp == 0) {
+                    constexpr int EACH = ALL / 32;
+                    float w[EACH];
+                    double upto = 0.0;
+                    const int n_k = need_k ? min(m, k) : m;
+#pragma unroll
+                    for (int j = 0; j < EACH; ++j) {
+                        const int i = lane * EACH + j;
+                        w[j] = i < m ? weights.of(value_of(sh.key[i])) : 0.0f;
+                        if (i < n_k) upto += (double)w[j];
+                        if (i < m) sh.weight[i] = __float2ull_rn(w[j] * ONE);
+                    }
+                    const double own = upto;
+#pragma unroll
+                    for (int o = 1; o < 32; o <<= 1) {
+                        const double x = __shfl_up_sync(0xffffffffu, upto, o);
+                        if (lane >= o) upto += x;
+                    }
+                    if (need_k) mass = __shfl_sync(0xffffffffu, upto, 31);
+                    const double want = (double)p * mass;
+                    const uint32_t least = least_key();
+                    double before = upto - own;
+                    int kept = 0;
+#pragma unroll
+                    for (int j = 0; j < EACH; ++j) {
+                        const int i = lane * EACH + j;
+                        kept += i < n_k && (i == 0 || ((!need_p || before < want) && sh.key[i] >= least));
+                        before += (double)w[j];
+                    }
+                    kept = __reduce_add_sync(0xffffffffu, kept);
+                    if (lane == 0) sh.kept = kept;
+                }
+                __syncthreads();
+                const int kept = (int)sh.kept;
+                if (tid < kept) {
+                    const uint32_t index = sh.index[tid];
+                    unsigned long long before = 0, total = 0;
+                    for (int j = 0; j < kept; ++j) {
+                        total += sh.weight[j];
+                        if (sh.index[j] < index) before += sh.weight[j];
+                    }
+                    const unsigned long long target = min((unsigned long long)(fmin(fmax((double)random, 0.0), 1.0) * (double)total), total - 1);
+                    if (before <= target && target < before + sh.weight[tid])
+                        answer((int)index, (float)((double)weights.of(value_of(sh.key[tid])) * (double)ONE / (double)total));
+                }
+            };
+
             for (int what = need_k ? 0 : 1; what <= (need_p ? 1 : 0); ++what) {
                 const double want = fmax((double)p * mass, 1e-30);       // of mass, for top-p
                 // The bin with the border, from this thread's: the first whose end reaches what is wanted; the last one with tokens if rounding keeps
@@ -308,11 +412,38 @@ sample_kernel(const __grid_constant__ twm_sample_args a, int slice, int ctas)
                 }
                 __syncthreads();
                 uint32_t hi = sh.ends[0], lo = sh.ends[1] + 1;
+                if (bin < BINS && over + left <= ALL && !(what == 1 && need_k)) {
+                    finish_alone(lo, over + left, need_k, mass);
+                    return;
+                }
+                // the logits that are left of this slice, one a thread, where there are so few
+                const bool many = left > FEW && lo < hi;
+                if (many) {
+                    if (tid == 0) sh.own_n = 0;
+                    __syncthreads();
+                    const float f_lo = value_of(lo), f_hi = value_of(hi);
+                    each([&](float v) {
+                        if (v >= f_lo && v <= f_hi) {
+                            const uint32_t slot = atomicAdd(&sh.own_n, 1u);
+                            if (slot < THREADS) sh.own[slot] = v;
+                        }
+                    });
+                    __syncthreads();
+                }
+                const uint32_t own_n = many ? sh.own_n : THREADS + 1;
+                auto each_left = [&](auto f) {                   // f for those of [lo, hi]
+                    const float f_lo = value_of(lo), f_hi = value_of(hi);
+                    if (own_n <= THREADS) {
+                        if (tid < own_n && sh.own[tid] >= f_lo && sh.own[tid] <= f_hi) f(sh.own[tid]);
+                    } else {
+                        each([&](float v) { if (v >= f_lo && v <= f_hi) f(v); });
+                    }
+                };
                 while (left > FEW && lo < hi) {
                     const int shift = max(0, 23 - __clz(hi - lo));               // (hi - lo) >> shift < 512
-                    const float w_top = weights.of(value_of(hi)), back = 1.0f / w_top, f_lo = value_of(lo), f_hi = value_of(hi);
-                    each([&](float v) {                          // beyond the bins mass does not count
-                        if (v >= f_lo && v <= f_hi) count((int)((hi - order_of(v)) >> shift), bin < BINS ? fmaxf(fmaf(-weights.of(v), back, 1.0f), 0.0f) : 0.0f);
+                    const float w_top = weights.of(value_of(hi)), back = 1.0f / w_top;
+                    each_left([&](float v) {                     // beyond the bins mass does not count
+                        count((int)((hi - order_of(v)) >> shift), bin < BINS ? fmaxf(fmaf(-weights.of(v), back, 1.0f), 0.0f) : 0.0f);
                     });
                     join();
                     const uint32_t x = sh.all_count[tid];
@@ -333,12 +464,9 @@ sample_kernel(const __grid_constant__ twm_sample_args a, int slice, int ctas)
                     mass = over_mass + (double)border_ties * w;
                 } else {
                     // the last ones, put in order by a warp of every CTA
-                    const float f_lo = value_of(lo), f_hi = value_of(hi);
-                    each([&](float v) {
-                        if (v >= f_lo && v <= f_hi) {
-                            const uint32_t slot = atomicAdd(&sh.list_n[what], 1u);
-                            if (slot < FEW) sh.list[what][slot] = order_of(v);
-                        }
+                    each_left([&](float v) {
+                        const uint32_t slot = atomicAdd(&sh.list_n[what], 1u);
+                        if (slot < FEW) sh.list[what][slot] = order_of(v);
                     });
                     cluster_sync_all();
                     if (warp == 0) {
@@ -394,15 +522,12 @@ sample_kernel(const __grid_constant__ twm_sample_args a, int slice, int ctas)
                 }
             }
         }
-        if (mp > 0.0f) {
-            const uint32_t least = order_of(__double2float_ru((double)mx + (double)t * log(fmin((double)mp, 1.0))) + 0.0f);
-            if (least > cut) { cut = least; ties = 0x7fffffffu; }
-        }
+        const uint32_t least = least_key();
+        if (least > cut) { cut = least; ties = 0x7fffffffu; }
     }
 
     // ---- running sums by index: neighbouring tokens a thread.  Weights as integers, 2^42 the largest:
     // the threads' sums add up exactly, in any order, so that exactly one thread has the token. ----
-    constexpr float ONE = 4398046511104.0f;
     const int per = 4 * (((ns + 4 * THREADS - 1) / (4 * THREADS)) | 1), i0 = min(ns, tid * per), i1 = min(ns, i0 + per);
     const float f_cut = cut < order_of(-INFINITY) ? -INFINITY : value_of(cut);       // all are over 0, but -inf weighs nothing
     float sum = 0.0f;                                    // of a thread's, in FP32, always in the same order
@@ -465,15 +590,7 @@ sample_kernel(const __grid_constant__ twm_sample_args a, int slice, int ctas)
             else if (v == f_cut && same_upto < ties) { ++same_upto; w = w_cut; }
             if (upto + __float2ull_rn(sum * ONE) + one_tie * min(same_upto, ties) > target) break;
         }
-        a.tokens[row] = n0 + i;
-        if (a.prob) a.prob[row] = (float)((double)w * (double)ONE / (double)total);
-        if (a.step) {
-            const int step = a.step[0];
-            if (a.history && step >= 0 && step < a.history_capacity) a.history[step] = n0 + i;
-            a.step[0] = step + 1;
-            a.pos[0] += 1;
-            a.len[0] += 1;
-        }
+        answer(n0 + i, (float)((double)w * (double)ONE / (double)total));
     }
 }
 
