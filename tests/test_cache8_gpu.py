@@ -389,3 +389,69 @@ def test_rows_said_wrongly_stay_inside():
         qkv = torch.randn((8, 512), generator=b.gen, device="cuda").half()
         cache8.append(b.cache, qkv, buf[:8], ints([100, -1, 90]), num_heads=4, row_start=ints(rows), max_rows=2)
         assert bool((buf[8:] == 7.0).all())
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim,rows", [(7, 1, 128, 1), (12, 1, 64, 1), (4, 1, 64, 3), (4, 1, 128, 30)])
+def test_many_sequences(heads, kv_heads, dim, rows):
+    """More sequences than warps look at by themselves, some of them out of the call or without a row."""
+    seqs = 300
+    b = Batch(seqs, 192, heads, kv_heads, dim)
+    lengths = [rows + 7 * s % (192 - rows + 1) for s in range(seqs)]
+    b.append([0] * seqs, lengths)
+    counts = [0 if s % 11 == 5 else 1 + s % rows for s in range(seqs)]
+    b.attend([-1 if s % 13 == 3 else n - c for s, (n, c) in enumerate(zip(lengths, counts))], counts, pad=1)
+
+
+@pytest.mark.parametrize("rows", [1, 3, 70])
+def test_up_to_the_capacity(rows):
+    """The last places of a full cache, rows of which some or all lie behind them, and a sequence that stands past the end."""
+    b = Batch(3, 256, 8, 2, 128)
+    b.append([0, 0, 0], [256, 256, 256])
+    b.attend([256 - rows] * 3, [rows] * 3)
+    q = 2 * torch.randn((3 * rows, 1024), generator=b.gen, device="cuda").half()
+    out = torch.full_like(q, 7.0)
+    starts, row_start = [256 - rows // 2, 256, 1 << 30], ints([0, rows, 2 * rows, 3 * rows])
+    cache8.attention(b.cache, q, out, ints(starts), num_heads=8, row_start=row_start, max_rows=rows)
+    assert bool((out[rows // 2:] == 7.0).all())
+    if rows > 1:
+        want, off = ref.attention(q[:rows // 2], *b.held.held(0, 256), starts[0], 8, 1 / math.sqrt(128), 0)
+        assert bool(((out[:rows // 2].double() - want).abs() <= off).all())
+    before = [t.clone() for t in (b.cache.k.view(torch.uint8), b.cache.v.view(torch.uint8), b.cache.k_tail, b.cache.v_tail)]
+    qkv = torch.randn((3 * rows, b.width), generator=b.gen, device="cuda").half()
+    cache8.append(b.cache, qkv, out, ints([256, 256, 1 << 30]), num_heads=8, row_start=row_start, max_rows=rows)
+    assert all(torch.equal(x, t) for x, t in zip(before, (b.cache.k.view(torch.uint8), b.cache.v.view(torch.uint8), b.cache.k_tail, b.cache.v_tail)))
+
+
+@pytest.mark.parametrize("rows", [1, 2, 9])
+def test_more_query_heads_than_rows_of_a_tile(rows):
+    b = Batch(2, 320, 300, 1, 64)
+    b.append([0, 0], [200, 31])
+    b.attend([200 - rows, 31 - rows], [rows, rows])
+    b.attend([200 - rows, 31 - rows], [rows, rows], window=(1 << 31) - 1)
+
+
+def test_two_captured_calls_at_once():
+    """Two graphs with workspaces of their own, of few rows and of many, run on two streams together."""
+    b = Batch(4, 2048, 16, 4, 128)
+    b.append([0] * 4, [2000, 1500, 1999, 700])
+    calls = []
+    for rows in (1, 64):
+        start, row_start = ints([2000 - rows, 1500 - rows, 1999 - rows, 700 - rows]), ints([rows * s for s in range(5)])
+        q = 2 * torch.randn((4 * rows, 2048), generator=b.gen, device="cuda").half()
+        for _ in range(2):
+            out, ws = torch.zeros_like(q), cache8.Workspace.for_cache(b.cache, 16, rows)
+            graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+            side.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.graph(graph, stream=side):
+                for _ in range(3):
+                    cache8.attention(b.cache, q, out, start, num_heads=16, row_start=row_start, max_rows=rows, workspace=ws, flags=_lib.TWM_FLAG_PDL)
+            want = torch.zeros_like(q)
+            cache8.attention(b.cache, q, want, start, num_heads=16, row_start=row_start, max_rows=rows)
+            calls.append((graph, side, out, want))
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for graph, side, _, _ in calls:
+            with torch.cuda.stream(side):
+                graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(out, want) for _, _, out, want in calls)

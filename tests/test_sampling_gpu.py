@@ -217,3 +217,30 @@ def test_other_stream():
     side.synchronize()
     sampling.sample(logits, u, here, top_p=f32([0.9] * 9))
     assert torch.equal(tokens, here)
+
+
+@pytest.mark.parametrize("vocab", [655361, 700001, 1 << 20])
+def test_largest_vocabularies(vocab):
+    """Rows of which a CTA's slice does not fit its shared memory."""
+    g = gen("largest", vocab)
+    pick = [SETTINGS[i] for i in (0, 4, 5, 8, 10, 13, 15)]
+    logits = 3.0 * torch.randn((len(pick), vocab), generator=g, device="cuda")
+    verify(logits, torch.rand(len(pick), generator=g, device="cuda"), f32([s.get("temperature", 1.0) for s in pick]), i32([s.get("top_k", 0) for s in pick]),
+           f32([s.get("top_p", 1.0) for s in pick]), f32([s.get("min_p", 0.0) for s in pick]))
+
+
+def test_two_calls_at_once():
+    g = gen("two")
+    logits = [3.0 * torch.randn((150, 50000), generator=g, device="cuda") for _ in range(2)]
+    u, p = torch.rand(150, generator=g, device="cuda"), f32([0.9] * 150)
+    want = [torch.zeros(150, dtype=torch.int32, device="cuda") for _ in range(2)]
+    got = [torch.zeros(150, dtype=torch.int32, device="cuda") for _ in range(2)]
+    for x, t in zip(logits, want):
+        sampling.sample(x, u, t, top_p=p)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for x, t, s in zip(logits, got, streams):
+            sampling.sample(x, u, t, top_p=p, stream=s)
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, y) for x, y in zip(want, got))
