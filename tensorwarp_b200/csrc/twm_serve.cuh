@@ -1,6 +1,7 @@
 // twm_serve.cuh — argument checks and launches of include/twm_serve.h.  Part of twmarlin.cu's translation unit.
 #pragma once
 
+#include <atomic>
 #include <climits>
 #include <cmath>
 
@@ -56,22 +57,18 @@ bool make_codes_map(CUtensorMap* map, const twm_cache8* c, void* codes)
                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// Lets a kernel take more than 48 KB of shared memory on the current device.  The limit belongs to the function: it is set once a device, to what
-// every launch of it asks for.
-twm_status allow_shared(const char* name, const void* kernel, size_t bytes)
+// Lets a kernel take more than 48 KB of shared memory on the current device.  The limit belongs to the function: it is set once a device (`done`, a
+// bit each), to what every launch of it asks for.
+twm_status allow_shared(const char* name, const void* kernel, size_t bytes, std::atomic<unsigned long long>& done)
 {
-    static std::mutex mutex;
-    static std::vector<std::pair<const void*, int>> done;
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
+    if (e == cudaSuccess && dev < 64 && (done.load() >> dev & 1)) return TWM_OK;
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
     if (e == cudaSuccess) {
-        std::lock_guard<std::mutex> lock(mutex);
-        for (const auto& x : done)
-            if (x.first == kernel && x.second == dev) return TWM_OK;
-        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
-        if (e == cudaSuccess) done.emplace_back(kernel, dev);
+        if (dev < 64) done |= 1ULL << dev;
+        return TWM_OK;
     }
-    if (e == cudaSuccess) return TWM_OK;
     set_error(name, e);
     return TWM_ELAUNCH;
 }
@@ -81,7 +78,8 @@ twm_status launch_few(const twm::cache8::AttnArgs& a, const AttnPlan& p, int fla
 {
     auto* kernel = twm::cache8::few_kernel<D, NT>;
     constexpr size_t smem = twm::cache8::Few<D, NT>::SMEM;
-    const twm_status st = allow_shared("twm_cache8_attention", (const void*)kernel, smem);
+    static std::atomic<unsigned long long> done{0};
+    const twm_status st = allow_shared("twm_cache8_attention", (const void*)kernel, smem, done);
     if (st != TWM_OK) return st;
     return launch_op("twm_cache8_attention", kernel, dim3(p.ctas), dim3(twm::cache8::FEW_THREADS), smem, flags, stream, a);
 }
@@ -92,7 +90,8 @@ twm_status launch_prompt(const twm::cache8::AttnArgs& a, const AttnPlan& p, int 
     auto* kernel = twm::cache8::prompt_kernel<D>;
     constexpr size_t smem = twm::cache8::Prompt<D>::SMEM;
     static_assert(smem + 1024 < 227 * 1024, "shared memory of a CTA");
-    const twm_status st = allow_shared("twm_cache8_attention", (const void*)kernel, smem);
+    static std::atomic<unsigned long long> done{0};
+    const twm_status st = allow_shared("twm_cache8_attention", (const void*)kernel, smem, done);
     if (st != TWM_OK) return st;
     return launch_op("twm_cache8_attention", kernel, dim3(p.ctas), dim3(twm::cache8::PROMPT_THREADS), smem, flags, stream, a);
 }
