@@ -17,6 +17,8 @@ def _generate(args) -> int:
     if args.kv_cache:
         options["kv_cache"] = args.kv_cache
     sampling = None
+    if args.temperature is None and (args.top_k, args.top_p, args.min_p) != (0, 1.0, 0.0):
+        raise SystemExit("generate: --top-k, --top-p and --min-p want a --temperature")
     if args.temperature is not None:
         from .sampling import SamplingParams
         sampling = [SamplingParams(args.temperature, args.top_k, args.top_p, args.min_p, args.seed + i) for i in range(len(args.tokens))]

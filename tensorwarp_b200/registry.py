@@ -41,7 +41,7 @@ def builder_for(config: dict) -> Callable:
 
 
 def load(folder: str, **options):
-    """An engine for the checkpoint in `folder` (options: dtype, max_tokens, max_live, portion, device)."""
+    """An engine for the checkpoint in `folder` (options: dtype, max_tokens, max_live, portion, device; kv_cache of the 4-bit decoder)."""
     config = checkpoint.read_config(folder)
     builder = builder_for(config)
     path = os.path.join(folder, "model.safetensors")

@@ -158,3 +158,9 @@ def test_command_line_takes_settings():
         main(["generate", "--model", "/nowhere", "--tokens", "1", "--temperature", "-1"])
     with pytest.raises(SystemExit):
         main(["generate", "--model", "/nowhere", "--tokens", "1", "--kv-cache", "int4"])
+
+
+def test_command_line_refuses_cuts_without_a_temperature():
+    from tensorwarp_b200.__main__ import main
+    with pytest.raises(SystemExit):
+        main(["generate", "--model", "/nowhere", "--tokens", "1", "--top-p", "0.9"])
