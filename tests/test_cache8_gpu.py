@@ -455,3 +455,26 @@ def test_two_captured_calls_at_once():
                 graph.replay()
     torch.cuda.synchronize()
     assert all(torch.equal(out, want) for _, _, out, want in calls)
+
+
+@pytest.mark.parametrize("rows", [1, 30])
+def test_append_in_place(rows):
+    """The rotated queries over those of the fused projection."""
+    b = Batch(2, 128, 8, 2, 128)
+    qkv = b.make(2 * rows).half()
+    want, place, row_start = torch.zeros((2 * rows, 1024), dtype=torch.float16, device="cuda"), qkv.clone(), ints([0, rows, 2 * rows])
+    kw = dict(num_heads=8, row_start=row_start, max_rows=rows, bias=b.bias, rope=b.rope)
+    cache8.append(b.cache, qkv, want, ints([0, 0]), **kw)
+    cache8.append(b.cache, place, place[:, :1024], ints([0, 0]), **kw)
+    assert torch.equal(place[:, :1024], want) and torch.equal(place[:, 1024:], qkv[:, 1024:])
+
+
+def test_calls_without_rows():
+    b = Batch(2, 128, 8, 2, 64)
+    b.append([0, 0], [70, 3])
+    none = torch.zeros((0, b.width), dtype=torch.float16, device="cuda")
+    cache8.append(b.cache, none, none[:, :512], ints([70, 3]), num_heads=8, row_start=ints([0, 0, 0]))
+    cache8.attention(b.cache, none[:, :512], none[:, :512], ints([70, 3]), num_heads=8, row_start=ints([0, 0, 0]))
+    b.held.check(b.cache)
+    with pytest.raises(_lib.TwmError):
+        cache8.attention(b.cache, none[:, :512], none[:, :512], ints([70, 3]), num_heads=8)
