@@ -447,14 +447,14 @@ def test_two_captured_calls_at_once():
                     cache8.attention(b.cache, q, out, start, num_heads=16, row_start=row_start, max_rows=rows, workspace=ws, flags=_lib.TWM_FLAG_PDL)
             want = torch.zeros_like(q)
             cache8.attention(b.cache, q, want, start, num_heads=16, row_start=row_start, max_rows=rows)
-            calls.append((graph, side, out, want))
+            calls.append((graph, side, out, want, (start, row_start, q, ws)))      # a graph does not keep what it uses
     torch.cuda.synchronize()
     for _ in range(20):
-        for graph, side, _, _ in calls:
+        for graph, side, *_ in calls:
             with torch.cuda.stream(side):
                 graph.replay()
     torch.cuda.synchronize()
-    assert all(torch.equal(out, want) for _, _, out, want in calls)
+    assert all(torch.equal(out, want) for _, _, out, want, _ in calls)
 
 
 @pytest.mark.parametrize("rows", [1, 30])
