@@ -57,6 +57,7 @@ __device__ __forceinline__ Tile tile_units(const Span& sp, int t, int tile, int 
 // A tile also takes time of its own, `extra` units' worth, which stand ahead of its units in the line.
 struct Deal {
     int group, tile, window, extra;
+    int least;                   // units of a CTA at least
     __device__ __forceinline__ int tiles(const Span& sp) const { return sp.n * group <= tile ? 1 : (sp.n * group + tile - 1) / tile; }
     __device__ __forceinline__ int units(const Span& sp, int t) const
     {
@@ -123,7 +124,7 @@ __device__ __forceinline__ Start find_start(const AttnArgs& a, const Deal& deal,
         total += sums[w];
     }
     upto += base;
-    const long long share = max(1LL, quotient(total + ctas - 1, ctas)), begin = min(total, share * cta), end = min(total, begin + share);
+    const long long share = max((long long)deal.least, quotient(total + ctas - 1, ctas)), begin = min(total, share * cta), end = min(total, begin + share);
     if (begin < end && upto - mine <= begin && begin < upto) {           // the same in all lanes of a warp where warps take sequences
         long long at = upto - mine;
         for (int s = s0; s < s1; ++s) {
@@ -209,7 +210,7 @@ struct Walk {
 };
 
 // The same where every sequence has one tile and there are at most 128 of them: every warp finds the start by itself, a few neighbouring sequences
-// a lane, in 32 bits (units of all sequences: cached rows / 64, and one tile more each).  2.3 + 1.0 thousand clocks of a call for one sequence
+// a lane, in 32 bits (units of all sequences: cached rows / 64, and a tile's extra each).  2.3 + 1.0 thousand clocks of a call for one sequence
 // with find_start and begin, 1.5 + 0.15 thousand this way.
 constexpr int START_BY_WARP = 128;
 __device__ __forceinline__ bool begin_by_warp(const AttnArgs& a, const Deal& d, int cta, int ctas, Start& start, Walk& w)
@@ -228,7 +229,7 @@ __device__ __forceinline__ bool begin_by_warp(const AttnArgs& a, const Deal& d, 
         const int v = __shfl_up_sync(0xffffffffu, upto, o);
         if (lane >= o) upto += v;
     }
-    const int total = __shfl_sync(0xffffffffu, upto, 31), share = max(1, (total + ctas - 1) / ctas);
+    const int total = __shfl_sync(0xffffffffu, upto, 31), share = max(d.least, (total + ctas - 1) / ctas);
     const int begin = (int)min((long long)share * cta, (long long)total), end = min(total, begin + share);
     start = {__any_sync(0xffffffffu, out) != 0, end - begin, share, 0, 0};
     if (begin >= end) return false;
@@ -279,7 +280,7 @@ __device__ __forceinline__ int exponent_of(float scale) { return (int)(__float_a
 
 // --------------------------------------------------------------------------------------------- few rows a sequence --
 // Up to 8 NT rows a sequence and key/value head (the query heads that share it, times the new tokens): they are one tile, and every key is
-// read once.  Bound by HBM.  Four consumer warps take 16 keys each of a unit; a producer warp brings units by TMA into a ring that runs on over
+// read once.  Bound by HBM (96 sequences of up to 6000 tokens, 28 heads on 4: 121 us, 6.0 TB/s).  Four consumer warps take 16 keys each of a unit; a producer warp brings units by TMA into a ring that runs on over
 // the borders of tiles, the tail's FP16 rows among them (keys and values in a stage each).  S^T = K Q^T and O^T += V^T P^T as mma.m16n8k16 with
 // the keys, and then the head's elements, as the 16 rows, so that eight rows of queries are a whole operand.  Elements and keys may stand in any
 // order in a sum: lane (g, t) takes D / 4 elements of keys g and g + 8 for the scores (4 codes a k-step of both registers), and D / 8 elements of
@@ -287,6 +288,7 @@ __device__ __forceinline__ int exponent_of(float scale) { return (int)(__float_a
 // layout that the TMA's swizzle leaves.  P^T needs only a transposition of 8 x 8.  Each warp has its own m; when the tile ends the four add up in
 // shared memory, while the next tile's queries are on their way.
 constexpr int FEW_EXTRA = 4;                                             // a tile's own time, in units (96 sequences: 1 124.5 us, 2 121.9, 4 120.8)
+constexpr int FEW_LEAST = 1;                                             // units of a CTA at least (2049 tokens, 28 heads: 1 9.2 us, 2 9.5, 4 10.4)
 constexpr int FEW_WARPS = 4, FEW_THREADS = 32 * FEW_WARPS + 32;
 template <int D, int NT>
 struct Few {
@@ -349,7 +351,7 @@ few_kernel(const __grid_constant__ AttnArgs a)
     }
     pdl_launch_dependents();
     pdl_wait_prior_grids();
-    const Deal deal = {a.num_heads / a.c.kv_heads, F::TILE, a.window, FEW_EXTRA};
+    const Deal deal = {a.num_heads / a.c.kv_heads, F::TILE, a.window, FEW_EXTRA, FEW_LEAST};
     Start start;
     Walk w;
     bool any;
@@ -655,9 +657,10 @@ few_kernel(const __grid_constant__ AttnArgs a)
 // ------------------------------------------------------------------------------------------------------------- merge --
 // Joins the tiles that several CTAs have keys of: CTA x takes the tile that CTA x of the kernel before began and did not end.  Its parts are
 // the last part of that CTA and the first parts of those behind it; the same call adds them up in the same order.
-// A row is LANES threads, four elements each; SIDES groups of them share a row's parts where there are few rows, and so many parts.
-constexpr int MERGE_THREADS = 256;
-template <int D, int SIDES>
+// A row is LANES threads, four elements each; SIDES groups of them share a row's parts: where there are few rows, there are many parts.  Bound by
+// latency.
+constexpr int MERGE_THREADS = 256, SIDES = 8;
+template <int D>
 __global__ void __launch_bounds__(MERGE_THREADS)
 merge_kernel(const __grid_constant__ AttnArgs a, int tile)
 {
@@ -702,23 +705,21 @@ merge_kernel(const __grid_constant__ AttnArgs a, int tile)
             l = fmaf(n[i], g, l);
         }
     }
-    if (SIDES > 1) {
-        red[side][mine][lane] = v;
-        if (lane == 0) red_ml[side][mine] = make_float2(top, l);
-        __syncthreads();
-        if (side > 0) return;
-        for (int x = 0; x < SIDES; ++x) top = fmaxf(top, red_ml[x][mine].x);
-        const float ref = top == -INFINITY ? 0.0f : top;
-        v = make_float4(0.f, 0.f, 0.f, 0.f);
-        l = 0.0f;
+    red[side][mine][lane] = v;
+    if (lane == 0) red_ml[side][mine] = make_float2(top, l);
+    __syncthreads();
+    if (side > 0) return;
+    for (int x = 0; x < SIDES; ++x) top = fmaxf(top, red_ml[x][mine].x);
+    const float ref = top == -INFINITY ? 0.0f : top;
+    v = make_float4(0.f, 0.f, 0.f, 0.f);
+    l = 0.0f;
 #pragma unroll
-        for (int x = 0; x < SIDES; ++x) {
-            const float2 ml = red_ml[x][mine];
-            const float4 y = red[x][mine][lane];
-            const float g = ex2(ml.x - ref);
-            v.x = fmaf(y.x, g, v.x); v.y = fmaf(y.y, g, v.y); v.z = fmaf(y.z, g, v.z); v.w = fmaf(y.w, g, v.w);
-            l = fmaf(ml.y, g, l);
-        }
+    for (int x = 0; x < SIDES; ++x) {
+        const float2 ml = red_ml[x][mine];
+        const float4 y = red[x][mine][lane];
+        const float g = ex2(ml.x - ref);
+        v.x = fmaf(y.x, g, v.x); v.y = fmaf(y.y, g, v.y); v.z = fmaf(y.z, g, v.z); v.w = fmaf(y.w, g, v.w);
+        l = fmaf(ml.y, g, l);
     }
     if ((int)blockIdx.y * ROWS + mine >= w.rows) return;
     const float n = 1.0f / l;
@@ -728,7 +729,8 @@ merge_kernel(const __grid_constant__ AttnArgs a, int tile)
 }
 
 // The same for tiles of PROMPT_ROWS rows, which lie in the workspace by columns, [D / 4][rows] of four, as the kernel before has them: neighbouring
-// threads take neighbouring rows, and 16 columns each.
+// threads take neighbouring rows, and 16 columns each; four parts' loads at once (a sequence of 60000 tokens, 64 rows of 28 heads on 4: one part after
+// another 66.4 us of the whole, four at once 54.8).
 constexpr int PROMPT_ROWS = 256, MERGE_ROWS = 32;
 template <int D>
 __global__ void __launch_bounds__(MERGE_ROWS * D / 16)
@@ -745,20 +747,37 @@ merge_columns_kernel(const __grid_constant__ AttnArgs a)
 #pragma unroll
     for (int c = 0; c < 4; ++c) v[c] = make_float4(0.f, 0.f, 0.f, 0.f);
     float top = -INFINITY, l = 0.0f;
-#pragma unroll 2
-    for (int j = 0; j < w.parts; ++j) {
-        const float* p = j == 0 ? base : base + (2 * (size_t)j - 1) * each;
-        float4 x[4];
+    constexpr int AT_ONCE = 4;
+    for (int j0 = 0; j0 < w.parts; j0 += AT_ONCE) {
+        float4 x[AT_ONCE][4];
+        float m[AT_ONCE], n[AT_ONCE];
 #pragma unroll
-        for (int c = 0; c < 4; ++c) x[c] = reinterpret_cast<const float4*>(p)[(c0 + c) * PROMPT_ROWS + r];
-        const float m = p[PROMPT_ROWS * D + r], n = p[PROMPT_ROWS * (D + 1) + r];
-        const float now = fmaxf(top, m), ref = now == -INFINITY ? 0.0f : now, f = ex2(top - ref), g = ex2(m - ref);
+        for (int i = 0; i < AT_ONCE; ++i) {
+            const int j = j0 + i;
+            const float* p = j == 0 ? base : base + (2 * (size_t)j - 1) * each;
+            const bool there = j < w.parts;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) x[i][c] = there ? reinterpret_cast<const float4*>(p)[(c0 + c) * PROMPT_ROWS + r] : make_float4(0.f, 0.f, 0.f, 0.f);
+            m[i] = there ? p[PROMPT_ROWS * D + r] : -INFINITY;
+            n[i] = there ? p[PROMPT_ROWS * (D + 1) + r] : 0.0f;
+        }
+        float now = top;
+#pragma unroll
+        for (int i = 0; i < AT_ONCE; ++i) now = fmaxf(now, m[i]);
+        const float ref = now == -INFINITY ? 0.0f : now, f = ex2(top - ref);
         top = now;
-        l = fmaf(n, g, l * f);
+        l *= f;
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-            v[c].x = fmaf(x[c].x, g, v[c].x * f); v[c].y = fmaf(x[c].y, g, v[c].y * f);
-            v[c].z = fmaf(x[c].z, g, v[c].z * f); v[c].w = fmaf(x[c].w, g, v[c].w * f);
+        for (int c = 0; c < 4; ++c) { v[c].x *= f; v[c].y *= f; v[c].z *= f; v[c].w *= f; }
+#pragma unroll
+        for (int i = 0; i < AT_ONCE; ++i) {
+            const float g = ex2(m[i] - ref);
+            l = fmaf(n[i], g, l);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                v[c].x = fmaf(x[i][c].x, g, v[c].x); v[c].y = fmaf(x[i][c].y, g, v[c].y);
+                v[c].z = fmaf(x[i][c].z, g, v[c].z); v[c].w = fmaf(x[i][c].w, g, v[c].w);
+            }
         }
     }
     const float n = 1.0f / l;

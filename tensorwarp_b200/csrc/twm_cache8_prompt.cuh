@@ -24,6 +24,7 @@ namespace cache8 {
 
 constexpr int PROMPT_THREADS = 448;
 constexpr int PROMPT_EXTRA = 8;                                          // a tile's own time, in units
+constexpr int PROMPT_LEAST = 4;                                          // units of a CTA at least (10 rows of 16 heads on 4 after 2024 tokens: 1 21.3 us, 4 18.3, 8 18.5)
 template <int D>
 struct Prompt {
     static constexpr int BOXES = D / 64;
@@ -95,7 +96,7 @@ prompt_kernel(const __grid_constant__ AttnArgs a)
     }
     // tensor memory is asked for once the kernel before has given its own back: an allocation waits without a limit
     pdl_wait_prior_grids();
-    const Deal deal = {a.num_heads / a.c.kv_heads, PROMPT_ROWS, a.window, PROMPT_EXTRA};
+    const Deal deal = {a.num_heads / a.c.kv_heads, PROMPT_ROWS, a.window, PROMPT_EXTRA, PROMPT_LEAST};
     const Start start = find_start<PROMPT_THREADS>(a, deal, blockIdx.x, gridDim.x);
     if (start.out) zero_rows(a, D, blockIdx.x, gridDim.x, tid, PROMPT_THREADS);
     Walk w;

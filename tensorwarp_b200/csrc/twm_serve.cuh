@@ -104,8 +104,8 @@ twm_status launch_merge(const twm::cache8::AttnArgs& a, const AttnPlan& p, int f
     if (p.tile == twm::cache8::PROMPT_ROWS)
         return launch_op("twm_cache8_attention(merge)", twm::cache8::merge_columns_kernel<D>, dim3(p.ctas, p.tile / twm::cache8::MERGE_ROWS),
                          dim3(twm::cache8::MERGE_ROWS * D / 16), 0, flags, stream, a);
-    const int rows = twm::cache8::MERGE_THREADS / (D / 4) / 8;
-    return launch_op("twm_cache8_attention(merge)", twm::cache8::merge_kernel<D, 8>, dim3(p.ctas, (p.tile + rows - 1) / rows),
+    const int rows = twm::cache8::MERGE_THREADS / (D / 4) / twm::cache8::SIDES;
+    return launch_op("twm_cache8_attention(merge)", twm::cache8::merge_kernel<D>, dim3(p.ctas, (p.tile + rows - 1) / rows),
                      dim3(twm::cache8::MERGE_THREADS), 0, flags, stream, a, p.tile);
 }
 
