@@ -280,13 +280,13 @@ __device__ __forceinline__ int exponent_of(float scale) { return (int)(__float_a
 
 // --------------------------------------------------------------------------------------------- few rows a sequence --
 // Up to 8 NT rows a sequence and key/value head (the query heads that share it, times the new tokens): they are one tile, and every key is
-// read once.  Bound by HBM (96 sequences of up to 6000 tokens, 28 heads on 4: 121 us, 6.0 TB/s).  Four consumer warps take 16 keys each of a unit; a producer warp brings units by TMA into a ring that runs on over
-// the borders of tiles, the tail's FP16 rows among them (keys and values in a stage each).  S^T = K Q^T and O^T += V^T P^T as mma.m16n8k16 with
-// the keys, and then the head's elements, as the 16 rows, so that eight rows of queries are a whole operand.  Elements and keys may stand in any
-// order in a sum: lane (g, t) takes D / 4 elements of keys g and g + 8 for the scores (4 codes a k-step of both registers), and D / 8 elements of
-// four keys for the output, whose codes are paired by a byte permutation; at D = 128 both reads are free of bank conflicts in the
-// layout that the TMA's swizzle leaves.  P^T needs only a transposition of 8 x 8.  Each warp has its own m; when the tile ends the four add up in
-// shared memory, while the next tile's queries are on their way.
+// read once.  Bound by HBM (96 sequences of up to 6000 tokens, 40 heads on 8: 121 us, 6.06 TB/s).  Four consumer warps take 16 keys each of a
+// unit; a producer warp brings units by TMA into a ring that runs on over the borders of tiles, the tail's FP16 rows among them (keys and
+// values in a stage each).  S^T = K Q^T and O^T += V^T P^T as mma.m16n8k16 with the keys, and then the head's elements, as the 16 rows, so that eight
+// rows of queries are a whole operand.  Elements and keys may stand in any order in a sum: lane (g, t) takes D / 4 elements of keys g and g + 8 for
+// the scores (4 codes a k-step of both registers), and D / 8 elements of four keys for the output, whose codes are paired by a byte permutation; at
+// D = 128 both reads are free of bank conflicts in the layout that the TMA's swizzle leaves.  P^T needs only a transposition of 8 x 8.  Each warp has
+// its own m; when the tile ends the four add up in shared memory, while the next tile's queries are on their way.
 constexpr int FEW_EXTRA = 4;                                             // a tile's own time, in units (96 sequences: 1 124.5 us, 2 121.9, 4 120.8)
 constexpr int FEW_LEAST = 1;                                             // units of a CTA at least (2049 tokens, 28 heads: 1 9.2 us, 2 9.5, 4 10.4)
 constexpr int FEW_WARPS = 4, FEW_THREADS = 32 * FEW_WARPS + 32;
