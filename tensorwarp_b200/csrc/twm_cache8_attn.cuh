@@ -658,8 +658,9 @@ few_kernel(const __grid_constant__ AttnArgs a)
 // Joins the tiles that several CTAs have keys of: CTA x takes the tile that CTA x of the kernel before began and did not end.  Its parts are
 // the last part of that CTA and the first parts of those behind it; the same call adds them up in the same order.
 // A row is LANES threads, four elements each; SIDES groups of them share a row's parts: where there are few rows, there are many parts.  Bound by
-// latency.
-constexpr int MERGE_THREADS = 256, SIDES = 8;
+// latency, that of the launch of CTAs without a tile among it (us of a call with 256 threads and eight groups, 128 and four, 128 and two: 500
+// tokens 8.7, 7.8, 7.5; 2049 tokens 9.1, 8.6, 9.0; 100 000 tokens 25.7, 26.4, 29.5; 96 sequences 121.4, 119.0, 117.9).
+constexpr int MERGE_THREADS = 128, SIDES = 4;
 template <int D>
 __global__ void __launch_bounds__(MERGE_THREADS)
 merge_kernel(const __grid_constant__ AttnArgs a, int tile)

@@ -23,7 +23,7 @@ namespace twm {
 namespace cache8 {
 
 constexpr int PROMPT_THREADS = 448;
-constexpr int PROMPT_EXTRA = 8;                                          // a tile's own time, in units
+constexpr int PROMPT_EXTRA = 8;                                          // a tile's own time, in units (prompt of 4000: 4 153.9 us, 8 155.3, 12 161.9; 56 of 642: 98, 95, 91.5)
 constexpr int PROMPT_LEAST = 4;                                          // units of a CTA at least (10 rows of 16 heads on 4 after 2024 tokens: 1 21.3 us, 4 18.3, 8 18.5)
 template <int D>
 struct Prompt {

@@ -33,14 +33,14 @@ twm::cache8::Cache device_cache(const twm_cache8* c)
     return {c->seqs, c->kv_heads, c->capacity, (uint8_t*)c->k, (uint8_t*)c->v, c->k_scale, c->v_scale, (__half*)c->k_tail, (__half*)c->v_tail};
 }
 
-// How attention is launched: the rows of a tile and the CTAs of the grid, whatever the lengths (which are on the device).
-struct AttnPlan { int tile, ctas; };
+// How attention is launched: the rows of a tile, how many of them there can be, and the CTAs of the grid, whatever the lengths (which are on the device).
+struct AttnPlan { int tile, rows, ctas; };
 AttnPlan plan_attention(int group, int max_rows, int head_dim)
 {
     const long rows = (long)max_rows * group;
-    if (rows <= 8) return {8, kDefaultSms * (head_dim == 64 ? twm::cache8::Few<64, 1>::CTAS : twm::cache8::Few<128, 1>::CTAS)};
-    if (rows <= 16) return {16, kDefaultSms * (head_dim == 64 ? twm::cache8::Few<64, 2>::CTAS : twm::cache8::Few<128, 2>::CTAS)};
-    return {twm::cache8::PROMPT_ROWS, kDefaultSms};
+    if (rows <= 8) return {8, (int)rows, kDefaultSms * (head_dim == 64 ? twm::cache8::Few<64, 1>::CTAS : twm::cache8::Few<128, 1>::CTAS)};
+    if (rows <= 16) return {16, (int)rows, kDefaultSms * (head_dim == 64 ? twm::cache8::Few<64, 2>::CTAS : twm::cache8::Few<128, 2>::CTAS)};
+    return {twm::cache8::PROMPT_ROWS, (int)std::min(rows, (long)twm::cache8::PROMPT_ROWS), kDefaultSms};
 }
 
 // The codes of keys or values as [cached rows][head_dim], a box a block, swizzled over its whole row.
@@ -102,10 +102,10 @@ twm_status launch_merge(const twm::cache8::AttnArgs& a, const AttnPlan& p, int f
 {
     flags |= TWM_FLAG_PDL;
     if (p.tile == twm::cache8::PROMPT_ROWS)
-        return launch_op("twm_cache8_attention(merge)", twm::cache8::merge_columns_kernel<D>, dim3(p.ctas, p.tile / twm::cache8::MERGE_ROWS),
+        return launch_op("twm_cache8_attention(merge)", twm::cache8::merge_columns_kernel<D>, dim3(p.ctas, (p.rows + twm::cache8::MERGE_ROWS - 1) / twm::cache8::MERGE_ROWS),
                          dim3(twm::cache8::MERGE_ROWS * D / 16), 0, flags, stream, a);
-    const int rows = twm::cache8::MERGE_THREADS / (D / 4) / twm::cache8::SIDES;
-    return launch_op("twm_cache8_attention(merge)", twm::cache8::merge_kernel<D>, dim3(p.ctas, (p.tile + rows - 1) / rows),
+    const int each = twm::cache8::MERGE_THREADS / (D / 4) / twm::cache8::SIDES;
+    return launch_op("twm_cache8_attention(merge)", twm::cache8::merge_kernel<D>, dim3(p.ctas, (p.rows + each - 1) / each),
                      dim3(twm::cache8::MERGE_THREADS), 0, flags, stream, a, p.tile);
 }
 
