@@ -280,7 +280,7 @@ __device__ __forceinline__ int exponent_of(float scale) { return (int)(__float_a
 
 // --------------------------------------------------------------------------------------------- few rows a sequence --
 // Up to 8 NT rows a sequence and key/value head (the query heads that share it, times the new tokens): they are one tile, and every key is
-// read once.  Bound by HBM (96 sequences of up to 6000 tokens, 40 heads on 8: 121 us, 6.06 TB/s).  Four consumer warps take 16 keys each of a
+// read once.  Bound by HBM (96 sequences of up to 6000 tokens, 40 heads on 8: 119 us, 6.18 TB/s).  Four consumer warps take 16 keys each of a
 // unit; a producer warp brings units by TMA into a ring that runs on over the borders of tiles, the tail's FP16 rows among them (keys and
 // values in a stage each).  S^T = K Q^T and O^T += V^T P^T as mma.m16n8k16 with the keys, and then the head's elements, as the 16 rows, so that eight
 // rows of queries are a whole operand.  Elements and keys may stand in any order in a sum: lane (g, t) takes D / 4 elements of keys g and g + 8 for
