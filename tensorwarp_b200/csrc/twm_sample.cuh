@@ -459,6 +459,7 @@ sample_kernel(const __grid_constant__ twm_sample_args a, int slice, int ctas)
                 }
                 uint32_t border, border_ties;
                 if (left > FEW) {                            // equal ones only
+                    __syncthreads();                         // all have read what the last `find` left, which that of the next pass resets
                     const double w = (double)weights.of(value_of(lo));
                     border = lo;
                     border_ties = what == 0 ? (uint32_t)k - over : w > 0.0 ? (uint32_t)fmin(fmax(ceil((want - over_mass) / w), 1.0), (double)left) : left;

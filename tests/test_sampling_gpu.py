@@ -244,3 +244,20 @@ def test_two_calls_at_once():
             sampling.sample(x, u, t, top_p=p, stream=s)
     torch.cuda.synchronize()
     assert all(torch.equal(x, y) for x, y in zip(want, got))
+
+
+@pytest.mark.parametrize("vocab", [700, 32771, 152064])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_many_equal_numbers_at_the_border_of_top_k(vocab, dtype):
+    """A few dozen different logits, so that hundreds are equal where top-k ends, and top-p behind it: a hundred calls, one result."""
+    g = gen("border", vocab)
+    ks, ps = [60, 100, 333, 600], [0.2, 0.5, 0.9, 0.999]
+    rows = len(ks) * len(ps)
+    logits = (torch.randint(0, 12, (rows, vocab), generator=g, device="cuda") * 0.25).to(dtype)
+    u = torch.rand(rows, generator=g, device="cuda")
+    top_k, top_p = i32([k for k in ks for _ in ps]), f32([p for _ in ks for p in ps])
+    want = verify(logits, u, top_k=top_k, top_p=top_p)
+    got = [torch.zeros(rows, dtype=torch.int32, device="cuda") for _ in range(100)]
+    for t in got:
+        sampling.sample(logits, u, t, top_k=top_k, top_p=top_p)
+    assert all(torch.equal(t, want) for t in got)
