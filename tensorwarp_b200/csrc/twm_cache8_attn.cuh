@@ -6,9 +6,12 @@
 //     x_j = (q . c_k) (scale 2^ek log2 e) + ev,
 // so that 2^x_j is the factor of the CODES c_v in the output, and 2^(x_j - ev) the weight that belongs into the sum of weights:
 //     o = sum 2^(x_j - m) c_v / sum 2^(x_j - m) 2^-ev.
-// One fused multiply-add an element as without scales, and since the running reference m is that of x_j, scale of the value
-// included, the largest FP16 factor of a row is near 1 however the scales of its blocks differ.  m moves only when a factor would pass 2^8.
-// A factor is rounded to FP16 (2^-11 of itself): the values' codes have four bits, and sums, scores and statistics are FP32.
+// One fused multiply-add an element as without scales.  The running reference m is that of x_j, scale of the value included: it is set
+// so that the largest factor is 2^7 and moves only when one would pass 2^15.  So a row's largest factor so far lies between them, whatever the scales of
+// its blocks are, and a factor is rounded to FP16 by 2^-11 of itself down to 2^-14, and by at most 2^-32 of the largest one below: the values' codes
+// have four bits, and sums, scores and statistics are FP32.
+// For that ev has to say how large values are.  A block of zeros has scale 1: its ev is NO_VALUES, below all others, so that it weighs in the sum and
+// leaves the reference to the others.  The tail has ev 0 however small its values are, but comes last: no factor of codes is taken behind it.
 #pragma once
 
 #include "twm_cache8.cuh"
@@ -278,6 +281,9 @@ __device__ __forceinline__ float ex2(float x) { float y; asm("ex2.approx.ftz.f32
 // the exponent of a block's scale, from the scale
 __device__ __forceinline__ int exponent_of(float scale) { return (int)(__float_as_uint(scale) >> 23) - 127; }
 
+constexpr float LEAST_TOP = 7.0f, MOST_TOP = 15.0f;                      // logarithms between which a row's largest factor lies
+constexpr int NO_VALUES = -64;
+
 // --------------------------------------------------------------------------------------------- few rows a sequence --
 // Up to 8 NT rows a sequence and key/value head (the query heads that share it, times the new tokens): they are one tile, and every key is
 // read once.  Bound by HBM (96 sequences of up to 6000 tokens, 40 heads on 8: 119 us, 6.18 TB/s).  Four consumer warps take 16 keys each of a
@@ -469,7 +475,8 @@ few_kernel(const __grid_constant__ AttnArgs a)
 #pragma unroll
                 for (int c = 0; c < 4; ++c) s[0][nt][c] = s[1][nt][c] = 0.0f;
             uint32_t vw[4][DPL / 4];                                     // codes of this lane's elements of four keys
-            const float factor = a.scale * LOG2E * ks, inv = power_of_two(-exponent_of(vs)), ev = (float)exponent_of(vs);
+            const float factor = a.scale * LOG2E * ks;
+            float inv = power_of_two(-exponent_of(vs)), ev = (float)exponent_of(vs);
             if (u + 1 < w.u0 + w.n) { ks = u + 1 < held ? k_scale[u + 1] : 1.0f; vs = u + 1 < held ? v_scale[u + 1] : 1.0f; }
             const bool codes = u < held;
             const int valid = length - u * BLOCK;                        // tokens of the tail that are there; what lies behind them is taken as zeros
@@ -499,6 +506,14 @@ few_kernel(const __grid_constant__ AttnArgs a)
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt) mma_16x8x16(s[k & 1][nt], a0, a1, a2, a3, q[nt][j * 4 + k][0], q[nt][j * 4 + k][1]);
                     }
+                }
+                if (ev == 0.0f) {                                        // that of zeros too
+                    uint32_t any = 0;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+#pragma unroll
+                        for (int k = 0; k < DPL / 4; ++k) any |= vw[j][k];
+                    if (!__any_sync(0xffffffffu, (any & 0x7f7f7f7fu) != 0)) { ev = (float)NO_VALUES; inv = power_of_two(-NO_VALUES); }
                 }
             } else {
                 const uint8_t* kt = stages + i % F::STAGES * F::STAGE;
@@ -531,7 +546,7 @@ few_kernel(const __grid_constant__ AttnArgs a)
                         if (!(key <= p && p - key < a.window)) x = -INFINITY;
                     }
                     s[0][nt][c] = x;
-                    over |= x > m[nt][c & 1] + 8.0f;
+                    over |= x > m[nt][c & 1] + MOST_TOP;
                 }
             if (__any_sync(0xffffffffu, over)) {
 #pragma unroll
@@ -541,6 +556,7 @@ few_kernel(const __grid_constant__ AttnArgs a)
                         float top = fmaxf(s[0][nt][c], s[0][nt][c + 2]);
 #pragma unroll
                         for (int x = 4; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+                        top -= LEAST_TOP;
                         if (top > m[nt][c]) {
                             const float before = ex2(m[nt][c] - top);
                             m[nt][c] = top;

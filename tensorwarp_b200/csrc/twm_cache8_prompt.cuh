@@ -7,7 +7,7 @@
 //               Lanes take four chunks of 16 codes of rows r and r ^ 5, so that neither the reads nor the writes meet in a bank.
 //   warp 13     one thread issues tcgen05.mma: half by half the scores of unit u + 1, then P V of unit u (P from tensor memory), so that the halves are
 //               not at their exponentials at once.
-//   warps 0-7   thread = row: maximum, weights, sum; the reference of the exponents moves only when a factor would pass 2^8, and then the row's output is
+//   warps 0-7   thread = row: maximum, weights, sum; the reference of the exponents moves only when a factor would pass 2^15, and then the row's output is
 //               scaled in tensor memory ahead of the unit's P V.  They bring the rows' queries to shared memory and store the results.
 // Tensor memory: two score buffers of 64 columns and D of output for each half; the factors, FP16, overwrite the scores.
 // Sharing a unit between two halves is what shared memory asks for: a unit costs 16 KB read and 32 KB written by the conversion and 64 KB read by
@@ -242,7 +242,7 @@ prompt_kernel(const __grid_constant__ AttnArgs a)
         const uint32_t lane_tmem = tmem + x * P::HALF + ((uint32_t)((warp & 3) * 32) << 16), lane_o = lane_tmem + P::OUT;
         const float base = a.scale * LOG2E;
         const bool wide = ((reinterpret_cast<uintptr_t>(a.out) | (uintptr_t)(a.ldo * 2)) & 31) == 0;
-        int n = 0, tile = -1;                             // units of this half; the tile's number
+        int n = 0, tile = -1, without = 0;                // units of this half; the tile's number; units of tiles without this half
         // The queries of a tile to shared memory: that of the next one while the last products of this one run (its scores are all done).
         struct Mine { int all, r, token, head; bool live; } now;
         auto bring = [&](const Walk& w) {
@@ -287,6 +287,7 @@ prompt_kernel(const __grid_constant__ AttnArgs a)
             const size_t at = (size_t)w.seq * a.c.kv_heads + w.head;
             if (x * 128 >= now.all) {                     // not ahead of the others, whose arrivals would be taken for this half's
                 tc::wait_uniform(&q_full, (uint32_t)tile & 1u, abort_flag);
+                without += w.n;
                 more = w.next(a, deal);
                 if (more) now = bring(w);
                 continue;
@@ -299,8 +300,21 @@ prompt_kernel(const __grid_constant__ AttnArgs a)
             float m = -INFINITY, l = 0.0f;
             for (int j = 0; j < w.n; ++j, ++n) {
                 const int u = w.u0 + j;
-                const float factor = base * ks, inv = power_of_two(-exponent_of(vs)), ev = (float)exponent_of(vs);
+                const float factor = base * ks;
+                float inv = power_of_two(-exponent_of(vs)), ev = (float)exponent_of(vs);
                 if (j + 1 < w.n) { ks = u + 1 < held ? k_scale[u + 1] : 1.0f; vs = u + 1 < held ? v_scale[u + 1] : 1.0f; }
+                if (ev == 0.0f) {                         // a scale of one, which a block of zeros has too; here, where no scores are in registers
+                    const int slot = (n + without) % P::UNITS;
+                    tc::wait_uniform(&unit_full[slot], (uint32_t)((n + without) / P::UNITS) & 1u, abort_flag);
+                    const uint4* values = reinterpret_cast<const uint4*>(units + slot * P::UNIT + P::BOXES * P::KBOX);
+                    bool any = false;
+#pragma unroll 1
+                    for (int c = lane; c < BLOCK * D / 8 && !any; c += 32) {
+                        const uint4 v = values[c];
+                        any = __any_sync(0xffffffffu, ((v.x | v.y | v.z | v.w) & 0x7fff7fffu) != 0);
+                    }
+                    if (!any) { ev = (float)NO_VALUES; inv = power_of_two(-NO_VALUES); }
+                }
                 const uint32_t scores = lane_tmem + (n & 1) * BLOCK;
                 tc::wait_uniform(&s_full[x][n & 1], (uint32_t)(n >> 1) & 1u, abort_flag);
                 tc::tc_fence_after();
@@ -333,10 +347,10 @@ prompt_kernel(const __grid_constant__ AttnArgs a)
                 }
                 const float top = fmaf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), factor, ev);
                 float before = 1.0f;
-                const bool moved = top > m + 8.0f;
+                const bool moved = top > m + MOST_TOP;
                 if (moved) {
-                    before = ex2(m - top);
-                    m = top;
+                    before = ex2(m - (top - LEAST_TOP));
+                    m = top - LEAST_TOP;
                     l *= before;
                 }
                 const float shift = ev - (m == -INFINITY ? 0.0f : m);

@@ -119,3 +119,30 @@ def attention(q, k, v, start, heads, scale, window):
     seen = torch.einsum("hgrl,hld->rhgd", (p > 0).double(), v.abs()).flatten(1)
     top = p.amax(dim=-1).permute(2, 0, 1).repeat_interleave(d, dim=2).flatten(1)
     return out, 2.0 ** -11 * out.abs() + (2.0 ** -11 + 2.0 ** -15 + 2 * (d + 8) * 2.0 ** -24 * largest) * size + 2.0 ** -25 * top * seen + 2.0 ** -25
+
+
+def attention_by_values(q, k, v, start, heads, scale, window):
+    """As ``attention``, with a bound that shrinks with the values, however the sizes of blocks of them differ.
+
+    Beside what the bound of ``attention`` says of scores, sums and the result: a weight times its values' unit enters the product as FP16, off by half a
+    step: 2^-11 of itself, or 2^-25 where it is below 2^-14, when the largest one of the row so far lies at 2^7 at least, so 2^-32 of that one.  The unit of a
+    full block is a power of two below 1/224 of its largest value ahead of the rounding to 4 bits, which takes 2^-4 of it at most; values of zeros have
+    none.  That of the tail, which comes last, is one.  In its unit a value of a full block is at most 448."""
+    rows, group, n = q.shape[0], heads // k.shape[0], k.shape[1]
+    d = k.shape[2]
+    x = torch.einsum("rhgd,hld->hgrl", q.double().unflatten(1, (k.shape[0], group, d)), k) * scale
+    far = torch.arange(start, start + rows, device="cuda")[:, None] - torch.arange(n, device="cuda")
+    x = x.masked_fill(~((far >= 0) & (far < (window or 1 << 40))), -math.inf)
+    p = torch.softmax(x, dim=-1)
+    wide = lambda t: t.permute(2, 0, 1).repeat_interleave(d, dim=2).flatten(1)  # noqa: E731
+    largest = wide(x.masked_fill(x == -math.inf, 0.0).abs().amax(dim=-1))
+    out = torch.einsum("hgrl,hld->rhgd", p, v).flatten(1)
+    size = torch.einsum("hgrl,hld->rhgd", p, v.abs()).flatten(1)
+    top = torch.stack([v[:, b:b + BLOCK].abs().amax(dim=(1, 2)) for b in range(0, n, BLOCK)], dim=1).repeat_interleave(BLOCK, dim=1)[:, :n]
+    unit = top / (224 * (1 - 2.0 ** -4))
+    full = n // BLOCK * BLOCK
+    small = (p[..., :full] * unit[:, None, None, :full]).amax(dim=-1) * 448.0 * full if full else torch.zeros_like(p[..., 0])
+    if full < n:
+        unit[:, full:] = 1.0
+        small = small + (p * unit[:, None, None]).amax(dim=-1) * top[:, None, None, -1] * (n - full)
+    return out, 2.0 ** -11 * out.abs() + (2.0 ** -11 + 2.0 ** -15 + 2 * (d + 8) * 2.0 ** -24 * largest) * size + 2.0 ** -32 * wide(small) + 2.0 ** -25

@@ -478,3 +478,67 @@ def test_calls_without_rows():
     b.held.check(b.cache)
     with pytest.raises(_lib.TwmError):
         cache8.attention(b.cache, none[:, :512], none[:, :512], ints([70, 3]), num_heads=8)
+
+
+def verify_copies(b, length, rows, window, scale, copies):
+    """Attention over as many copies of the batch's one sequence, so that a CTA has a run of many units; what the runs begin and end with differs."""
+    c = b.cache
+    many = lambda t: t.view(torch.uint8 if t.dtype.itemsize == 1 else t.dtype).expand(copies, *t.shape[1:]).contiguous()  # noqa: E731
+    cache = cache8.Cache8(*(many(t) for t in (c.k, c.v, c.k_scale, c.v_scale, c.k_tail, c.v_tail)))
+    one = torch.rand((rows, b.heads * b.dim), generator=b.gen, device="cuda").half() + 0.5
+    q = one.repeat(copies, 1)
+    out = torch.zeros_like(q)
+    cache8.attention(cache, q, out, ints([length - rows] * copies), num_heads=b.heads, row_start=ints([rows * s for s in range(copies + 1)]), max_rows=rows,
+                     window=window, scale=scale)
+    want, off = ref.attention_by_values(one, *b.held.held(0, length), length - rows, b.heads, scale, window)
+    worst = ((out.double().unflatten(0, (copies, rows)) - want).abs() / off).max()
+    assert bool(worst <= 1), (length, window, float(worst))
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim", [(4, 1, 128), (2, 2, 64)])
+@pytest.mark.parametrize("rows", [1, 3, 40])
+@pytest.mark.parametrize("size", [1e-4, 1e-3, 1e-2, 1.0])
+@pytest.mark.parametrize("blocks", ["alike", "zeros first", "zeros between", "zeros in the tail", "units of one", "larger tail", "smaller tail", "zeros"])
+def test_small_values_keep_their_bits(heads, kv_heads, dim, rows, size, blocks):
+    """Values of any size, beside blocks or a tail of zeros, of values whose scale is one, and of larger and smaller ones."""
+    def make(n):
+        x = torch.randn((n, (heads + 2 * kv_heads) * dim), generator=gen("v", n, dim), device="cuda")
+        block = torch.arange(n, device="cuda")[:, None] // 64
+        tail = block == n // 64
+        v = x[:, (heads + kv_heads) * dim:]
+        v *= size
+        if blocks.startswith("zeros"):
+            v *= ~{"zeros": block >= 0, "zeros first": block == 0, "zeros between": (block == 2) | (block == 5), "zeros in the tail": tail}[blocks]
+        elif blocks == "units of one":
+            v *= torch.where(block == 6, 60.0 / size, 1.0)
+        elif blocks != "alike":
+            v *= torch.where(tail, 2.0 ** 5 if blocks == "larger tail" else 2.0 ** -5, 1.0)
+        return x
+    for length in (448, 451, 500):
+        b = Batch(1, 512, heads, kv_heads, dim, bias=False, rope=False, make=make)
+        b.append([0], [length])
+        for window in (0, 8, 70):
+            verify_copies(b, length, rows, window, 1 / math.sqrt(dim), 400 if rows < 9 else 40)
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim", [(4, 1, 128), (2, 2, 64)])
+@pytest.mark.parametrize("rows", [1, 3, 40, 70])
+@pytest.mark.parametrize("size", [1e-4, 1e-3, 1e-2])
+@pytest.mark.parametrize("where", ["tail", "zeros", "zeros of one warp"])
+def test_equal_weights_of_small_values(heads, kv_heads, dim, rows, size, where):
+    """All tokens but those of the tail, or of a block of zeros, weigh the same, so that what a weight is off by does not average out."""
+    length = 64 * 7 + (40 if where == "tail" else 0)
+
+    def make(n):
+        x = torch.zeros((n, heads + 2 * kv_heads, dim), device="cuda")
+        token = torch.arange(n, device="cuda")[:, None]
+        other = token // 64 == (7 if where == "tail" else 1)
+        x[:, heads:heads + kv_heads, 0] = torch.where(other, 0.25, 0.0)
+        v = size * (1 + torch.rand((n, kv_heads, dim), generator=gen("w", n), device="cuda"))
+        none = {"tail": other & False, "zeros": other, "zeros of one warp": other & (token % 64 < 16)}[where]
+        x[:, heads + kv_heads:] = torch.where(none[:, :, None], 0.0, v)
+        return x.flatten(1)
+    b = Batch(1, 512, heads, kv_heads, dim, bias=False, rope=False, make=make)
+    b.append([0], [length])
+    for window in (0, 300):
+        verify_copies(b, length, rows, window, 1.0, 400 if rows < 9 else 40)
