@@ -174,7 +174,7 @@ struct Walk {
         const int tiles = d.tiles(sp), lane = threadIdx.x & 31;
         const long long per = tiles == 1 ? d.units(sp, 0) : d.units_by_warp(sp);
         head = (int)quotient(s.before, per);
-        int rest = (int)(s.before - head * per);
+        long long rest = s.before - head * per;                          // 32 tiles' units fit 32 bits (cached rows / 64 each), a head's need not
         t = 0;
         while (tiles > 1) {                                              // 32 tiles at a time
             const int mine = t + lane < tiles ? d.units(sp, t + lane) : 0;
@@ -194,7 +194,7 @@ struct Walk {
             rest -= __shfl_sync(0xffffffffu, upto, 31);
             t += 32;
         }
-        take(d, rest);
+        take(d, (int)rest);
         return n > 0;
     }
     __device__ __forceinline__ bool next(const AttnArgs& a, const Deal& d)
