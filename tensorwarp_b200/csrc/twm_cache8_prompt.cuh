@@ -74,7 +74,7 @@ prompt_kernel(const __grid_constant__ AttnArgs a)
     extern __shared__ uint8_t prompt_raw[];
     __shared__ uint64_t raw_full[P::RAWS], raw_empty[P::RAWS], unit_full[P::UNITS], unit_empty[P::UNITS], q_full, s_full[2][2], p_full[2][2], o_done[2][2];
     __shared__ uint32_t s_tmem;
-    __shared__ int s_abort;
+    __shared__ int s_abort, s_without[8];                                // units of tiles that a warp of rows had no part in
     uint8_t* qs = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(prompt_raw) + 1023) & ~(uintptr_t)1023);
     uint8_t* units = qs + 2 * P::BOXES * P::QBOX;
     uint8_t* raws = units + P::UNITS * P::UNIT;
@@ -92,6 +92,7 @@ prompt_kernel(const __grid_constant__ AttnArgs a)
             mbar_init(&o_done[x][1], 1);
         }
         s_abort = 0;
+        for (int i = 0; i < 8; ++i) s_without[i] = 0;
         mbar_fence_init();
     }
     // tensor memory is asked for once the kernel before has given its own back: an allocation waits without a limit
@@ -242,7 +243,7 @@ prompt_kernel(const __grid_constant__ AttnArgs a)
         const uint32_t lane_tmem = tmem + x * P::HALF + ((uint32_t)((warp & 3) * 32) << 16), lane_o = lane_tmem + P::OUT;
         const float base = a.scale * LOG2E;
         const bool wide = ((reinterpret_cast<uintptr_t>(a.out) | (uintptr_t)(a.ldo * 2)) & 31) == 0;
-        int n = 0, tile = -1, without = 0;                // units of this half; the tile's number; units of tiles without this half
+        int n = 0, tile = -1;                             // units of this half; the tile's number
         // The queries of a tile to shared memory: that of the next one while the last products of this one run (its scores are all done).
         struct Mine { int all, r, token, head; bool live; } now;
         auto bring = [&](const Walk& w) {
@@ -287,7 +288,8 @@ prompt_kernel(const __grid_constant__ AttnArgs a)
             const size_t at = (size_t)w.seq * a.c.kv_heads + w.head;
             if (x * 128 >= now.all) {                     // not ahead of the others, whose arrivals would be taken for this half's
                 tc::wait_uniform(&q_full, (uint32_t)tile & 1u, abort_flag);
-                without += w.n;
+                if (lane == 0) s_without[warp] += w.n;
+                __syncwarp();
                 more = w.next(a, deal);
                 if (more) now = bring(w);
                 continue;
@@ -304,8 +306,8 @@ prompt_kernel(const __grid_constant__ AttnArgs a)
                 float inv = power_of_two(-exponent_of(vs)), ev = (float)exponent_of(vs);
                 if (j + 1 < w.n) { ks = u + 1 < held ? k_scale[u + 1] : 1.0f; vs = u + 1 < held ? v_scale[u + 1] : 1.0f; }
                 if (ev == 0.0f) {                         // a scale of one, which a block of zeros has too; here, where no scores are in registers
-                    const int slot = (n + without) % P::UNITS;
-                    tc::wait_uniform(&unit_full[slot], (uint32_t)((n + without) / P::UNITS) & 1u, abort_flag);
+                    const int i = n + s_without[warp], slot = i % P::UNITS;
+                    tc::wait_uniform(&unit_full[slot], (uint32_t)(i / P::UNITS) & 1u, abort_flag);
                     const uint4* values = reinterpret_cast<const uint4*>(units + slot * P::UNIT + P::BOXES * P::KBOX);
                     bool any = false;
 #pragma unroll 1
