@@ -232,12 +232,10 @@ class DenseEngine:
         return self._generate("greedy", seq, tokens, count)
 
     def sample(self, seq: int, tokens: Sequence[int], count: int, params: SamplingParams, generator: torch.Generator) -> List[int]:
-        random = torch.rand(max(count, 0), generator=generator)
-        with torch.cuda.stream(self.stream):
-            self._loop.set(params, random[:self.capacity])          # more than that are refused below
-        return self._generate("sample", seq, tokens, count)
+        return self._generate("sample", seq, tokens, count, params, generator)
 
-    def _generate(self, kind: str, seq: int, tokens: Sequence[int], count: int) -> List[int]:
+    def _generate(self, kind: str, seq: int, tokens: Sequence[int], count: int, params: Optional[SamplingParams] = None,
+                  generator: Optional[torch.Generator] = None) -> List[int]:
         if count < 1:
             return []
         tokens = list(tokens)
@@ -247,6 +245,8 @@ class DenseEngine:
             raise ValueError(f"{first} + {len(tokens)} tokens and {count} new ones run past the slot's {self.capacity}")
         replays = count
         with torch.cuda.stream(self.stream):
+            if kind == "sample":                                    # a refused call has drawn nothing
+                self._loop.set(params, torch.rand(count, generator=generator))
             self._buf["meta"][3:4].zero_()                          # the step counter indexes the history
             if len(tokens) > 1:
                 self.step(seq, tokens, [len(tokens) - 1])

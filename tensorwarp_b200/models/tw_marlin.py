@@ -73,15 +73,17 @@ class Q4StepEngine:
         return torch.stack(rows) if rows else None
 
     def greedy(self, seq: int, tokens: Sequence[int], count: int) -> List[int]:
-        return self._generate(seq, tokens, count, {})
+        return self._generate(seq, tokens, count)
 
     def sample(self, seq: int, tokens: Sequence[int], count: int, params: SamplingParams, generator: torch.Generator) -> List[int]:
-        return self._generate(seq, tokens, count, {"sampling": params, "random": torch.rand(max(count, 0), generator=generator)})
+        return self._generate(seq, tokens, count, params, generator)
 
-    def _generate(self, seq: int, tokens: Sequence[int], count: int, how: dict) -> List[int]:
+    def _generate(self, seq: int, tokens: Sequence[int], count: int, params: Optional[SamplingParams] = None,
+                  generator: Optional[torch.Generator] = None) -> List[int]:
         self._reserve(seq, tokens, max(count - 1, 0))
         if count < 1:
             return []
+        how = {} if params is None else {"sampling": params, "random": torch.rand(count, generator=generator)}
         for token in tokens[:-1]:
             self._run(token)
         self.engine.reset_history()

@@ -164,3 +164,28 @@ def test_command_line_refuses_cuts_without_a_temperature():
     from tensorwarp_b200.__main__ import main
     with pytest.raises(SystemExit):
         main(["generate", "--model", "/nowhere", "--tokens", "1", "--top-p", "0.9"])
+
+
+def test_refused_calls_draw_no_random_numbers():
+    """A call that an engine refuses leaves the generator and the settings of its loop as they were."""
+    from types import SimpleNamespace
+
+    from tensorwarp_b200.engine import DenseEngine
+    from tensorwarp_b200.models.tw_marlin import Q4StepEngine
+    from tensorwarp_b200.state import StateError
+
+    def touched(*a, **kw):
+        raise AssertionError("a refused call has set the loop's numbers")
+
+    dense = DenseEngine.__new__(DenseEngine)
+    dense.vocab, dense.capacity, dense.stream, dense.state, dense._loop = 100, 20, None, SimpleNamespace(length=lambda seq: 10), SimpleNamespace(set=touched)
+    q4 = Q4StepEngine(SimpleNamespace(cfg=SimpleNamespace(vocab=100, max_seq=20), generate_tw_marlin_graph=touched))
+    q4._length = 10
+    for engine in (dense, q4):
+        generator, params = torch.Generator().manual_seed(3), sampling.SamplingParams()
+        before = generator.get_state()
+        for tokens, count in (([1, 2], 10), ([1], 1000), ([], 2), ([100], 2), ([-1, 4], 3)):
+            with pytest.raises((ValueError, StateError)):
+                engine.sample(0, tokens, count, params, generator)
+            assert torch.equal(generator.get_state(), before), (type(engine).__name__, tokens, count)
+        assert engine.sample(0, [1], 0, params, generator) == [] and torch.equal(generator.get_state(), before)
