@@ -90,7 +90,7 @@ twm_status twm_cache8_attention(const twm_cache8* cache, const twm_cache8_attent
  *   top_p   of these the shortest head of the order that holds top_p of their sum of w (>= 1: all; the first one always);
  *   min_p   of these the ones with w >= min_p (<= 0: all; values over 1 count as 1).
  * The token is the first index, rising, at which the running sum of the kept w exceeds random * their sum; prob is its w over
- * that sum.  temperature 0 (or not > 0): the first largest logit.  A NaN logit counts as -inf; a row without any other gives
+ * that sum.  temperature 0 (or not > 0): the first largest logit; +inf: all finite logits weigh the same.  A NaN logit counts as -inf; a row without any other gives
  * token 0.  Sums do not depend on an order: the same call gives the same token. */
 typedef struct twm_sample_args {
     int rows, vocab;             /* vocab: at most 2^20 */

@@ -219,8 +219,8 @@ sample_kernel(const __grid_constant__ twm_sample_args a, int slice, int ctas)
             a.len[0] += 1;
         }
     };
-    // the lowest key that min_p keeps
-    auto least_key = [&]() { return mp > 0.0f ? order_of(__double2float_ru((double)mx + (double)t * log(fmin((double)mp, 1.0))) + 0.0f) : 0u; };
+    // the lowest key that min_p keeps; at an infinite temperature all finite logits weigh 1, and the others nothing
+    auto least_key = [&]() { return mp > 0.0f && t < INFINITY ? order_of(__double2float_ru((double)mx + (double)t * log(fmin((double)mp, 1.0))) + 0.0f) : 0u; };
 
     uint32_t cut = 0, ties = 0x7fffffffu;                // kept: keys over cut, and the first `ties` of those that are cut
     Weights weights = {mx, 0.0f, 0.0f};

@@ -261,3 +261,21 @@ def test_many_equal_numbers_at_the_border_of_top_k(vocab, dtype):
     for t in got:
         sampling.sample(logits, u, t, top_k=top_k, top_p=top_p)
     assert all(torch.equal(t, want) for t in got)
+
+
+@pytest.mark.parametrize("vocab", [5, 3000, 152064])
+def test_infinite_temperature(vocab):
+    """All finite logits weigh the same, whatever cut is asked for, and the loop's counters advance."""
+    cuts = [dict(), dict(min_p=1.0), dict(min_p=0.5), dict(min_p=3.0), dict(top_k=3), dict(top_k=1000, min_p=1.0), dict(top_p=0.3), dict(top_p=0.9, min_p=1.0),
+            dict(top_k=200, top_p=0.5, min_p=0.1)]
+    logits = 5 * torch.randn((len(cuts), vocab), generator=gen("inf", vocab), device="cuda")
+    logits[:, 1], logits[:, 3] = -math.inf, math.nan
+    for u in (0.0, 0.37, 0.999):
+        verify(logits, f32([u] * len(cuts)), f32([math.inf] * len(cuts)), i32([c.get("top_k", 0) for c in cuts]), f32([c.get("top_p", 1.0) for c in cuts]),
+               f32([c.get("min_p", 0.0) for c in cuts]))
+    tokens, step, pos, length = (torch.full((1,), v, dtype=torch.int32, device="cuda") for v in (-1, 0, 7, 8))
+    u, t, m = f32([0.5]), f32([math.inf]), f32([1.0])
+    args = _lib.SampleArgs(1, vocab, _lib.TWM_F32, logits.data_ptr(), vocab, u.data_ptr(), t.data_ptr(), None, None, m.data_ptr(), tokens.data_ptr(), None, step.data_ptr(),
+                           1, None, 0, pos.data_ptr(), length.data_ptr())
+    _lib.check(_lib.lib().twm_sample(_lib.C.addressof(args), 0, torch.cuda.current_stream().cuda_stream), "twm_sample")
+    assert int(tokens) >= 0 and int(step) == 1 and int(pos) == 8 and int(length) == 9
