@@ -45,7 +45,7 @@ typedef struct twm_cache8 {
 /* Bias and rotate-half RoPE on q and k, bias on v, k and v appended; qkv is the fused QKV output [rows][q | k | v] (f16, row
  * stride ldqkv), q_out the rotated queries [rows][q] (f16, row stride ldq).  rope_table: f32 [capacity][head_dim], cosines then
  * sines of every position, or NULL for none; bias: f32 [q | k | v] or NULL.  What twm_rope_append is to the FP16 cache.
- * q_out may be the q columns of qkv themselves.  Pointers on 16 bytes, row strides multiples of 8. */
+ * q_out may be the q columns of qkv themselves, and overlaps qkv in no other way (refused).  Pointers on 16 bytes, row strides multiples of 8. */
 typedef struct twm_cache8_append_args {
     void* q_out;
     long ldq;
@@ -66,7 +66,7 @@ size_t twm_cache8_attention_bytes(const twm_cache8* cache, int num_heads, int ma
 /* Softmax attention of the rows of a call over the cache, which already holds their own keys and values: the row at position p
  * sees the keys j <= p with p - j < window (window 0: all).  A sequence taken out of the call gets zeros.
  * out and q: f16 [rows][num_heads * head_dim], row strides ldo and ldq; query head h reads key/value head
- * h / (num_heads / kv_heads); scale is positive.  out must not overlap q.  Pointers on 16 bytes, row strides multiples of 8.
+ * h / (num_heads / kv_heads); scale is positive.  out must not overlap q (refused).  Pointers on 16 bytes, row strides multiples of 8.
  * Calls that share a workspace must not overlap. */
 typedef struct twm_cache8_attention_args {
     void* out;

@@ -110,7 +110,7 @@ def append(cache: Cache8, qkv: torch.Tensor, q_out: torch.Tensor, start: torch.T
     """qkv f16 [rows, (num_heads + 2 kv_heads) * head_dim]: queries out, rotated, to q_out [rows, num_heads * head_dim]; keys, rotated, and
     values to the cache.  start int32 [seqs]: tokens of each sequence before the call (< 0: not in the call); row_start int32
     [seqs + 1]: its rows among the call's, at most `max_rows` (None: one row a sequence).  rope: ``rope_table`` of the cache's capacity;
-    bias f32 of a whole row.  q_out may be the columns of the queries in qkv; a call without rows (row_start of zeros) does nothing."""
+    bias f32 of a whole row.  q_out may be the columns of the queries in qkv, else it must not overlap them; a call without rows (row_start of zeros) does nothing."""
     # Once per layer and token, and as long as the call itself takes: sizes and strides are read at once, and the arguments packed by struct.
     d, index, f16 = cache.head_dim, cache.index, torch.float16
     columns, out_columns = (num_heads + 2 * cache.kv_heads) * d, num_heads * d
@@ -144,8 +144,8 @@ def attention(cache: Cache8, q: torch.Tensor, out: torch.Tensor, start: torch.Te
               stream: Optional[torch.cuda.Stream] = None, flags: int = 0) -> None:
     """Causal softmax attention of q f16 [rows, num_heads * head_dim] over the cache, which holds the rows' own keys and values already
     (``append`` with the same start and row_start); out like q.  scale: 1/sqrt(head_dim) if None; window: how many of the newest keys
-    a row sees (0: all).  workspace: ``Workspace.for_cache``; without one the call makes its own.  out must not overlap q; a call
-    without rows (row_start of zeros) does nothing."""
+    a row sees (0: all).  workspace: ``Workspace.for_cache``; without one the call makes its own.  out must not overlap q (refused); a
+    call without rows (row_start of zeros) does nothing."""
     d, index, f16 = cache.head_dim, cache.index, torch.float16
     columns = num_heads * d
     size, ld, out_size, out_ld = q.size(), q.stride(), out.size(), out.stride()

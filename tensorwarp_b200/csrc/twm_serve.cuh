@@ -28,6 +28,20 @@ twm_status check_cache8(const twm_cache8* c, int num_heads, int rows, const int*
     if (off16(c->k) || off16(c->v) || off16(c->k_tail) || off16(c->v_tail)) return TWM_EALIGN;
     return TWM_OK;
 }
+// Whether two lots of FP16 rows, of `wa` and `wb` numbers, have memory in common.  Columns of one buffer have none, though they lie in one another's range.
+bool rows_overlap(const void* a, long lda, long wa, const void* b, long ldb, long wb, int rows)
+{
+    typedef long long ll;
+    const ll x0 = (ll)reinterpret_cast<uintptr_t>(a), y0 = (ll)reinterpret_cast<uintptr_t>(b), sx = 2 * (ll)lda, sy = 2 * (ll)ldb, nx = 2 * (ll)wa, ny = 2 * (ll)wb;
+    if (x0 + (rows - 1) * sx + nx <= y0 || y0 + (rows - 1) * sy + ny <= x0) return false;
+    // of equal strides the first and the last row show what all others do
+    for (ll i = 0; i < rows; i += lda == ldb ? std::max(rows - 1, 1) : 1) {
+        const ll x = x0 + i * sx, behind = x - ny - y0;                  // the first of b's rows that ends behind x
+        const ll j = behind < 0 ? 0 : behind / sy + 1;
+        if (j < rows && y0 + j * sy < x + nx) return true;
+    }
+    return false;
+}
 twm::cache8::Cache device_cache(const twm_cache8* c)
 {
     return {c->seqs, c->kv_heads, c->capacity, (uint8_t*)c->k, (uint8_t*)c->v, c->k_scale, c->v_scale, (__half*)c->k_tail, (__half*)c->v_tail};
@@ -122,6 +136,9 @@ twm_status twm_cache8_append(const twm_cache8* cache, const twm_cache8_append_ar
         return TWM_EINVAL;
     if (st != TWM_OK) return st;
     if (off16(x->q_out) || off16(x->qkv) || off16(x->bias) || off16(x->rope_table) || (x->ldq & 7) || (x->ldqkv & 7)) return TWM_EALIGN;
+    if (!(x->q_out == x->qkv && (x->ldq == x->ldqkv || x->rows == 1)) &&
+        rows_overlap(x->q_out, x->ldq, (long)x->num_heads * cache->head_dim, x->qkv, x->ldqkv, (long)(x->num_heads + 2 * cache->kv_heads) * cache->head_dim, x->rows))
+        return TWM_EINVAL;
     if ((st = ensure_device(nullptr)) != TWM_OK) return st;
     const twm::cache8::AppendArgs a = {device_cache(cache), {x->row_start, x->start, x->rows, x->max_rows}, (__half*)x->q_out, (const __half*)x->qkv, x->bias,
                                        x->rope_table, x->ldq, x->ldqkv, x->num_heads, x->max_rows >= TWM_CACHE8_BLOCK / 4 ? 1 : 0};
@@ -149,6 +166,7 @@ twm_status twm_cache8_attention(const twm_cache8* cache, const twm_cache8_attent
         return TWM_EINVAL;
     if (st != TWM_OK) return st;
     if (off16(x->out) || off16(x->q) || off16(x->workspace) || (x->ldo & 7) || (x->ldq & 7)) return TWM_EALIGN;
+    if (rows_overlap(x->out, x->ldo, (long)x->num_heads * D, x->q, x->ldq, (long)x->num_heads * D, x->rows)) return TWM_EINVAL;
     if (x->workspace_bytes < twm_cache8_attention_bytes(cache, x->num_heads, x->max_rows)) return TWM_EWORKSPACE;
     if ((st = ensure_device(nullptr)) != TWM_OK) return st;
     const AttnPlan p = plan_attention(x->num_heads / cache->kv_heads, x->max_rows, D);

@@ -189,3 +189,21 @@ def test_refused_calls_draw_no_random_numbers():
                 engine.sample(0, tokens, count, params, generator)
             assert torch.equal(generator.get_state(), before), (type(engine).__name__, tokens, count)
         assert engine.sample(0, [1], 0, params, generator) == [] and torch.equal(generator.get_state(), before)
+
+
+def test_rows_over_one_another_are_refused(twm_lib):
+    """Results over what is still to be read: the same rows, shifted ones, and rows of other strides that meet somewhere; columns of one buffer do not."""
+    base, ws = 0x1000000, 0x9000000
+    def attend(out, ldo, q, ldq, rows=6):
+        # a workspace that is too small: what is not refused for its rows is for that
+        return attention(twm_lib, cache(seqs=rows), out=base + 2 * out, ldo=ldo, q=base + 2 * q, ldq=ldq, rows=rows, ws=ws, nbytes=8)
+    for args in ((0, 1024, 0, 1024), (0, 1024, 1016, 1024), (8, 1024, 0, 1024), (0, 1024, 5 * 1024, 1024), (6 * 1024 - 8, 1024, 0, 1024), (0, 2048, 1016, 2048), (1032, 2048, 0, 2048),
+                 (0, 2048, 1016 + 2048 * 3, 2048), (0, 2048, 1024, 3080), (4000, 1024, 0, 4096), (0, 1024, 0, 1024, 1), (0, 9000, 1016, 7000, 1)):
+        assert attend(*args) == attend(args[2], args[3], args[0], args[1], *args[4:]) == _lib.TWM_EINVAL, args
+    for args in ((0, 2048, 1024, 2048), (0, 2048, 1024 + 2048, 2048), (0, 1024, 6 * 1024, 1024), (0, 2048, 1024, 4096), (0, 1024, 1024, 1024, 1), (0, 4096, 1024, 8192),
+                 (0, 2056, 1024, 2056)):
+        assert attend(*args) == attend(args[2], args[3], args[0], args[1], *args[4:]) == _lib.TWM_EWORKSPACE, args
+    # q_out among qkv's columns, of queries, keys and values: the queries' own or none
+    append_at = lambda q, ldq, rows=6: append(twm_lib, cache(seqs=rows), q=base + 2 * q, ldq=ldq, qkv=base, ldqkv=3080, rows=rows)  # noqa: E731
+    for args in ((8, 3080), (1024, 3080), (3080, 3080), (2040, 3080), (0, 1024), (0, 3088), (16, 1024, 1)):
+        assert append_at(*args) == _lib.TWM_EINVAL, args
