@@ -14,7 +14,7 @@
  * appending there next.
  *
  * The rows of a call.  Sequence s of the cache has the rows row_start[s] <= r < row_start[s + 1] of the call (device
- * array of seqs + 1; NULL: one row each, rows == seqs), `max_rows` of them at most; its first row is at position start[s]
+ * array of seqs + 1; NULL: one row each, rows == seqs and max_rows == 1), `max_rows` of them at most (1 <= max_rows <= rows); its first row is at position start[s]
  * (device array of seqs), which is the number of tokens cached before the step.  start[s] < 0 takes the sequence out of the call.
  * Rows behind row_start[seqs], and rows at positions past the capacity, are left as they were.
  */

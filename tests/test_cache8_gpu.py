@@ -542,3 +542,21 @@ def test_equal_weights_of_small_values(heads, kv_heads, dim, rows, size, where):
     b.append([0], [length])
     for window in (0, 300):
         verify_copies(b, length, rows, window, 1.0, 400 if rows < 9 else 40)
+
+
+@pytest.mark.parametrize("rows,most", [(1, 2), (3, 40), (20, 64)])
+def test_room_for_more_rows_than_the_call_has(rows, most):
+    """max_rows, and a workspace for as many, above the call's rows: what a program keeps for its largest calls serves the small ones."""
+    b = Batch(1, 256, 8, 2, 128)
+    b.append([0], [130])
+    ws = cache8.Workspace.for_cache(b.cache, 8, most)
+    qkv = b.make(rows).half()
+    q, out = torch.zeros((rows, 1024), dtype=torch.float16, device="cuda"), torch.zeros((rows, 1024), dtype=torch.float16, device="cuda")
+    kw = dict(num_heads=8, row_start=ints([0, rows]), max_rows=most)
+    cache8.append(b.cache, qkv, q, ints([130]), bias=b.bias, rope=b.rope, **kw)
+    qs, k, v = ref.project(qkv, torch.arange(130, 130 + rows, device="cuda"), 8, 2, 128, b.bias, b.rope)
+    b.held.append(0, 130, k, v)
+    b.held.check(b.cache)
+    cache8.attention(b.cache, q, out, ints([130]), workspace=ws, **kw)
+    want, off = ref.attention(qs, *b.held.held(0, 130 + rows), 130, 8, 1 / math.sqrt(128), 0)
+    assert torch.equal(q, qs) and bool(((out.double() - want).abs() <= off).all())

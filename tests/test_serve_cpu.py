@@ -207,3 +207,11 @@ def test_rows_over_one_another_are_refused(twm_lib):
     append_at = lambda q, ldq, rows=6: append(twm_lib, cache(seqs=rows), q=base + 2 * q, ldq=ldq, qkv=base, ldqkv=3080, rows=rows)  # noqa: E731
     for args in ((8, 3080), (1024, 3080), (3080, 3080), (2040, 3080), (0, 1024), (0, 3088), (16, 1024, 1)):
         assert append_at(*args) == _lib.TWM_EINVAL, args
+
+
+def test_a_larger_workspace_serves_fewer_rows(twm_lib):
+    """What is enough for `max_rows` rows a sequence is enough for fewer."""
+    for head_dim in (64, 128):
+        for heads in (4, 8, 12, 20, 28, 64, 284):
+            sizes = [twm_lib.twm_cache8_attention_bytes(C.addressof(cache(head_dim=head_dim)), heads, n) for n in range(1, 200)]
+            assert sizes == sorted(sizes)
