@@ -134,7 +134,8 @@ def append(cache: Cache8, qkv: torch.Tensor, q_out: torch.Tensor, start: torch.T
         with torch.cuda.device(index):
             return append(cache, qkv, q_out, start, num_heads=num_heads, row_start=row_start, max_rows=max_rows, bias=bias, rope=rope, stream=stream, flags=flags)
     rows = size[0]
-    args = _lib.pack_append_args(q_out.data_ptr(), out_ld[0], qkv.data_ptr(), ld[0], bias_at, rope_at, num_heads, rows, min(max_rows, rows) if at else max_rows, at,
+    q_ld, qkv_ld = (out_ld[0], ld[0]) if rows > 1 else (out_columns, columns)                # the stride of a single row says nothing
+    args = _lib.pack_append_args(q_out.data_ptr(), q_ld, qkv.data_ptr(), qkv_ld, bias_at, rope_at, num_heads, rows, min(max_rows, rows) if at else max_rows, at,
                                  start.data_ptr())
     status = _lib.lib().twm_cache8_append(cache._ref, args, flags, _stream_ptr(stream))
     if status:
@@ -167,7 +168,8 @@ def attention(cache: Cache8, q: torch.Tensor, out: torch.Tensor, start: torch.Te
     elif workspace.index != index:
         raise TwmError(_lib.TWM_EINVAL, "attention: the workspace is on another device")
     rows = size[0]
-    args = _lib.pack_attention_args(out.data_ptr(), out_ld[0], q.data_ptr(), ld[0], num_heads, rows, min(max_rows, rows) if at else max_rows, window, at,
+    o_ld, q_ld = (out_ld[0], ld[0]) if rows > 1 else (columns, columns)                      # the stride of a single row says nothing
+    args = _lib.pack_attention_args(out.data_ptr(), o_ld, q.data_ptr(), q_ld, num_heads, rows, min(max_rows, rows) if at else max_rows, window, at,
                                     start.data_ptr(), workspace.ptr, workspace.nbytes, 1.0 / math.sqrt(d) if scale is None else scale)
     status = _lib.lib().twm_cache8_attention(cache._ref, args, flags, _stream_ptr(stream))
     if status:

@@ -560,3 +560,21 @@ def test_room_for_more_rows_than_the_call_has(rows, most):
     cache8.attention(b.cache, q, out, ints([130]), workspace=ws, **kw)
     want, off = ref.attention(qs, *b.held.held(0, 130 + rows), 130, 8, 1 / math.sqrt(128), 0)
     assert torch.equal(q, qs) and bool(((out.double() - want).abs() <= off).all())
+
+
+def test_single_rows_of_any_stride():
+    """One row has no next one: a transposed column, and a row of a buffer whose width is odd."""
+    b = Batch(1, 128, 8, 2, 128)
+    b.append([0], [70])
+    columns = b.make(1).half()[0]
+    qs, k, v = ref.project(columns[None], torch.tensor([70], device="cuda"), 8, 2, 128, b.bias, b.rope)
+    b.held.append(0, 70, k, v)
+    want, off = ref.attention(qs, *b.held.held(0, 71), 70, 8, 1 / math.sqrt(128), 0)
+    for place in (lambda n: torch.zeros((n, 1), dtype=torch.float16, device="cuda").t(), lambda n: torch.zeros((1, n + 3), dtype=torch.float16, device="cuda")[:, :n]):
+        qkv, q, out = place(b.width), place(1024), place(1024)
+        qkv.copy_(columns[None])
+        assert qkv.stride(0) not in (b.width,) and qkv.stride(1) == 1
+        cache8.append(b.cache, qkv, q, ints([70]), num_heads=8, bias=b.bias, rope=b.rope)
+        b.held.check(b.cache)
+        cache8.attention(b.cache, q, out, ints([70]), num_heads=8)
+        assert torch.equal(q, qs) and bool(((out.double() - want).abs() <= off).all())
