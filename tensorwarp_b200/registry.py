@@ -7,6 +7,7 @@ step interface of ``engine.StepEngine``.
 from __future__ import annotations
 
 import importlib
+import inspect
 import os
 from typing import Callable, Dict, Optional
 
@@ -44,6 +45,8 @@ def load(folder: str, **options):
     """An engine for the checkpoint in `folder` (options: dtype, max_tokens, max_live, portion, device; kv_cache of the 4-bit decoder)."""
     config = checkpoint.read_config(folder)
     builder = builder_for(config)
+    if "kv_cache" in options and "kv_cache" not in inspect.signature(builder).parameters:
+        raise ValueError(f"{config['architecture']} holds keys and values in its own type only: kv_cache is an option of the 4-bit decoder")
     path = os.path.join(folder, "model.safetensors")
     weights: Optional[checkpoint.SafetensorsFile] = checkpoint.SafetensorsFile(path) if os.path.exists(path) else None
     try:

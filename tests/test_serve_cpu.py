@@ -215,3 +215,19 @@ def test_a_larger_workspace_serves_fewer_rows(twm_lib):
         for heads in (4, 8, 12, 20, 28, 64, 284):
             sizes = [twm_lib.twm_cache8_attention_bytes(C.addressof(cache(head_dim=head_dim)), heads, n) for n in range(1, 200)]
             assert sizes == sorted(sizes)
+
+
+@pytest.mark.parametrize("architecture", ["Bidasun", "Zukotar"])
+def test_the_8_bit_cache_is_refused_where_there_is_none(tmp_path, architecture):
+    """The option's name is in the error, ahead of any weights; the 4-bit decoder's builder takes it."""
+    import inspect
+
+    from tensorwarp_b200 import registry
+    from tensorwarp_b200.__main__ import main
+    (tmp_path / "config.json").write_text('{"architecture": "%s"}' % architecture)
+    for kind in ("e4m3", "f16"):
+        with pytest.raises(ValueError, match="kv_cache is an option of the 4-bit decoder"):
+            registry.load(str(tmp_path), kv_cache=kind)
+        with pytest.raises(ValueError, match="kv_cache is an option of the 4-bit decoder"):
+            main(["generate", "--model", str(tmp_path), "--tokens", "1", "--kv-cache", kind])
+    assert "kv_cache" in inspect.signature(registry.builder_for({"architecture": "TWMarlinQ4"})).parameters
