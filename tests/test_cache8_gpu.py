@@ -578,3 +578,21 @@ def test_single_rows_of_any_stride():
         b.held.check(b.cache)
         cache8.attention(b.cache, q, out, ints([70]), num_heads=8)
         assert torch.equal(q, qs) and bool(((out.double() - want).abs() <= off).all())
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("first", ["zeros", "units of one"])
+def test_second_half_behind_a_tile_without_it(dim, first):
+    """280 rows a sequence, a tile of 256 and one of 24: the rows of the second half come to the next sequence's first block, whose scale is one, ahead
+    of its values."""
+    def make(n):
+        x = torch.zeros((n, 6, dim), device="cuda")
+        token = torch.arange(n, device="cuda")[:, None]
+        x[:, 4:5, 0] = torch.where(token < 64, 0.25, 0.0)
+        v = 1e-4 * (1 + torch.rand((n, 1, dim), generator=gen("half", n), device="cuda"))
+        x[:, 5:] = torch.where((token < 64)[:, :, None], 0.0 if first == "zeros" else 230.0, v)
+        return x.flatten(1)
+    b = Batch(1, 512, 4, 1, dim, bias=False, rope=False, make=make)
+    b.append([0], [448])
+    for _ in range(3):
+        verify_copies(b, 448, 70, 0, 1.0, 300)
