@@ -106,7 +106,9 @@ struct AppendArgs {
 // from the tail) for the largest value, then rounded; the two newest blocks go to the tail.  A call may begin inside a block whose
 // earlier tokens are read from a half of the tail that the call's last block takes over: both are then the work of the CTA of the
 // first block, in that order.  Of a token or a few every thread has one item, so that all loads are on their way at once.  Prompts are
-// bound by memory and take a CTA for every query head of a block as well (4000 tokens, 28 heads: 29 us without, 23 us with).
+// bound by memory and take a CTA for every query head of a block as well (4000 tokens, 28 heads: 29 us without, 23 us with), from a quarter of a block
+// on: there it gains for few sequences and costs for many, which from half a block on gain too (40 heads on 8, us without and with: 8 rows of 1, 8 and
+// 64 sequences 4.9 and 3.6, 5.1 and 4.3, 10.2 and 14.6; 16 rows 5.7 and 3.8, 5.9 and 4.7, 13.2 and 16.2; 32 rows 7.4 and 4.1, 7.6 and 5.1, 24.3 and 23.7).
 constexpr int APPEND_THREADS = 256;
 template <int D>
 __global__ void __launch_bounds__(APPEND_THREADS)

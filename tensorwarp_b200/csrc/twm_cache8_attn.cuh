@@ -289,7 +289,8 @@ constexpr int NO_VALUES = -64;
 // read once.  Bound by HBM (96 sequences of up to 6000 tokens, 40 heads on 8: 119 us, 6.18 TB/s).  Four consumer warps take 16 keys each of a
 // unit; a producer warp brings units by TMA into a ring that runs on over the borders of tiles, the tail's FP16 rows among them (keys and
 // values in a stage each).  S^T = K Q^T and O^T += V^T P^T as mma.m16n8k16 with the keys, and then the head's elements, as the 16 rows, so that eight
-// rows of queries are a whole operand.  Elements and keys may stand in any order in a sum: lane (g, t) takes D / 4 elements of keys g and g + 8 for
+// rows of queries are a whole operand (with NT = 2 and D = 128 registers do not reach: 434 bytes of them are stored, and 96 sequences of 4000 tokens, 40
+// heads on 8, take 257 us with two new tokens each, 125 with one).  Elements and keys may stand in any order in a sum: lane (g, t) takes D / 4 elements of keys g and g + 8 for
 // the scores (4 codes a k-step of both registers), and D / 8 elements of four keys for the output, whose codes are paired by a byte permutation; at
 // D = 128 both reads are free of bank conflicts in the layout that the TMA's swizzle leaves.  P^T needs only a transposition of 8 x 8.  Each warp has
 // its own m; when the tile ends the four add up in shared memory, while the next tile's queries are on their way.

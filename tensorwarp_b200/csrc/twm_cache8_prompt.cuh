@@ -12,7 +12,9 @@
 // Tensor memory: two score buffers of 64 columns and D of output for each half; the factors, FP16, overwrite the scores.
 // Sharing a unit between two halves is what shared memory asks for: a unit costs 16 KB read and 32 KB written by the conversion and 64 KB read by
 // each half's MMAs, 1400 clocks at 128 bytes each for 256 rows against 1024 of MMA and 1024 of exponentials; with 128 rows it would be 1800.
-// A prompt of 4000 tokens of 28 heads takes 153 us, 748 TFLOP/s, about 2400 clocks a unit: what a unit's softmax takes with two warps a scheduler.
+// A prompt of 4000 tokens of 28 heads takes 153 us, 748 TFLOP/s, about 2400 clocks a unit.  What bounds that is not settled: without exponentials it takes
+// 151 us, without the conversion 145, without the scores' MMAs 152, without all three 109, which is more than the products and the loads
+// need.  All fourteen warps have 128 registers a thread, and the rows' (D = 128) store 72 bytes of them.
 // Both halves' scores first and both halves' products then took 159 us; sixteen warps, half a row each, 174.
 #pragma once
 

@@ -48,6 +48,10 @@ twm::cache8::Cache device_cache(const twm_cache8* c)
 }
 
 // How attention is launched: the rows of a tile, how many of them there can be, and the CTAs of the grid, whatever the lengths (which are on the device).
+// Up to 16 rows the kernel for few is the faster one, though it spills with more than 8 of heads of 128 (us, and those of the kernel for many: 96
+// sequences of 4000 tokens, 40 heads on 8, 10 rows 257 and 357, 15 rows 264 and 357; 16 heads on 1, 16 rows 52 and 60; one sequence of 2048, 14 rows
+// 13.7 and 16.6; 40 of 3000, heads of 64, 16 rows 50 and 104).  It has no form for more; the other takes 361 us for 20 rows of the first batch, and
+// 71 us (1.9 TB/s) for 64 sequences of 8000 tokens with 71 heads on 1.
 struct AttnPlan { int tile, rows, ctas; };
 AttnPlan plan_attention(int group, int max_rows, int head_dim)
 {

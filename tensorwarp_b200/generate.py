@@ -150,7 +150,9 @@ class QuantizedGenerationEngine:
     """Decode engine on TW-Marlin weights (generate.rs:1191-2547, Q4 + marlin + graph path)."""
 
     def __init__(self, model: Q4Model, use_pdl: bool = True, q4_lm_head: bool = False, kv_cache: str = "f16"):
-        """kv_cache: "f16", or "e4m3" for keys and values held in 8 bits (half the memory; ``cache8``)."""
+        """kv_cache: "f16", or "e4m3" for keys and values held in 8 bits (``cache8``): half the memory, any length, heads of 64 too.  A token takes
+        three launches a layer where "f16" takes two, so that it gains time on long contexts only (28 layers, 28 heads on 4: 1761 us on 2048 tokens, "f16"
+        1725; on 32640 tokens 1948 and 2207)."""
         if kv_cache not in ("f16", "e4m3"):
             raise _lib.TwmError(_lib.TWM_EINVAL, f"QuantizedGenerationEngine: kv_cache {kv_cache!r} is neither 'f16' nor 'e4m3'")
         if kv_cache == "e4m3" and model.cfg.head_dim not in (64, 128):
