@@ -450,7 +450,7 @@ sample_kernel(const __grid_constant__ twm_sample_args a, int slice, int ctas)
                     });
                     join();
                     const uint32_t x = sh.all_count[tid];
-                    const double y = (double)w_top * ((double)x - (double)sh.all_delta[tid] * unit);
+                    const double y = bin < BINS ? (double)w_top * ((double)x - (double)sh.all_delta[tid] * unit) : 0.0;
                     find(over, over_mass, x, y, scan(sh, x, y), 0);
                     const uint32_t b = sh.found_bin;
                     left = sh.found_count;

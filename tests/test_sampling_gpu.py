@@ -279,3 +279,17 @@ def test_infinite_temperature(vocab):
                            1, None, 0, pos.data_ptr(), length.data_ptr())
     _lib.check(_lib.lib().twm_sample(_lib.C.addressof(args), 0, torch.cuda.current_stream().cuda_stream), "twm_sample")
     assert int(tokens) >= 0 and int(step) == 1 and int(pos) == 8 and int(length) == 9
+
+
+@pytest.mark.parametrize("vocab", [50, 3000, 18169, 152064])
+def test_tokens_without_weight_do_not_move_a_border(vocab):
+    """Two equal logits far above all others: at a half of the mass top-p keeps the first one, whatever top-k leaves beside them."""
+    ks = [0, 2, vocab // 2, vocab - 1, vocab]
+    logits = torch.round(torch.randn((len(ks), vocab), generator=gen("weight", vocab), device="cuda").clamp(-2, 2))
+    first, second = vocab // 3, vocab - 2
+    logits[:, first] = logits[:, second] = 4.0
+    for u in (0.1, 0.9):
+        for p, want, share in ((0.5, first, 1.0), (0.75, first if u < 0.5 else second, 0.5)):
+            tokens, prob = torch.zeros(len(ks), dtype=torch.int32, device="cuda"), torch.zeros(len(ks), device="cuda")
+            sampling.sample(logits, f32([u] * len(ks)), tokens, temperature=f32([1e-4] * len(ks)), top_k=i32(ks), top_p=f32([p] * len(ks)), prob=prob)
+            assert tokens.tolist() == [want] * len(ks) and prob.tolist() == [share] * len(ks), (u, p)
